@@ -38,6 +38,7 @@ extern "C" {
 const char* ng_last_error(void);
 int ng_init(int device);
 int ng_device_count(int* count);
+int ng_current_device(int* device);            /* of this thread */
 int ng_sm_count(int* count);
 int ng_malloc(void** ptr, size_t bytes);
 int ng_free(void* ptr);
@@ -225,6 +226,58 @@ int ng_pool_argmax_bytes(const ng_pool_desc* desc, int dtype_bytes, size_t* byte
 int ng_pool_fprop_argmax(const ng_pool_desc* desc, int dtype_bytes, const void* I, void* O, void* argmax, void* stream);
 int ng_pool_bprop_argmax(const ng_pool_desc* desc, int dtype_bytes, const void* argmax, const void* E, void* gradI,
                          int relu_mask, void* stream);
+
+/* ---- matrices in blocks of small floating-point numbers ------------------------------------------
+ * A matrix of rows x cols numbers, stored in runs of 16 or 32 neighbours along one axis that share a
+ * scale. Formats:
+ *   NG_BLOCK_MXFP4  4-bit numbers (E2M1, up to 6), blocks of 32, scale a power of two (E8M0)
+ *   NG_BLOCK_NVFP4  4-bit numbers, blocks of 16, scale an E4M3 number times `scale`, one power of two for
+ *                   the matrix (2^-64 .. 2^64)
+ *   NG_BLOCK_MXFP8  8-bit numbers (E4M3, up to 448), blocks of 32, scale a power of two; a number that is not
+ *                   zero never becomes zero
+ * A power-of-two scale is the smallest that brings the block's largest magnitude within the format; an
+ * nvfp4 scale is RN_E4M3(largest / 6 / scale), kept from 2^-9 to 448. Numbers are rounded to nearest, ties to
+ * even, and limited to the largest. A block that holds an infinity or NaN reads back as NaN.
+ * axis: 1 = blocks run along the rows (neighbouring columns), 0 = down the columns.
+ * codes, scales: device memory of ng_block_bytes() bytes each, 128-byte aligned, zeroed when it is allocated
+ * (the padding of rows and tiles has to be zero; no call writes it) and laid out for one axis and format.
+ * device: the CUDA device that holds them; calls on another current device are refused.
+ * The reference has nothing like these: its low-precision storage is fp16 (nervanagpu/nervanagpu.py:469-520). */
+#define NG_BLOCK_MXFP4 0
+#define NG_BLOCK_NVFP4 1
+#define NG_BLOCK_MXFP8 2
+typedef struct ng_block_desc {
+  int format, axis;
+  int rows, cols;
+  int device;
+  float scale;           /* nvfp4; 1 for the others */
+  void* codes;
+  void* scales;
+} ng_block_desc;
+
+int ng_block_bytes(const ng_block_desc* desc, size_t* codes_bytes, size_t* scales_bytes);
+/* Every element of A (rows x cols, fp16 or fp32, element (r, c) at r * row_stride + c * col_stride elements) into
+ * the n_outs (1 to 4) matrices in blocks, all of A's shape. */
+int ng_block_quantize(const void* A, int dtype_bytes, long long row_stride, long long col_stride,
+                      const ng_block_desc* outs, int n_outs, void* stream);
+/* The values that the codes stand for; where dtype_bytes is 2, rounded to fp16 and limited to +-65504. */
+int ng_block_dequantize(const ng_block_desc* q, void* out, int dtype_bytes, long long row_stride, long long col_stride,
+                        void* stream);
+/* E = q > 0 ? E : 0 in place, q in mxfp8: the mask of a ReLU whose output was put into q. */
+int ng_block_relu_mask(const ng_block_desc* q, void* E, int dtype_bytes, long long row_stride, long long col_stride,
+                       void* stream);
+/* C[m x n] = relu?(alpha * A * B) + beta * C, C row-major, fp16 or fp32 (out_f32), fp32 accumulation; rounding
+ * as in ng_hgemm. A is m x k with axis 1, B is k x n with axis 0: the blocks run along the sum. Both are in the
+ * same 4-bit format. (A matrix is its transpose with rows and cols exchanged and the other axis: the memory is the
+ * same.) */
+int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ldc, int out_f32, float alpha,
+                 float beta, int relu, int sr_bits, unsigned long long seed, unsigned int rng_offset, void* stream);
+/* The same with A an m x k fp16 matrix (leading dimension lda) and B in mxfp8: the weight gradient of a
+ * fully-connected layer, from its deltas and the 8-bit record of its input. The record's values are taken as
+ * fp16, limited to +-65504; all others are exact when the record was made from fp16 numbers. */
+int ng_block_dot_f16(const void* A, int lda, const ng_block_desc* B, void* C, int m, int ldc, int out_f32, float alpha,
+                     float beta, int relu, int sr_bits, unsigned long long seed, unsigned int rng_offset,
+                     void* stream);
 
 /* ---- generated element-wise kernels -----------------------------------------------------------
  * Replace pycuda.compiler.SourceModule / Function.prepare / prepared_async_call for the CUDA-C

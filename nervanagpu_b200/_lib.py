@@ -39,11 +39,17 @@ class PoolDesc(ctypes.Structure):
                 "N C D H W J T R S pad_j pad_d pad_h pad_w str_j str_d str_h str_w".split()]
 
 
+class BlockDesc(ctypes.Structure):
+    _fields_ = [(n, c_int) for n in "format axis rows cols device".split()] + [
+        ("scale", c_float), ("codes", c_void_p), ("scales", c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/nervana_b200.h declares
 SIGNATURES = {
     "ng_last_error": (c_char_p, []),
     "ng_init": (c_int, [c_int]),
     "ng_device_count": (c_int, [ctypes.POINTER(c_int)]),
+    "ng_current_device": (c_int, [ctypes.POINTER(c_int)]),
     "ng_sm_count": (c_int, [ctypes.POINTER(c_int)]),
     "ng_malloc": (c_int, [ctypes.POINTER(c_void_p), c_size_t]),
     "ng_free": (c_int, [c_void_p]),
@@ -105,6 +111,14 @@ SIGNATURES = {
     "ng_pool_fprop_argmax": (c_int, [ctypes.POINTER(PoolDesc), c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "ng_pool_bprop_argmax": (c_int, [ctypes.POINTER(PoolDesc), c_int, c_void_p, c_void_p, c_void_p, c_int,
                                      c_void_p]),
+    "ng_block_bytes": (c_int, [ctypes.POINTER(BlockDesc), ctypes.POINTER(c_size_t), ctypes.POINTER(c_size_t)]),
+    "ng_block_quantize": (c_int, [c_void_p, c_int, c_longlong, c_longlong, ctypes.POINTER(BlockDesc), c_int, c_void_p]),
+    "ng_block_dequantize": (c_int, [ctypes.POINTER(BlockDesc), c_void_p, c_int, c_longlong, c_longlong, c_void_p]),
+    "ng_block_relu_mask": (c_int, [ctypes.POINTER(BlockDesc), c_void_p, c_int, c_longlong, c_longlong, c_void_p]),
+    "ng_block_dot": (c_int, [ctypes.POINTER(BlockDesc), ctypes.POINTER(BlockDesc), c_void_p, c_int, c_int, c_float,
+                             c_float, c_int, c_int, c_ulonglong, c_uint, c_void_p]),
+    "ng_block_dot_f16": (c_int, [c_void_p, c_int, ctypes.POINTER(BlockDesc), c_void_p, c_int, c_int, c_int, c_float,
+                                 c_float, c_int, c_int, c_ulonglong, c_uint, c_void_p]),
     "ng_ew_compile": (c_int, [c_char_p, c_char_p, c_int, ctypes.POINTER(c_void_p)]),
     "ng_ew_compile_only": (c_int, [c_char_p, c_int]),
     "ng_ew_compile_log": (c_char_p, []),

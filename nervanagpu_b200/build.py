@@ -13,7 +13,8 @@ LIB = os.path.join(HERE, "libnervana_b200.so")
 EXT = os.path.join(HERE, "_native.so")     # CPython module: the native half of the host path
 EXT_SOURCE = os.path.join(CSRC, "pyext.cpp")
 
-SOURCES = ["runtime.cu", "tc_host.cu", "gemm.cu", "conv.cu", "pool.cu", "ew_rt.cu", "legacy_api.cu", "comm.cu"]
+SOURCES = ["runtime.cu", "tc_host.cu", "gemm.cu", "conv.cu", "pool.cu", "ew_rt.cu", "legacy_api.cu", "comm.cu",
+           "blocks.cu", "block_dot.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,455 @@
+// Products of matrices in blocks of small floating-point numbers (the formats: blocks.cuh).
+//
+// 4-bit x 4-bit (block_dot_kernel): C = epilogue(sum_k A[i,k] B[k,j]) on tcgen05.mma.kind::mxf4nvf4, which takes the
+// packed codes from shared memory and the scales of both operands from tensor memory, multiplies each block's
+// products by its two scales and accumulates in fp32. Both operands lie along the sum in rows of 128-byte units, so
+// one TMA box of [rows][128 bytes] is a k-block of 256 numbers (four MMAs of 64), and its scales, laid out at
+// quantisation as tensor memory holds them, are one plain bulk copy into shared memory and one tcgen05.cp per 512
+// bytes from there.
+//
+// A CTA computes a tile of 128 rows x kN columns (kN from 16 to 256). Few tiles are split along the sum over the
+// CTAs of a thread-block cluster, which add their partial tiles up over distributed shared memory in the order of the
+// partitions: one launch, no scratch memory, the same bits every time.
+//
+//   warp 0     TMA producer
+//   warp 1     tensor memory, scale copies and MMAs, by one thread
+//   warps 2-5  tensor memory -> shared memory
+//   all        sum over the cluster, output stage (epilogue.cuh), stores
+#include <algorithm>
+
+#include "blocks.h"
+#include "epilogue.cuh"
+
+namespace ngb {
+
+namespace {
+
+constexpr uint32_t kCodesA = 128u * 128u;       // bytes of a k-block of A
+constexpr int kDotThreads = 192;
+constexpr uint32_t kDotSmemLimit = 232448;      // 227 KB
+constexpr uint32_t kDotCtrl = 256;              // barriers, tensor-memory address, abort flag
+constexpr int kDotStages = 8;                   // most
+
+// Everything that follows from the tile's columns and the format.
+template <int kN, bool kNv>
+struct DotTile {
+  static constexpr int kScaleTiles = kNv ? 4 : 2;            // 512-byte scale tiles per k-block and 128 rows
+  static constexpr int kRowTiles = (kN + 127) / 128;         // of B's scales
+  static constexpr uint32_t kCodesB = kN * 128u;
+  static constexpr uint32_t kScalesA = kScaleTiles * kScaleTile;
+  static constexpr uint32_t kStageBytes = (kCodesA + kCodesB + kScalesA * (1 + kRowTiles) + 1023u) & ~1023u;
+  static constexpr int kStages =
+      static_cast<int>((kDotSmemLimit - 1024u - kDotCtrl) / kStageBytes) < kDotStages ? static_cast<int>((kDotSmemLimit - 1024u - kDotCtrl) / kStageBytes) : kDotStages;
+  // tensor memory: the accumulator, then two buffers of scales, A's before B's
+  static constexpr int kAccCols = kN < 32 ? 32 : kN;
+  static constexpr int kScaleCols = kScaleTiles * 4 * (1 + kRowTiles);
+  static constexpr int kColsUsed = kAccCols + 2 * kScaleCols;
+  static constexpr uint32_t kCols = kColsUsed <= 128 ? 128 : (kColsUsed <= 256 ? 256 : 512);
+  // partial tiles in shared memory: rows of kN + 4 floats, so that lanes in successive rows meet different banks
+  static constexpr int kPitch = kN + 4;
+  static constexpr uint32_t kSmem = kStages * kStageBytes + 1024u + kDotCtrl;
+  static_assert(128u * kPitch * 4u <= kStages * kStageBytes, "the partial tile takes the ring's place");
+};
+
+struct DotParams {
+  int M, N;                  // rows of the two operands
+  int num_kb;
+  int tiles_m;
+  const uint8_t *sa, *sb;    // scales
+  long long spitch;          // bytes of a row of scale tiles (the same for both: one format, one length)
+  int sa_tiles, sb_tiles;    // rows of scale tiles that exist
+  uint32_t idesc;
+  void* C;
+  long long ldc;
+  int out_f32, vec_ok;
+  int swapped;               // the tile's rows are C's columns
+  EpiArgs ea;
+  int* status;
+  unsigned long long wait_limit_ns;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+// 32 rows of 16 bytes in shared memory to 4 columns of tensor memory, the same in each of the four groups of 32 lanes
+__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint32_t smem) {
+  const uint64_t desc = (static_cast<uint64_t>((128u >> 4) | (1u << 14)) << 32) | (1u << 16) | (smem >> 4);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <bool kNv>
+__device__ __forceinline__ void tc_mma_blocks(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                              uint32_t accumulate) {
+  if (kNv) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  }
+}
+__device__ __forceinline__ void tc_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ float4 load_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float load_cluster_f1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return n;
+}
+
+template <int kN, bool kNv>
+__global__ void __launch_bounds__(kDotThreads, 1)
+block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
+                 const __grid_constant__ DotParams p) {
+  using T = DotTile<kN, kNv>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t ctrl = ring + T::kStages * T::kStageBytes;
+  uint8_t* ring_gen = smem_raw + (ring - smem_u32(smem_raw));
+  auto full_bar = [&](int s) { return ctrl + 8u * s; };
+  auto empty_bar = [&](int s) { return ctrl + 8u * (kDotStages + s); };
+  const uint32_t acc_bar = ctrl + 8u * (2 * kDotStages);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_gen + T::kStages * T::kStageBytes + 8 * (2 * kDotStages + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t splits = cluster_size(), rank = cluster_cta_rank();
+  const int tile = blockIdx.x / splits;
+  const int m0 = (tile % p.tiles_m) * 128, n0 = (tile / p.tiles_m) * kN;
+  const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * rank / splits);
+  const int count = static_cast<int>(static_cast<long long>(p.num_kb) * (rank + 1) / splits) - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < T::kStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(acc_bar, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&mapA);
+    tma_prefetch_desc(&mapB);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), T::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const int rt = m0 / 128, ct = n0 / 128;
+      const int ct_live = min(T::kRowTiles, p.sb_tiles - ct);    // (the last column tile may reach beyond B's scales)
+      const uint32_t tx = kCodesA + T::kCodesB + T::kScalesA * (1 + ct_live);
+      int i = 0;
+      bool ok = true;
+      for (; i < count; ++i) {
+        const int s = i % T::kStages, lap = i / T::kStages;
+        if (lap > 0 && !mbar_wait(empty_bar(s), (lap - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns)) {
+          ok = false;
+          break;
+        }
+        const uint32_t a = ring + s * T::kStageBytes, b = a + kCodesA, sa = b + T::kCodesB, sb = sa + T::kScalesA;
+        const int kb = kb0 + i;
+        mbar_expect_tx(full_bar(s), tx);
+        tma_load_5d(a, &mapA, full_bar(s), kb * 64, m0, 0, 0, 0);
+        tma_load_5d(b, &mapB, full_bar(s), kb * 64, n0, 0, 0, 0);
+        const long long koff = static_cast<long long>(kb) * T::kScalesA;
+        bulk_load(sa, p.sa + rt * p.spitch + koff, T::kScalesA, full_bar(s));
+        for (int c = 0; c < ct_live; ++c) bulk_load(sb + c * T::kScalesA, p.sb + (ct + c) * p.spitch + koff, T::kScalesA, full_bar(s));
+      }
+      // given up: the loads in flight must land before the CTA may end
+      if (!ok) {
+        int none = 0;
+        for (int j = max(0, i - T::kStages); j < i; ++j)
+          mbar_wait(full_bar(j % T::kStages), (j / T::kStages) & 1, &none, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);     // 8 rows of 128 bytes apart, version 1, 128-byte swizzle
+      const uint32_t scales = tmem + T::kAccCols;
+      const uint32_t b_shift = static_cast<uint32_t>(n0 % 128) / 32u;   // columns of the scale tile before this tile's first
+      bool ok = true;
+      for (int i = 0; i < count; ++i) {
+        const int s = i % T::kStages;
+        if (!mbar_wait(full_bar(s), (i / T::kStages) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_MMA, p.wait_limit_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a = ring + s * T::kStageBytes, b = a + kCodesA, sa = b + T::kCodesB, sb = sa + T::kScalesA;
+        const uint32_t ta = scales + (i & 1) * T::kScaleCols, tb = ta + T::kScaleTiles * 4;
+#pragma unroll
+        for (int t = 0; t < T::kScaleTiles; ++t) {
+          tc_copy_scales(ta + t * 4, sa + t * kScaleTile);
+#pragma unroll
+          for (int c = 0; c < T::kRowTiles; ++c)
+            tc_copy_scales(tb + (t * T::kRowTiles + c) * 4, sb + c * T::kScalesA + t * kScaleTile);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t da = (static_cast<uint64_t>(hi) << 32) | (1u << 16) | ((a + 32u * j) >> 4);
+          const uint64_t db = (static_cast<uint64_t>(hi) << 32) | (1u << 16) | ((b + 32u * j) >> 4);
+          const int t = kNv ? j : j / 2;
+          const uint32_t id = kNv ? 0u : (j & 1) * 2u;       // which of the tile's four scales are this MMA's first
+          tc_mma_blocks<kNv>(tmem, da, db, p.idesc | (id << 4) | (id << 29), ta + t * 4, tb + t * T::kRowTiles * 4 + b_shift,
+                             (i | j) != 0);
+        }
+        tc_commit(empty_bar(s));
+      }
+      tc_commit(acc_bar);
+      if (!ok) {     // what was issued must end before tensor memory is given back
+        int none = 0;
+        mbar_wait(acc_bar, 0, &none, p.status, NG_DEV_TIMEOUT_MMA, p.wait_limit_ns);
+      }
+    }
+    __syncwarp();
+  } else {
+    const bool ok = mbar_wait(acc_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
+    if (ok && !*abort_flag) {
+      tc_fence_after();
+      const int group = warp & 3;
+      float* row = reinterpret_cast<float*>(ring_gen) + (group * 32 + lane) * T::kPitch;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(group * 32) << 16);
+      if constexpr (kN < 32) {
+        uint32_t r[16];
+        tc_ld_32x16(taddr, r);
+        tc_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) reinterpret_cast<uint4*>(row)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < kN; c += 32) {
+          uint32_t r[32];
+          tc_ld_32x32(taddr + c, r);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            reinterpret_cast<uint4*>(row + c)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, T::kCols);
+  }
+  if (splits > 1) cluster_sync_all();
+
+  // This CTA's share of the tile: 128 / splits rows, summed over the cluster.
+  // (a partition that gave up leaves the tile unwritten only in its own share: the status word tells)
+  if (!*abort_flag) {
+    const int rows = 128 / splits, r0 = static_cast<int>(rank) * rows;
+    auto finish = [&](float (&v)[8], long long row, int col, int ncols, int nvalid) {
+      // 8 neighbours of C's row `row` from column `col` on
+      const unsigned long long lin = static_cast<unsigned long long>(row) * ncols + col;
+      uint8_t* crow = static_cast<uint8_t*>(p.C) + row * p.ldc * (p.out_f32 ? 4 : 2);
+      if (p.out_f32) epi_store8<true>(p.ea, v, crow, crow, col, lin, nvalid, p.vec_ok != 0);
+      else epi_store8<false>(p.ea, v, crow, crow, col, lin, nvalid, p.vec_ok != 0);
+    };
+    if (!p.swapped) {
+      for (int i = threadIdx.x; i < rows * (kN / 8); i += kDotThreads) {
+        const int r = r0 + i / (kN / 8), c = (i % (kN / 8)) * 8;
+        const int row = m0 + r, col = n0 + c;
+        if (row >= p.M || col >= p.N) continue;
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        const uint32_t at = ring + (r * T::kPitch + c) * 4u;
+        for (uint32_t s = 0; s < splits; ++s) {
+          const uint32_t src = map_to_cta(at, s);
+          const float4 x = load_cluster_f4(src), y = load_cluster_f4(src + 16u);
+          v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+          v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+        }
+        finish(v, row, col, p.N, min(8, p.N - col));
+      }
+    } else {
+      for (int i = threadIdx.x; i < kN * (rows / 8); i += kDotThreads) {
+        const int c = i / (rows / 8), r = r0 + (i % (rows / 8)) * 8;
+        const int row = n0 + c, col = m0 + r;      // of C
+        if (row >= p.N || col >= p.M) continue;
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t s = 0; s < splits; ++s) {
+          const uint32_t src = map_to_cta(ring + (r * T::kPitch + c) * 4u, s);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] += load_cluster_f1(src + j * T::kPitch * 4u);
+        }
+        finish(v, row, col, p.M, min(8, p.M - col));
+      }
+    }
+  }
+  if (splits > 1) cluster_sync_all();     // the others may still be reading this CTA's partial tile
+}
+
+// [rows][128 bytes] boxes of a matrix's codes (as 16-bit units), zeros beyond its last row
+int codes_map(CUtensorMap* map, const BlockView& v, int box_rows) {
+  const uint64_t dims[5] = {static_cast<uint64_t>(v.pitch / 2), static_cast<uint64_t>(v.outer), 1, 1, 1};
+  const uint64_t all = static_cast<uint64_t>(v.pitch) * v.outer;
+  const uint64_t strides[4] = {static_cast<uint64_t>(v.pitch), all, all, all};
+  const uint32_t box[5] = {64, static_cast<uint32_t>(box_rows), 1, 1, 1};
+  return make_tensor_map(map, v.codes, dims, strides, box);
+}
+
+template <int kN, bool kNv>
+int launch_dot(DeviceCtx* c, const BlockView& a, const BlockView& b, DotParams& p, int splits, cudaStream_t stream) {
+  using T = DotTile<kN, kNv>;
+  CUtensorMap mapA, mapB;
+  int rc = codes_map(&mapA, a, 128);
+  if (rc == NG_OK) rc = codes_map(&mapB, b, kN);
+  if (rc != NG_OK) return rc;
+  // E2M1 operands, N >> 3, scales E4M3 or E8M0, M >> 4
+  p.idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(kN >> 3) << 17) | ((kNv ? 0u : 1u) << 23) | ((128u >> 4) << 24);
+  const long long tiles = static_cast<long long>(p.tiles_m) * ((p.N + kN - 1ll) / kN);
+  if (tiles * splits > 0x7fffffffll) return fail(NG_ERR_TOO_LARGE, "too many tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+  cfg.blockDim = dim3(kDotThreads);
+  cfg.dynamicSmemBytes = T::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  NG_CUDA(cudaFuncSetAttribute(block_dot_kernel<kN, kNv>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
+  NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_kernel<kN, kNv>, mapA, mapB, p));
+  NG_CHECK_LAUNCH();
+  return NG_OK;
+}
+
+int pad_columns(int n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : (n + 127) / 128 * 128; }
+
+int check_output(const void* C, int ldc, int n, int sr_bits, int out_f32) {
+  if (!C) return fail(NG_ERR_INVALID_ARG, "null operand");
+  if (ldc < n) return fail(NG_ERR_INVALID_ARG, "leading dimension too small");
+  if (sr_bits < 0 || sr_bits > 10) return fail(NG_ERR_INVALID_ARG, "stochastic rounding keeps 1..10 mantissa bits");
+  if (sr_bits && out_f32) return fail(NG_ERR_UNSUPPORTED, "stochastic rounding is to fp16");
+  return NG_OK;
+}
+
+}  // namespace
+
+}  // namespace ngb
+
+using namespace ngb;
+
+extern "C" {
+
+int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ldc, int out_f32, float alpha,
+                 float beta, int relu, int sr_bits, unsigned long long seed, unsigned int rng_offset, void* stream) {
+  int rc = check_shape(A);
+  if (rc == NG_OK) rc = check_shape(B);
+  if (rc != NG_OK) return rc;
+  if (A->format == NG_BLOCK_MXFP8 || A->format != B->format) return fail(NG_ERR_UNSUPPORTED, "both operands are in the same 4-bit format");
+  if (A->axis != 1 || B->axis != 0) return fail(NG_ERR_UNSUPPORTED, "blocks run along the sum: axis 1 of A, axis 0 of B");
+  if (A->cols != B->rows) return fail(NG_ERR_INVALID_ARG, "inner dimensions differ: %d and %d", A->cols, B->rows);
+  const int m = A->rows, n = B->cols;
+  rc = check_output(C, ldc, n, sr_bits, out_f32);
+  if (rc != NG_OK) return rc;
+  DeviceCtx* c = current_ctx();
+  if (!c) return NG_ERR_CUDA;
+  BlockView a, b;
+  rc = block_view(c, A, a);
+  if (rc == NG_OK) rc = block_view(c, B, b);
+  if (rc != NG_OK) return rc;
+
+  const bool nv = A->format == NG_BLOCK_NVFP4;
+  DotParams p = {};
+  p.ea.alpha = nv ? alpha * a.t * b.t : alpha;     // (powers of two)
+  p.ea.beta = beta; p.ea.relu = relu; p.ea.sr_bits = sr_bits;
+  p.ea.seed_lo = static_cast<uint32_t>(seed); p.ea.seed_hi = static_cast<uint32_t>(seed >> 32); p.ea.rng_offset = rng_offset;
+  p.C = C; p.ldc = ldc; p.out_f32 = out_f32;
+  p.vec_ok = (reinterpret_cast<uintptr_t>(C) & 15u) == 0 && ldc % (out_f32 ? 4 : 8) == 0;
+  // The operand with more rows goes to the tile's 128 rows where that leaves less of the tiles empty.
+  const long long as_is = (m + 127ll) / 128 * 128 * pad_columns(n), turned = (n + 127ll) / 128 * 128 * pad_columns(m);
+  p.swapped = turned < as_is;
+  if (p.swapped) std::swap(a, b);
+  p.M = a.outer; p.N = b.outer;
+  p.tiles_m = (p.M + 127) / 128;
+  p.num_kb = static_cast<int>(a.pitch / kRowPad);
+  p.sa = a.scales; p.sb = b.scales; p.spitch = a.spitch;
+  p.sa_tiles = (a.outer + 127) / 128; p.sb_tiles = (b.outer + 127) / 128;
+  p.status = c->status; p.wait_limit_ns = c->wait_limit_ns;
+  int cols = pad_columns(p.N);
+  if (cols > 128) cols = static_cast<long long>(p.tiles_m) * ((p.N + 255) / 256) >= c->sm_count ? 256 : 128;
+  const long long tiles = static_cast<long long>(p.tiles_m) * ((p.N + cols - 1) / cols);
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= c->sm_count && p.num_kb >= splits * 4) splits *= 2;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define NG_DOT(kn) (nv ? launch_dot<kn, true>(c, a, b, p, splits, s) : launch_dot<kn, false>(c, a, b, p, splits, s))
+  switch (cols) {
+    case 16: return NG_DOT(16);
+    case 32: return NG_DOT(32);
+    case 64: return NG_DOT(64);
+    case 128: return NG_DOT(128);
+    default: return NG_DOT(256);
+  }
+#undef NG_DOT
+}
+
+int ng_block_dot_f16(const void* A, int lda, const ng_block_desc* B, void* C, int m, int ldc, int out_f32, float alpha,
+                     float beta, int relu, int sr_bits, unsigned long long seed, unsigned int rng_offset, void* stream) {
+  int rc = check_shape(B);
+  if (rc != NG_OK) return rc;
+  if (!A) return fail(NG_ERR_INVALID_ARG, "null operand");
+  if (B->format != NG_BLOCK_MXFP8) return fail(NG_ERR_UNSUPPORTED, "an fp16 matrix is multiplied with one in mxfp8");
+  if (B->axis != 0) return fail(NG_ERR_UNSUPPORTED, "blocks run along the sum: axis 0 of B");
+  const int n = B->cols, k = B->rows;
+  if (m < 1) return fail(NG_ERR_INVALID_ARG, "m must be positive");
+  if (lda < k) return fail(NG_ERR_INVALID_ARG, "leading dimension too small");
+  rc = check_output(C, ldc, n, sr_bits, out_f32);
+  if (rc != NG_OK) return rc;
+  DeviceCtx* c = current_ctx();
+  if (!c) return NG_ERR_CUDA;
+  BlockView b;
+  rc = block_view(c, B, b);
+  if (rc != NG_OK) return rc;
+  AuxClaim room;
+  void* plain = nullptr;
+  const long long ld = (k + 7ll) / 8 * 8;
+  rc = room.room(c, static_cast<cudaStream_t>(stream), static_cast<size_t>(ld) * n * 2, &plain);
+  if (rc != NG_OK) return rc;
+  rc = dequantize_f16(c, *B, b, static_cast<__half*>(plain), ld, static_cast<cudaStream_t>(stream));
+  if (rc != NG_OK) return rc;
+  GemmCall g = {};
+  g.A = A; g.B = plain; g.C = C; g.b_t = 1; g.m = m; g.n = n; g.k = k;
+  g.lda = lda; g.ldb = ld; g.ldc = ldc; g.alpha = alpha; g.beta = beta; g.relu = relu; g.sr_bits = sr_bits;
+  g.seed = seed; g.rng_offset = rng_offset; g.batch = 1; g.loops = 1; g.out_f32 = out_f32;
+  return run_gemm(g, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

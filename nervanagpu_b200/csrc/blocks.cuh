@@ -1,0 +1,178 @@
+// Matrices held in blocks of small floating-point numbers: layout and the arithmetic of the formats.
+//
+// A block is a run of neighbours along one axis of the matrix (the axis that products sum over) with a scale:
+//
+//   mxfp4   E2M1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6), blocks of 32, scale 2^e (E8M0: the byte is e + 127)
+//   nvfp4   E2M1 numbers, blocks of 16, scale s * t: s an E4M3 byte, t one power of two for the matrix
+//   mxfp8   E4M3 numbers (up to 448), blocks of 32, scale 2^e
+//
+//   e = the smallest with which max|x| <= top * 2^e (top = 6 or 448): nothing saturates, and the largest number
+//       of a block is off by no more than its rounding
+//   s = RN_E4M3(max|x| / (6 t)), kept from 2^-9 (a block that is not all zero keeps a scale) to 448
+//   code = RN(x / scale), ties to even, limited to the largest number
+//   mxfp8: a number that is not zero gets a code that is not zero, so that x > 0 can be told from the code.
+//
+// Read as fp16, values are limited to +-65504: a number next to fp16's largest may have been rounded to one beyond it.
+//
+// A block with an infinity or a NaN has the scale NaN (0xff, or 0x7f in E4M3): all of it reads back as NaN. A
+// product sums over the block, so its result is lost either way. mxfp8 codes keep the signs in such blocks too.
+//
+// Layout. The matrix is stored along its blocked axis ("inner"), one row of codes per index of the other axis
+// ("outer"), two 4-bit codes per byte (the even one in the low half). Rows are padded with zeros to 128 bytes:
+// every row can be addressed by TMA, and a product's k-block of 128 bytes needs no case for the end of the row.
+// 4-bit scales lie as the tensor cores take them: tiles of 512 bytes hold 4 consecutive blocks of 128 outer rows,
+// byte (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4, so that a tile goes to tensor memory in one copy.
+// mxfp8 scales lie row by row. Scales are padded with zeros too (2^-127 or 0: with the zero codes they give zero).
+#pragma once
+#include "../../include/nervana_b200.h"
+#include "common.cuh"
+
+namespace ngb {
+
+constexpr int kRowPad = 128;        // bytes: rows of codes are multiples of this
+constexpr int kScaleTile = 512;     // bytes of a tile of 4-bit formats' scales
+
+// What a kernel needs to know of a matrix in blocks.
+struct BlockView {
+  uint8_t* codes;
+  uint8_t* scales;
+  long long pitch;        // bytes from one row of codes to the next
+  long long spitch;       // bytes from one row (mxfp8) or one row of tiles (4-bit formats) of scales to the next
+  int outer, inner;
+  float t;                // nvfp4: the matrix's power of two
+};
+
+template <int kFmt>
+struct BlockFormat {
+  static constexpr bool k4 = kFmt != NG_BLOCK_MXFP8;
+  static constexpr bool kNv = kFmt == NG_BLOCK_NVFP4;
+  static constexpr int kBlock = kNv ? 16 : 32;
+  static constexpr int kBytes8 = k4 ? 4 : 8;      // bytes of 8 codes
+
+  static __device__ __forceinline__ long long scale_at(const BlockView& v, int o, int b) {
+    if (!k4) return o * v.spitch + b;
+    return (o >> 7) * v.spitch + (b >> 2) * kScaleTile + (o & 31) * 16 + ((o >> 5) & 3) * 4 + (b & 3);
+  }
+};
+
+// fp32 -> E4M3 / E2M1, two at a time, the first in the low half; to nearest, ties to even, limited to the largest
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t cvt_e2m1x8(const float (&y)[8]) {
+  uint32_t r;
+  asm("{\n .reg .b8 a, b, c, d;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+      " mov.b32 %0, {a, b, c, d};\n}\n"
+      : "=r"(r)
+      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+  return r;
+}
+__device__ __forceinline__ __half2 half2_of_e4m3x2(uint32_t codes) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(codes)));
+  return *reinterpret_cast<__half2*>(&r);
+}
+__device__ __forceinline__ void half2_of_e2m1x8(uint32_t codes, __half2 (&h)[4]) {
+  uint32_t r[4];
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
+      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(codes));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<__half2*>(&r[i]);
+}
+
+// Scale of a block from the bits of its largest magnitude: the byte to store, and what the numbers are multiplied
+// with (powers of two, exact) or divided by (nvfp4).
+struct BlockScale {
+  uint32_t byte;
+  float by;
+  bool nan;
+};
+template <int kFmt>
+__device__ __forceinline__ BlockScale block_scale(uint32_t amax_bits, float t) {
+  BlockScale s;
+  s.nan = amax_bits >= 0x7f800000u;
+  if (BlockFormat<kFmt>::kNv) {
+    // (amax / 6t is rounded to fp32 first. That cannot put it on the border between two E4M3 numbers, 5 bits long:
+    // an fp32 number next to 6 t * border is more than half an ulp of the quotient away from it.)
+    s.byte = s.nan ? 0x7fu : cvt_e4m3x2(__fdiv_rn(__uint_as_float(amax_bits), 6.0f * t), 0.0f);
+    if (s.byte == 0u) s.byte = 1u;
+    s.by = __low2float(half2_of_e4m3x2(s.byte)) * t;
+  } else {
+    constexpr int kEmax = BlockFormat<kFmt>::k4 ? 2 : 8;
+    constexpr uint32_t kMant = BlockFormat<kFmt>::k4 ? 0x400000u : 0x600000u;   // 6 = 1.5 * 2^2, 448 = 1.75 * 2^8
+    // biased exponent, one more when the mantissa is above that of the largest number
+    const int e = static_cast<int>((amax_bits + (0x7fffffu - kMant)) >> 23) - kEmax;
+    s.byte = s.nan ? 0xffu : static_cast<uint32_t>(max(e, 0));
+    s.by = __uint_as_float(static_cast<uint32_t>(254 - min(max(e, 0), 253)) << 23);
+  }
+  return s;
+}
+
+// 8 numbers of a block to codes: 4 bytes in x (4-bit formats) or 8 in x and y
+template <int kFmt>
+__device__ __forceinline__ uint2 block_encode8(const float (&x)[8], const BlockScale& s) {
+  float y[8];
+  uint2 r = make_uint2(0u, 0u);
+  if constexpr (BlockFormat<kFmt>::k4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = BlockFormat<kFmt>::kNv ? __fdiv_rn(x[i], s.by) : x[i] * s.by;
+    if (!s.nan) r.x = cvt_e2m1x8(y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // not zero: no less than the smallest code; in a block with the scale NaN the smallest code of x's sign
+      const float mag = s.nan ? 0.001953125f : fmaxf(fabsf(x[i]) * s.by, 0.001953125f);
+      y[i] = (x[i] > 0.0f || x[i] < 0.0f) ? copysignf(mag, x[i]) : 0.0f;
+    }
+    r.x = cvt_e4m3x2(y[0], y[1]) | (cvt_e4m3x2(y[2], y[3]) << 16);
+    r.y = cvt_e4m3x2(y[4], y[5]) | (cvt_e4m3x2(y[6], y[7]) << 16);
+  }
+  return r;
+}
+
+// The scale that a stored byte stands for.
+template <int kFmt>
+__device__ __forceinline__ float block_scale_value(uint32_t byte, float t) {
+  if (BlockFormat<kFmt>::kNv) return __low2float(half2_of_e4m3x2(byte)) * t;
+  if (byte == 0xffu) return __uint_as_float(0x7fffffffu);
+  return __uint_as_float(byte ? byte << 23 : 0x400000u);   // (2^-127 is below the normal range)
+}
+
+// The values of 8 codes.
+template <int kFmt>
+__device__ __forceinline__ void block_decode8(uint2 codes, float scale, float (&v)[8]) {
+  __half2 h[4];
+  if (BlockFormat<kFmt>::k4) {
+    half2_of_e2m1x8(codes.x, h);
+  } else {
+    h[0] = half2_of_e4m3x2(codes.x & 0xffffu);
+    h[1] = half2_of_e4m3x2(codes.x >> 16);
+    h[2] = half2_of_e4m3x2(codes.y & 0xffffu);
+    h[3] = half2_of_e4m3x2(codes.y >> 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x * scale;
+    v[2 * i + 1] = f.y * scale;
+  }
+}
+
+// The same for an fp16 result: limited to its largest number (a NaN stays one).
+template <int kFmt>
+__device__ __forceinline__ void block_limit_f16(float scale, float (&v)[8]) {
+  if (scale * (BlockFormat<kFmt>::k4 ? 6.0f : 448.0f) > 65504.0f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (fabsf(v[i]) > 65504.0f) v[i] = copysignf(65504.0f, v[i]);
+  }
+}
+
+}  // namespace ngb

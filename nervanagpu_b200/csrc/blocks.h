@@ -1,0 +1,15 @@
+// Host-side view of matrices in blocks, shared by the element-wise kernels and the products on them.
+#pragma once
+#include "blocks.cuh"
+#include "host.h"
+
+namespace ngb {
+
+// Checks what a descriptor says, without a device.
+int check_shape(const ng_block_desc* d);
+// Checks a descriptor against the current device and fills in what the kernels need.
+int block_view(const DeviceCtx* c, const ng_block_desc* d, BlockView& v);
+// The values of a checked matrix as rows of `ld` fp16 numbers along its blocked axis.
+int dequantize_f16(DeviceCtx* c, const ng_block_desc& d, const BlockView& q, __half* out, long long ld, cudaStream_t stream);
+
+}  // namespace ngb

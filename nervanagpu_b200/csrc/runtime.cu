@@ -259,6 +259,12 @@ int ng_device_count(int* count) {
   return NG_OK;
 }
 
+int ng_current_device(int* device) {
+  if (!device) return fail(NG_ERR_INVALID_ARG, "device is null");
+  NG_CUDA(cudaGetDevice(device));
+  return NG_OK;
+}
+
 int ng_sm_count(int* count) {
   if (!count) return fail(NG_ERR_INVALID_ARG, "count is null");
   DeviceCtx* c = current_ctx();

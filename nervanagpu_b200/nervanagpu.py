@@ -16,6 +16,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import native as _native
+from .blocks import BlockTensor
 from .float_ew import call_compound_kernel, operation_numbers, prepare_assignment
 from .layers import ConvLayer, DeconvLayer, PoolLayer
 
@@ -759,6 +760,96 @@ class NervanaGPU(object):
             gflops = (batch_loops * batch_grid * m * n * k * 2.0) / (msecs * 1000000.0)
             print("%7.3f msecs %4.0f gflops (hgemm_%s: %d,%d,%d) grid:%d loops:%d" %
                   (msecs, gflops, op, m, n, k, batch_grid, batch_loops))
+            if repeat > 1:
+                return gflops
+        return C
+
+    # ---- matrices in blocks of small floating-point numbers -----------------------------------
+    def block_empty(self, shape, format, axis=1, scale=1.0, name=None):
+        """A matrix of zeros in blocks of "mxfp4", "nvfp4" or "mxfp8" numbers along `axis` (see BlockTensor)."""
+        return BlockTensor(self, shape, format, axis, scale, name)
+
+    @staticmethod
+    def _plain_matrix(A, Q):
+        """Checks of the plain side of a matrix in blocks."""
+        assert isinstance(Q, BlockTensor), "not a matrix in blocks"
+        assert A.take_array is None, "views through index arrays are not supported here"
+        assert A.shape == Q.shape
+        if A.dtype.type not in (np.float16, np.float32):
+            raise TypeError("matrices in blocks are made from and read as fp16 and fp32")
+
+    def quantize(self, A, *outs):
+        """The numbers of A (fp16 or fp32, any strides), to nearest, into each of up to four matrices in blocks, of
+        any formats and axes: a layer's input as an operand of its product and as the record of its backward pass, say.
+        A block that holds an infinity or NaN reads back as NaN."""
+        assert 1 <= len(outs) <= 4, "one to four matrices in blocks"
+        for Q in outs:
+            self._plain_matrix(A, Q)
+        if len(outs) == 1:
+            descs = outs[0].desc
+        else:
+            descs = (_lib.BlockDesc * len(outs))(*[Q.desc for Q in outs])
+        _lib.check(self.lib.ng_block_quantize(A.ptr, A.dtype.itemsize, A.strides[0], A.strides[1], descs, len(outs), self.stream))
+        return outs[0] if len(outs) == 1 else outs
+
+    def dequantize(self, Q, out):
+        """out = the values that Q's codes stand for (fp16: rounded, and limited to +-65504)."""
+        self._plain_matrix(out, Q)
+        _lib.check(self.lib.ng_block_dequantize(Q.desc, out.ptr, out.dtype.itemsize, out.strides[0], out.strides[1], self.stream))
+        return out
+
+    def relu_mask(self, Q, E):
+        """E = Q > 0 ? E : 0 in place, Q an "mxfp8" record: the mask of the ReLU that Q is the output of, as
+        E *= Q > 0 on the plain activation but that what is masked becomes 0 even from an infinity or NaN. A record
+        keeps for every number whether it was positive."""
+        self._plain_matrix(E, Q)
+        if Q.format != "mxfp8":
+            raise TypeError("only mxfp8 keeps which numbers were positive")
+        _lib.check(self.lib.ng_block_relu_mask(Q.desc, E.ptr, E.dtype.itemsize, E.strides[0], E.strides[1], self.stream))
+        return E
+
+    def block_dot(self, A, B, C, alpha=1.0, beta=0.0, relu=False, repeat=1, stochastic_round=None):
+        """C = alpha * A * B + beta * C with operands in blocks along the sum (A of axis 1, B of axis 0): both in
+        the same 4-bit format, or A a plain fp16 matrix and B in "mxfp8". C is fp16 or fp32 with contiguous rows;
+        sums are taken in fp32. relu and stochastic_round as in dot.
+
+        With X a layer's input (features x images): block_dot(W, X4, Y, relu=True) is its forward product from 4-bit
+        weights and inputs, block_dot(E, X8.T, dW) its weight gradient from the input's 8-bit record."""
+        assert isinstance(B, BlockTensor), "not a matrix in blocks"
+        assert A.shape[1] == B.shape[0] and len(C.shape) == 2 and C.shape == (A.shape[0], B.shape[1])
+        m, n, k = A.shape[0], B.shape[1], A.shape[1]
+        if C.dtype.type not in (np.float16, np.float32):
+            raise TypeError("block_dot writes fp16 or fp32")
+        assert C.take_array is None and (n == 1 or C.strides[1] == 1), "C must have contiguous rows"
+        ldc = C.strides[0] if m > 1 else n
+        assert n <= ldc < 2 ** 31, "C must have contiguous rows"
+        out_f32 = int(C.dtype.type is np.float32)
+        sr = 0 if out_f32 and stochastic_round is None else self._gemm_flags(C, stochastic_round)
+        lib, stream, rs = self.lib, self.stream, self.rand_state
+        if isinstance(A, BlockTensor):
+            if A.format != B.format or A.format == "mxfp8":
+                raise TypeError("block_dot multiplies two matrices in the same 4-bit format, or fp16 and mxfp8")
+            assert A.axis == 1 and B.axis == 0, "blocks must run along the sum: axis 1 of A, axis 0 of B"
+
+            def launch():
+                off = rs.next_offset() if sr else 0
+                _lib.check(lib.ng_block_dot(A.desc, B.desc, C.ptr, ldc, out_f32, alpha, beta, int(bool(relu)), sr, rs.seed, off, stream))
+        else:
+            if A.dtype.type is not np.float16 or B.format != "mxfp8":
+                raise TypeError("block_dot multiplies two matrices in the same 4-bit format, or fp16 and mxfp8")
+            assert B.axis == 0, "blocks must run along the sum: axis 0 of B"
+            assert A.take_array is None and len(A.shape) == 2 and (k == 1 or A.strides[1] == 1), "A must have contiguous rows"
+            lda = A.strides[0] if m > 1 else k
+            assert k <= lda < 2 ** 31, "A must have contiguous rows"
+
+            def launch():
+                off = rs.next_offset() if sr else 0
+                _lib.check(lib.ng_block_dot_f16(A.ptr, lda, B.desc, C.ptr, m, ldc, out_f32, alpha, beta, int(bool(relu)), sr, rs.seed, off, stream))
+
+        msecs = self._timed(launch, repeat)
+        if msecs is not None:
+            gflops = (m * n * k * 2.0) / (msecs * 1000000.0)
+            print("%7.3f msecs %4.0f gflops (block_dot %s: %d,%d,%d)" % (msecs, gflops, B.format, m, n, k))
             if repeat > 1:
                 return gflops
         return C

@@ -554,3 +554,51 @@ def fp16_neighbours(x, mantissa_bits=10):
     # truncation never produces infinity from a finite value: clamp at the largest fp16
     big = np.float32(65504.0)
     return np.clip(lo, -big, big).astype(np.float16), np.clip(hi, -big, big).astype(np.float16)
+
+
+# ---- matrices in blocks of small floating-point numbers ----------------------------------------------
+# (no counterpart in the reference; the definitions are those of include/nervana_b200.h, in 64 bits)
+BLOCK_FORMATS = {"mxfp4": (32, 6.0), "nvfp4": (16, 6.0), "mxfp8": (32, 448.0)}
+
+
+def block_numbers(fmt):
+    """The numbers of a format from zero up; those with an even last bit have an even place."""
+    if fmt == "mxfp8":
+        subnormal = [m * 2.0 ** -9 for m in range(8)]
+        return np.array(subnormal + [(8 + m) * 2.0 ** (e - 3) for e in range(-6, 9) for m in range(8)][:-1])
+    return np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def nearest_number(y, fmt):
+    """Magnitudes to the nearest number of a format, ties to the one with an even last bit, limited to the largest."""
+    q = block_numbers(fmt)
+    border = (q[1:] + q[:-1]) / 2
+    lo, hi = np.searchsorted(border, y, side="left"), np.searchsorted(border, y, side="right")
+    return q[np.where(lo % 2 == 0, lo, hi)]
+
+
+def block_values(x, fmt, axis=1, scale=1.0):
+    """The values that a matrix in blocks holds after quantisation of x, in 64 bits."""
+    x = np.asarray(x)
+    if axis == 0:
+        return block_values(x.T, fmt, 1, scale).T
+    block, top = BLOCK_FORMATS[fmt]
+    rows, cols = x.shape
+    full = np.zeros((rows, -(-cols // block) * block))
+    full[:, :cols] = x
+    full = full.reshape(rows, -1, block)
+    bad = ~np.isfinite(full).all(axis=2)
+    mag = np.abs(np.where(bad[:, :, None], 0.0, full))
+    amax = mag.max(axis=2)
+    if fmt == "nvfp4":
+        s = np.maximum(nearest_number(amax / top / scale, "mxfp8"), 2.0 ** -9) * scale
+    else:
+        powers = 2.0 ** np.arange(-127, 128)
+        s = powers[np.searchsorted(powers * top, amax)]
+    y = mag / s[:, :, None]
+    q = nearest_number(y, fmt)
+    if fmt == "mxfp8":
+        q = np.where((q == 0) & (y > 0), 2.0 ** -9, q)
+    v = np.copysign(q * s[:, :, None], full)
+    v[bad] = np.nan
+    return v.reshape(rows, -1)[:, :cols]
