@@ -16,6 +16,7 @@
 //   warps 2-5  tensor memory -> shared memory
 //   all        sum over the cluster, output stage (epilogue.cuh), stores
 #include <algorithm>
+#include <atomic>
 
 #include "blocks.h"
 #include "epilogue.cuh"
@@ -345,7 +346,11 @@ int launch_dot(DeviceCtx* c, const BlockView& a, const BlockView& b, DotParams& 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  NG_CUDA(cudaFuncSetAttribute(block_dot_kernel<kN, kNv>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
+  static std::atomic<unsigned long long> ready{0};      // devices on which this instance may use its shared memory
+  if (!(ready.load(std::memory_order_relaxed) >> c->device & 1u)) {
+    NG_CUDA(cudaFuncSetAttribute(block_dot_kernel<kN, kNv>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
+    ready.fetch_or(1ull << c->device, std::memory_order_relaxed);
+  }
   NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_kernel<kN, kNv>, mapA, mapB, p));
   NG_CHECK_LAUNCH();
   return NG_OK;

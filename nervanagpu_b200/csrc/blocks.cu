@@ -3,9 +3,8 @@
 //
 // All three move each number once and are bound by that: a quantisation reads 2 or 4 bytes per number and writes
 // half a byte or one, plus a scale per block. Two forms each, by how the blocks lie in the plain matrix:
-//   rows      neighbours of a block are neighbours in memory: a lane takes 8 of them (16 bytes of fp16), 2 or 4
-//             lanes share a block and exchange its largest magnitude by shuffles
-//   strided   a thread takes a whole block, lanes run along the other axis, which is then the contiguous one (the
+//   rows      neighbours of a block are neighbours in memory: a lane takes 16 of them, two share a block of 32
+//   strided   a thread takes whole blocks, lanes run along the other axis, which is then the contiguous one (the
 //             usual case: a layer's inputs, features x images, in blocks of features); any strides
 #include <algorithm>
 #include <cmath>
@@ -23,96 +22,196 @@ template <typename T>
 struct PlainView {
   T* p;
   long long so, sl;
+  bool wide;        // rows form: every row starts on 32 bytes
 };
 
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ void from_f32(float v, __half& x) { x = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(float v, float& x) { x = v; }
-
-// 8 neighbours at p, 16-byte aligned when kVec; only the first n exist
-template <bool kVec>
-__device__ __forceinline__ void load8(const __half* p, int n, float (&x)[8]) {
-  if (kVec && n >= 8) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const __half2* h = reinterpret_cast<const __half2*>(&w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(h[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = i < n ? __half2float(p[i]) : 0.0f;
-}
-template <bool kVec>
-__device__ __forceinline__ void load8(const float* p, int n, float (&x)[8]) {
-  if (kVec && n >= 8) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = i < n ? p[i] : 0.0f;
-}
-template <bool kVec>
-__device__ __forceinline__ void store8(__half* p, int n, const float (&v)[8]) {
-  if (kVec && n >= 8) {
-    uint4 w;
-    __half2* h = reinterpret_cast<__half2*>(&w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = w;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) p[i] = __float2half_rn(v[i]);
-}
-template <bool kVec>
-__device__ __forceinline__ void store8(float* p, int n, const float (&v)[8]) {
-  if (kVec && n >= 8) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) p[i] = v[i];
-}
-
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// ---- rows form. Lane g of a row takes numbers 8 g .. 8 g + 7; rows in steps of the grid.
+// ---- rows form: 16 numbers per lane ------------------------------------------------------------------
+constexpr int kLane = 16;
+
+// 16 neighbours as they lie in memory
+template <typename T>
+struct Raw {
+  static constexpr int kVecs = kLane * sizeof(T) / 16;
+  uint4 v[kVecs];
+  __device__ __forceinline__ T* at() { return reinterpret_cast<T*>(v); }
+  __device__ __forceinline__ const T* at() const { return reinterpret_cast<const T*>(v); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  // The first n of 16 numbers at a 16-byte aligned address. wide: the rows are 32-byte aligned, and whole sectors
+  // are moved at a time (by halves, the two accesses of a warp each touched every sector).
+  __device__ __forceinline__ void load(const T* p, int n, bool wide) {
+    if (n >= kLane && wide) {
+#pragma unroll
+      for (int i = 0; i < kVecs; i += 2)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w), "=r"(v[i + 1].x), "=r"(v[i + 1].y),
+                       "=r"(v[i + 1].z), "=r"(v[i + 1].w)
+                     : "l"(reinterpret_cast<const uint4*>(p) + i));
+    } else if (n >= kLane) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLane; ++i) at()[i] = i < n ? p[i] : T(0.0f);
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int n, bool wide) const {
+    if (n >= kLane && wide) {
+#pragma unroll
+      for (int i = 0; i < kVecs; i += 2)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint4*>(p) + i),
+                     "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w), "r"(v[i + 1].x), "r"(v[i + 1].y), "r"(v[i + 1].z),
+                     "r"(v[i + 1].w)
+                     : "memory");
+    } else if (n >= kLane) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLane; ++i)
+        if (i < n) p[i] = at()[i];
+    }
+  }
+};
+
+// Largest magnitude, as the bits of an fp32 number (above those of infinity for a NaN).
+__device__ __forceinline__ uint32_t top_bits(const Raw<__half>& r) {
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w[4] = {r.v[i].x, r.v[i].y, r.v[i].z, r.v[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
+  }
+  const uint16_t bits = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+  return magnitude_bits(__half2float(__ushort_as_half(bits)));
+}
+__device__ __forceinline__ uint32_t top_bits(const Raw<float>& r) {
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < kLane; ++i) top = max(top, magnitude_bits(r.at()[i]));
+  return top;
+}
+
+// Rows at addresses that are no multiples of 16 bytes: the warp moves its 512 numbers (a run of 16 << log_tx of each
+// of its rows, at least 128) in order, one number per lane and access, through shared memory. (A lane that moved its
+// own 16 one by one touched 32 sectors per access: 139968 x 125 fp16 read back from 8 bits took 51 us.)
+template <typename T, bool kStore>
+__device__ __forceinline__ void warp_move(T* base, long long so, long long o_first, int outer, int l_first, int inner, int log_tx, T* stage) {
+  const int lane = threadIdx.x + threadIdx.y * blockDim.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long o = o_first + (i >> (log_tx - 3));
+    const int l = l_first + (i & ((1 << (log_tx - 3)) - 1)) * 128 + lane;
+    T* p = base + o * so + l;
+    T* s = stage + i * 128 + lane;
+    const int n = o < outer ? inner - l : 0;
+    if (kStore) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j * 32 < n) p[j * 32] = s[j * 32];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j * 32] = j * 32 < n ? p[j * 32] : T(0.0f);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void warp_load(const T* base, long long so, long long o_first, int outer, int l_first, int inner, int log_tx,
+                                          T* stage, Raw<T>& r) {
+  const int lane = threadIdx.x + threadIdx.y * blockDim.x & 31;
+  warp_move<T, false>(const_cast<T*>(base), so, o_first, outer, l_first, inner, log_tx, stage);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < Raw<T>::kVecs; ++i) r.v[i] = reinterpret_cast<const uint4*>(stage + lane * kLane)[i];
+  __syncwarp();
+}
+template <typename T>
+__device__ __forceinline__ void warp_store(T* base, long long so, long long o_first, int outer, int l_first, int inner, int log_tx,
+                                           T* stage, const Raw<T>& r) {
+  const int lane = threadIdx.x + threadIdx.y * blockDim.x & 31;
+#pragma unroll
+  for (int i = 0; i < Raw<T>::kVecs; ++i) reinterpret_cast<uint4*>(stage + lane * kLane)[i] = r.v[i];
+  __syncwarp();
+  warp_move<T, true>(base, so, o_first, outer, l_first, inner, log_tx, stage);
+  __syncwarp();
+}
+
+// One step of a rows kernel: this thread's row, and the warp's first row and first group (warp_load).
+#define NG_ROWS_PROLOGUE(T)                                                                             \
+  __shared__ __align__(16) T stage_all[kVec ? 1 : 256 * kLane];                                         \
+  const int tid = threadIdx.x + threadIdx.y * blockDim.x;                                               \
+  T* stage = kVec ? stage_all : stage_all + (tid & ~31) * kLane;                                        \
+  const int log_tx = min(31 - __clz(blockDim.x), 5);      /* lanes of one warp in a row */              \
+  const int g = blockIdx.x * blockDim.x + threadIdx.x, n = q.inner - g * kLane;                         \
+  const int l_warp = (g - (tid & 31 & (static_cast<int>(blockDim.x) - 1))) * kLane;                     \
+  const int y_warp = (tid & ~31) / static_cast<int>(blockDim.x);                                        \
+  const long long step = static_cast<long long>(gridDim.y) * blockDim.y
+
 template <typename T, int kFmt, bool kVec>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(BlockView q, PlainView<const T> a) {
   using F = BlockFormat<kFmt>;
-  const int g = blockIdx.x * blockDim.x + threadIdx.x;
-  const int n = q.inner - g * 8;                   // numbers that exist, from this lane's first on
-  const long long step = static_cast<long long>(gridDim.y) * blockDim.y;
-  // (a warp's lanes may be in different rows, but a block's are together: whole warps take part in the shuffles)
-  for (long long o0 = blockIdx.y * blockDim.y; o0 < q.outer; o0 += step) {
-    const int o = static_cast<int>(o0) + threadIdx.y;
-    const bool live = o < q.outer && n > 0;
-    float x[8];
+  NG_ROWS_PROLOGUE(T);
+  constexpr int kUnroll = kVec ? 2 : 1;       // rows whose loads are in flight together
+  // (whole warps stay to the end of the loop: lanes exchange magnitudes and scales)
+  for (long long o0 = static_cast<long long>(blockIdx.y) * blockDim.y; o0 < q.outer; o0 += kUnroll * step) {
+    Raw<T> raw[kUnroll];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    if (live) load8<kVec>(a.p + o * a.so + g * 8ll, n, x);
-    uint32_t top = 0u;
+    for (int u = 0; u < kUnroll; ++u) {
+      const long long o = o0 + u * step + threadIdx.y;
+      if (kVec) {
+        raw[u].clear();
+        if (o < q.outer && n > 0) raw[u].load(a.p + o * a.so + static_cast<long long>(g) * kLane, n, a.wide);
+      } else {
+        warp_load(a.p, a.so, o0 + u * step + y_warp, q.outer, l_warp, q.inner, log_tx, stage, raw[u]);
+      }
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(x[i]));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    if (F::kBlock == 32) top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const BlockScale s = block_scale<kFmt>(top, q.t);
-    const uint2 codes = block_encode8<kFmt>(x, s);
-    if (live) {
-      uint8_t* dst = q.codes + o * q.pitch + g * F::kBytes8;
-      if (F::k4) *reinterpret_cast<uint32_t*>(dst) = codes.x;
-      else *reinterpret_cast<uint2*>(dst) = codes;
-      if (g % (F::kBlock / 8) == 0) q.scales[F::scale_at(q, o, g / (F::kBlock / 8))] = static_cast<uint8_t>(s.byte);
+    for (int u = 0; u < kUnroll; ++u) {
+      const long long o = o0 + u * step + threadIdx.y;
+      const bool live = o < q.outer && n > 0;
+      uint32_t top = top_bits(raw[u]);
+      if (!F::kNv) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      const BlockScale s = block_scale<kFmt>(top, q.t);
+      uint2 c[2];
+      // (by up to 2^30 is two fp16 factors; a block of zeros needs none)
+      if (!F::k4 && sizeof(T) == 2 && !s.nan && (s.by <= 1073741824.0f || top == 0u)) {
+        __half2 by0, by1;
+        block_scale_f16(s.by, by0, by1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          c[h].x = block_encode4_f16(raw[u].v[h].x, raw[u].v[h].y, by0, by1);
+          c[h].y = block_encode4_f16(raw[u].v[h].z, raw[u].v[h].w, by0, by1);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = to_f32(raw[u].at()[8 * h + i]);
+          c[h] = block_encode8<kFmt, sizeof(T) == 2>(x, s);
+        }
+      }
+      // the scales of four blocks leave together: four lanes, or eight that hold each twice
+      constexpr int kShare = F::kNv ? 1 : 2;
+      uint32_t word = live ? s.byte << (8 * (g / kShare % 4)) : 0u;
+      word |= __shfl_xor_sync(0xffffffffu, word, kShare);
+      word |= __shfl_xor_sync(0xffffffffu, word, 2 * kShare);
+      if (live) {
+        uint8_t* dst = q.codes + o * q.pitch + static_cast<long long>(g) * (2 * F::kBytes8);
+        if (F::k4) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0].x, c[1].x);
+        else *reinterpret_cast<uint4*>(dst) = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
+        if (g % (4 * kShare) == 0)
+          *reinterpret_cast<uint32_t*>(q.scales + F::scale_at(q, static_cast<int>(o), g / kShare)) = word;
+      }
     }
   }
 }
@@ -120,131 +219,271 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(BlockView q, PlainVi
 template <typename T, int kFmt, bool kVec>
 __global__ void __launch_bounds__(256) dequantize_rows_kernel(BlockView q, PlainView<T> a) {
   using F = BlockFormat<kFmt>;
-  const int g = blockIdx.x * blockDim.x + threadIdx.x;
-  const int n = q.inner - g * 8;
-  if (n <= 0) return;
-  const long long step = static_cast<long long>(gridDim.y) * blockDim.y;
-  for (long long o = static_cast<long long>(blockIdx.y) * blockDim.y + threadIdx.y; o < q.outer; o += step) {
-    const uint8_t* src = q.codes + o * q.pitch + g * F::kBytes8;
-    uint2 codes = make_uint2(0u, 0u);
-    if (F::k4) codes.x = *reinterpret_cast<const uint32_t*>(src);
-    else codes = *reinterpret_cast<const uint2*>(src);
-    const uint32_t byte = q.scales[F::scale_at(q, static_cast<int>(o), g / (F::kBlock / 8))];
-    const float scale = block_scale_value<kFmt>(byte, q.t);
-    float v[8];
-    block_decode8<kFmt>(codes, scale, v);
-    if (sizeof(T) == 2) block_limit_f16<kFmt>(scale, v);
-    store8<kVec>(a.p + o * a.so + g * 8ll, n, v);
+  NG_ROWS_PROLOGUE(T);
+  constexpr int kShare = F::kNv ? 1 : 2;
+  constexpr int kUnroll = kVec ? 2 : 1;
+  for (long long o0 = static_cast<long long>(blockIdx.y) * blockDim.y; o0 < q.outer; o0 += kUnroll * step) {
+    uint4 codes[kUnroll];
+    uint32_t byte[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const long long o = o0 + u * step + threadIdx.y;
+      codes[u] = make_uint4(0u, 0u, 0u, 0u);
+      byte[u] = 0u;
+      if (o < q.outer && n > 0) {
+        const uint8_t* src = q.codes + o * q.pitch + static_cast<long long>(g) * (2 * F::kBytes8);
+        if (F::k4) {
+          const uint2 c = *reinterpret_cast<const uint2*>(src);
+          codes[u].x = c.x;
+          codes[u].z = c.y;
+        } else {
+          codes[u] = *reinterpret_cast<const uint4*>(src);
+        }
+        byte[u] = q.scales[F::scale_at(q, static_cast<int>(o), g / kShare)];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const long long o = o0 + u * step + threadIdx.y;
+      const float scale = block_scale_value<kFmt>(byte[u], q.t);
+      Raw<T> r;
+      if (sizeof(T) == 2 && block_scale_fits_f16<kFmt>(scale)) {
+        const __half2 by = __float2half2_rn(scale);
+        r.v[0] = block_decode8_f16<kFmt>(make_uint2(codes[u].x, codes[u].y), by);
+        r.v[1] = block_decode8_f16<kFmt>(make_uint2(codes[u].z, codes[u].w), by);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[8];
+          block_decode8<kFmt>(h == 0 ? make_uint2(codes[u].x, codes[u].y) : make_uint2(codes[u].z, codes[u].w), scale, v);
+          if (sizeof(T) == 2) block_limit_f16<kFmt>(scale, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) from_f32(v[i], r.at()[8 * h + i]);
+        }
+      }
+      if (!kVec) warp_store(a.p, a.so, o0 + u * step + y_warp, q.outer, l_warp, q.inner, log_tx, stage, r);
+      else if (o < q.outer && n > 0) r.store(a.p + o * a.so + static_cast<long long>(g) * kLane, n, a.wide);
+    }
   }
 }
+
+// a code of a number that is not positive: 0, or with the sign bit
+__device__ __forceinline__ bool not_positive(uint32_t code) { return code - 1u >= 0x7fu; }
 
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256) relu_mask_rows_kernel(BlockView q, PlainView<T> a) {
-  const int g = blockIdx.x * blockDim.x + threadIdx.x;
-  const int n = q.inner - g * 8;
-  if (n <= 0) return;
+  const int tid = threadIdx.x + threadIdx.y * blockDim.x, lane = tid & 31;
+  const int log_tx = min(31 - __clz(blockDim.x), 5);
+  const int g = blockIdx.x * blockDim.x + threadIdx.x, n = q.inner - g * kLane;
   const long long step = static_cast<long long>(gridDim.y) * blockDim.y;
-  for (long long o = static_cast<long long>(blockIdx.y) * blockDim.y + threadIdx.y; o < q.outer; o += step) {
-    const uint2 codes = *reinterpret_cast<const uint2*>(q.codes + o * q.pitch + g * 8);
-    T* p = a.p + o * a.so + g * 8ll;
-    uint32_t zero = 0u;      // bit i: number i is not positive (its code is 0 or has the sign bit)
+  for (long long o0 = static_cast<long long>(blockIdx.y) * blockDim.y; o0 < q.outer; o0 += step) {
+    const long long o = o0 + threadIdx.y;
+    const bool live = o < q.outer && n > 0;
+    uint4 codes = make_uint4(0u, 0u, 0u, 0u);
+    if (live) codes = *reinterpret_cast<const uint4*>(q.codes + o * q.pitch + static_cast<long long>(g) * kLane);
+    uint32_t off = 0u;       // bit i: number i was not positive
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t c = ((i < 4 ? codes.x : codes.y) >> (8 * (i & 3))) & 0xffu;
-      zero |= (c - 1u >= 0x7fu ? 1u : 0u) << i;
+    for (int i = 0; i < kLane; ++i) {
+      const uint32_t w = i < 4 ? codes.x : i < 8 ? codes.y : i < 12 ? codes.z : codes.w;
+      off |= (not_positive(w >> (8 * (i & 3)) & 0xffu) ? 1u : 0u) << i;
     }
-    if (kVec && n >= 8) {
-      // whole vectors; fp32 in two of them
-      constexpr int kPer = 16 / sizeof(T);
+    if (kVec) {
+      if (!live) continue;
+      T* p = a.p + o * a.so + static_cast<long long>(g) * kLane;
+      Raw<T> r;
+      r.load(p, n, a.wide);
 #pragma unroll
-      for (int h = 0; h < 8 / kPer; ++h) {
-        uint4 w = reinterpret_cast<uint4*>(p)[h];
-        T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (zero >> (h * kPer + i) & 1u) e[i] = T(0.0f);
-        reinterpret_cast<uint4*>(p)[h] = w;
-      }
+      for (int i = 0; i < kLane; ++i)
+        if (off >> i & 1u) r.at()[i] = T(0.0f);
+      r.store(p, n, a.wide);
     } else {
+      // zeros, one number per lane and access, in the order of warp_move
+      const int l_warp = (g - (lane & (static_cast<int>(blockDim.x) - 1))) * kLane;
+      const long long o_warp = o0 + (tid & ~31) / static_cast<int>(blockDim.x);
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const long long row = o_warp + (i >> (log_tx - 3));
+        const int l = l_warp + (i & ((1 << (log_tx - 3)) - 1)) * 128 + lane;
+        T* p = a.p + row * a.so + l;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n && (zero >> i & 1u)) p[i] = T(0.0f);
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t mask = __shfl_sync(0xffffffffu, off, i * 8 + j * 2 + (lane >> 4));
+          if ((mask >> (lane & 15) & 1u) && row < q.outer && l + j * 32 < q.inner) p[j * 32] = T(0.0f);
+        }
+      }
     }
   }
 }
 
-// ---- strided form. Lanes along the outer axis, a block of numbers per thread.
-template <typename T, int kFmt>
-__global__ void __launch_bounds__(256) quantize_strided_kernel(BlockView q, PlainView<const T> a, int blocks) {
+// ---- strided form --------------------------------------------------------------------------------------
+// A CTA takes 64 outer rows x 4 blocks: half a tile of 4-bit scales, and 32 to 128 neighbouring bytes of codes per outer
+// row, so that a quantisation leaves in whole sectors through shared memory. A warp has one block, a lane two outer
+// rows: kVec (the outer axis is the contiguous one, in aligned pairs): neighbours, in one access; else 32
+// apart, one by one. (Four rows per lane were faster for large matrices by 5 % and took 6.7 us instead of 2.9 for a
+// minibatch of 9216 x 128, with too few warps to hide their latency.)
+constexpr int kStridedThreads = 128;
+constexpr int kStridedRows = 64;
+
+template <int kFmt>
+struct StridedTile {
   using F = BlockFormat<kFmt>;
-  const int o = blockIdx.x * 32 + threadIdx.x;
-  if (o >= q.outer) return;
-  for (int b = blockIdx.y * 8 + threadIdx.y; b < blocks; b += gridDim.y * 8) {
-    const T* p = a.p + o * a.so + static_cast<long long>(b) * F::kBlock * a.sl;
-    const int n = q.inner - b * F::kBlock;
-    T raw[F::kBlock];
+  static constexpr int kBytes = F::kBlock / 8 * F::kBytes8;     // of a block's codes
+  static constexpr int kRow = 4 * kBytes;
+  static constexpr int kPitch = kRow + 16;                      // (rows in shared memory, off each other's banks)
+};
+// Two numbers of neighbouring outer rows as they lie in memory.
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using Vec = uint32_t;
+  static __device__ __forceinline__ Vec of(__half a, __half b) { return __half_as_ushort(a) | static_cast<uint32_t>(__half_as_ushort(b)) << 16; }
+  static __device__ __forceinline__ float get(Vec v, int j) { return __half2float(__ushort_as_half(static_cast<uint16_t>(j ? v >> 16 : v & 0xffffu))); }
+};
+template <>
+struct Pair<float> {
+  using Vec = uint2;
+  static __device__ __forceinline__ Vec of(float a, float b) { return make_uint2(__float_as_uint(a), __float_as_uint(b)); }
+  static __device__ __forceinline__ float get(Vec v, int j) { return __uint_as_float(j ? v.y : v.x); }
+};
+// Largest magnitudes of both rows, as the bits of fp32 numbers.
+template <int kN>
+__device__ __forceinline__ void top_of_pairs(const uint32_t (&raw)[kN], uint32_t (&top)[2]) {
+  uint32_t t = 0u;
 #pragma unroll
-    for (int i = 0; i < F::kBlock; ++i) raw[i] = i < n ? p[i * a.sl] : T(0.0f);
-    uint32_t top = 0u;
+  for (int i = 0; i < kN; ++i) t = __vmaxu2(t, raw[i] & 0x7fff7fffu);
+  top[0] = magnitude_bits(Pair<__half>::get(t, 0));
+  top[1] = magnitude_bits(Pair<__half>::get(t, 1));
+}
+template <int kN>
+__device__ __forceinline__ void top_of_pairs(const uint2 (&raw)[kN], uint32_t (&top)[2]) {
+  top[0] = top[1] = 0u;
 #pragma unroll
-    for (int i = 0; i < F::kBlock; ++i) top = max(top, magnitude_bits(to_f32(raw[i])));
-    const BlockScale s = block_scale<kFmt>(top, q.t);
-    uint8_t* dst = q.codes + o * q.pitch + static_cast<long long>(b) * (F::kBlock / 8 * F::kBytes8);
-    uint32_t w[F::kBlock / 8 * F::kBytes8 / 4];
+  for (int i = 0; i < kN; ++i) {
+    top[0] = max(top[0], raw[i].x & 0x7fffffffu);
+    top[1] = max(top[1], raw[i].y & 0x7fffffffu);
+  }
+}
+// row of the tile that is this lane's j-th
+template <bool kVec>
+__device__ __forceinline__ int strided_row(int j) {
+  const int lane = threadIdx.x & 31;
+  return kVec ? 2 * lane + j : lane + 32 * j;
+}
+
+template <typename T, int kFmt, bool kVec>
+__global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(BlockView q, PlainView<const T> a, int blocks) {
+  using F = BlockFormat<kFmt>;
+  using S = StridedTile<kFmt>;
+  using P = Pair<T>;
+  __shared__ __align__(16) uint8_t codes[kStridedRows * S::kPitch];
+  __shared__ __align__(16) uint8_t scales[kStridedRows * 4];
+  const int which = threadIdx.x >> 5;               // of the four blocks
+  const int o0 = blockIdx.x * kStridedRows;
+  for (int b0 = blockIdx.y * 4; b0 < blocks; b0 += gridDim.y * 4) {
+    const int b = b0 + which;
+    const int n = q.inner - b * F::kBlock;          // numbers of the block that exist
+    typename P::Vec raw[F::kBlock];
+    const T* p = a.p + static_cast<long long>(b) * F::kBlock * a.sl;
+    const int r0 = o0 + strided_row<kVec>(0), r1 = o0 + strided_row<kVec>(1);
+    if (kVec) {
+      const bool live = r0 < q.outer;
 #pragma unroll
-    for (int j = 0; j < F::kBlock / 8; ++j) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = to_f32(raw[8 * j + i]);
-      const uint2 c = block_encode8<kFmt>(x, s);
-      if (F::k4) {
-        w[j] = c.x;
-      } else {
-        w[2 * j] = c.x;
-        w[2 * j + 1] = c.y;
+      for (int i = 0; i < F::kBlock; ++i) {
+        raw[i] = P::of(T(0.0f), T(0.0f));
+        if (live && i < n) raw[i] = *reinterpret_cast<const typename P::Vec*>(p + r0 + i * a.sl);
       }
-    }
-    if (F::kNv) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
     } else {
+      const T *p0 = p + r0 * a.so, *p1 = p + r1 * a.so;
 #pragma unroll
-      for (int j = 0; j < F::kBytes8 / 4; ++j)
-        reinterpret_cast<uint4*>(dst)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+      for (int i = 0; i < F::kBlock; ++i)
+        raw[i] = P::of(r0 < q.outer && i < n ? p0[i * a.sl] : T(0.0f), r1 < q.outer && i < n ? p1[i * a.sl] : T(0.0f));
     }
-    q.scales[F::scale_at(q, o, b)] = static_cast<uint8_t>(s.byte);
+    uint32_t top[2];
+    top_of_pairs(raw, top);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = strided_row<kVec>(j);
+      const BlockScale s = block_scale<kFmt>(top[j], q.t);
+      uint8_t* dst = codes + row * S::kPitch + which * S::kBytes;
+#pragma unroll
+      for (int h = 0; h < F::kBlock / 8; ++h) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = P::get(raw[8 * h + i], j);
+        const uint2 c = block_encode8<kFmt, sizeof(T) == 2>(x, s);
+        if (F::k4) *reinterpret_cast<uint32_t*>(dst + 4 * h) = c.x;
+        else *reinterpret_cast<uint2*>(dst + 8 * h) = c;
+      }
+      scales[row * 4 + which] = n > 0 && o0 + row < q.outer ? static_cast<uint8_t>(s.byte) : 0;
+    }
+    __syncthreads();
+    // (a group of four blocks is whole within a row's padding; what lies behind the last number is zero)
+#pragma unroll
+    for (int i = threadIdx.x; i < kStridedRows * (S::kRow / 16); i += kStridedThreads) {
+      const int row = i / (S::kRow / 16), c = i % (S::kRow / 16);
+      if (o0 + row < q.outer)
+        *reinterpret_cast<uint4*>(q.codes + (o0 + row) * q.pitch + static_cast<long long>(b0) * S::kBytes + c * 16) =
+            *reinterpret_cast<const uint4*>(codes + row * S::kPitch + c * 16);
+    }
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(scales);
+    if (F::k4) {
+      if (threadIdx.x < 32)
+        *reinterpret_cast<uint2*>(q.scales + F::scale_at(q, o0, b0) + threadIdx.x * 16) = make_uint2(words[threadIdx.x], words[threadIdx.x + 32]);
+    } else if (threadIdx.x < kStridedRows && o0 + static_cast<int>(threadIdx.x) < q.outer) {
+      *reinterpret_cast<uint32_t*>(q.scales + F::scale_at(q, o0 + threadIdx.x, b0)) = words[threadIdx.x];
+    }
+    __syncthreads();
   }
 }
 
-template <typename T, int kFmt>
-__global__ void __launch_bounds__(256) dequantize_strided_kernel(BlockView q, PlainView<T> a, int blocks) {
+// (codes are read block by block: the four warps of a CTA find each other's neighbours in the L1 cache)
+template <typename T, int kFmt, bool kVec>
+__global__ void __launch_bounds__(kStridedThreads) dequantize_strided_kernel(BlockView q, PlainView<T> a, int blocks) {
   using F = BlockFormat<kFmt>;
-  const int o = blockIdx.x * 32 + threadIdx.x;
-  if (o >= q.outer) return;
-  for (int b = blockIdx.y * 8 + threadIdx.y; b < blocks; b += gridDim.y * 8) {
-    T* p = a.p + o * a.so + static_cast<long long>(b) * F::kBlock * a.sl;
+  using S = StridedTile<kFmt>;
+  using P = Pair<T>;
+  const int o0 = blockIdx.x * kStridedRows;
+  const int r[2] = {o0 + strided_row<kVec>(0), o0 + strided_row<kVec>(1)};
+  for (int b = blockIdx.y * 4 + (threadIdx.x >> 5); b < blocks; b += gridDim.y * 4) {
     const int n = q.inner - b * F::kBlock;
-    const uint8_t* src = q.codes + o * q.pitch + static_cast<long long>(b) * (F::kBlock / 8 * F::kBytes8);
-    uint32_t w[F::kBlock / 8 * F::kBytes8 / 4];
-    if (F::kNv) {
-      const uint2 c = *reinterpret_cast<const uint2*>(src);
-      w[0] = c.x;
-      w[1] = c.y;
-    } else {
+    uint32_t w[2][S::kBytes / 4];
+    float scale[2];
 #pragma unroll
-      for (int j = 0; j < F::kBytes8 / 4; ++j) {
-        const uint4 c = reinterpret_cast<const uint4*>(src)[j];
-        w[4 * j] = c.x; w[4 * j + 1] = c.y; w[4 * j + 2] = c.z; w[4 * j + 3] = c.w;
+    for (int j = 0; j < 2; ++j) {
+      const uint2* src = reinterpret_cast<const uint2*>(q.codes + r[j] * q.pitch + static_cast<long long>(b) * S::kBytes);
+#pragma unroll
+      for (int i = 0; i < S::kBytes / 8; ++i) {
+        const uint2 c = r[j] < q.outer ? src[i] : make_uint2(0u, 0u);
+        w[j][2 * i] = c.x;
+        w[j][2 * i + 1] = c.y;
       }
+      scale[j] = block_scale_value<kFmt>(r[j] < q.outer ? q.scales[F::scale_at(q, r[j], b)] : 0u, q.t);
     }
-    const float scale = block_scale_value<kFmt>(q.scales[F::scale_at(q, o, b)], q.t);
+    T* p = a.p + static_cast<long long>(b) * F::kBlock * a.sl;
+    T *p0 = p + r[0] * a.so, *p1 = p + r[1] * a.so;
 #pragma unroll
-    for (int j = 0; j < F::kBlock / 8; ++j) {
-      float v[8];
-      block_decode8<kFmt>(F::k4 ? make_uint2(w[j], 0u) : make_uint2(w[2 * j], w[2 * j + 1]), scale, v);
-      if (sizeof(T) == 2) block_limit_f16<kFmt>(scale, v);
+    for (int h = 0; h < F::kBlock / 8; ++h) {
+      T v[2][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (8 * j + i < n) from_f32(v[i], p[(8 * j + i) * a.sl]);
+      for (int j = 0; j < 2; ++j) {
+        float f[8];
+        block_decode8<kFmt>(F::k4 ? make_uint2(w[j][h], 0u) : make_uint2(w[j][2 * h], w[j][2 * h + 1]), scale[j], f);
+        if (sizeof(T) == 2) block_limit_f16<kFmt>(scale[j], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) from_f32(f[i], v[j][i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const long long at = (8 * h + i) * a.sl;
+        const bool live = 8 * h + i < n;
+        if (kVec) {
+          if (live && r[0] < q.outer) *reinterpret_cast<typename P::Vec*>(p0 + at) = P::of(v[0][i], v[1][i]);
+        } else {
+          if (live && r[0] < q.outer) p0[at] = v[0][i];
+          if (live && r[1] < q.outer) p1[at] = v[1][i];
+        }
+      }
     }
   }
 }
@@ -255,10 +494,13 @@ __global__ void __launch_bounds__(256) relu_mask_strided_kernel(BlockView q, Pla
   if (o >= q.outer) return;
   for (int b = blockIdx.y * 8 + threadIdx.y; b < blocks; b += gridDim.y * 8) {
     T* p = a.p + o * a.so + b * 32ll * a.sl;
-    const uint8_t* src = q.codes + o * q.pitch + b * 32ll;
-    const int n = min(32, q.inner - b * 32);
-    for (int i = 0; i < n; ++i)
-      if (src[i] - 1u >= 0x7fu) p[i * a.sl] = T(0.0f);
+    const uint4* src = reinterpret_cast<const uint4*>(q.codes + o * q.pitch + b * 32ll);
+    const uint4 lo = src[0], hi = src[1];
+    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    const int n = q.inner - b * 32;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n && not_positive(w[i / 4] >> (8 * (i & 3)) & 0xffu)) p[i * a.sl] = T(0.0f);
   }
 }
 
@@ -266,18 +508,17 @@ __global__ void __launch_bounds__(256) relu_mask_strided_kernel(BlockView q, Pla
 struct RowGrid {
   dim3 grid, block;
 };
-// lanes per row: the number of 8-number groups, in whole blocks, over CTAs of 256 threads with as few idle lanes as
-// a power of two allows; rows over the rest, several per thread once the device is full
+// Lanes per row: its groups of 16 numbers, rounded up to 8 (four blocks of 32, whose scales leave together), over
+// CTAs of 256 threads with as few idle lanes as a power of two allows; the other threads take other rows.
 RowGrid row_grid(const DeviceCtx* c, const BlockView& q) {
-  const int groups = ((q.inner + 31) / 32) * 4;
+  const int groups = static_cast<int>((q.inner + 127ll) / 128 * 8);
   int tx = 256;
-  while (tx > 16 && (groups + tx / 2 - 1) / (tx / 2) * (tx / 2) < (groups + tx - 1) / tx * tx) tx /= 2;
-  while (tx > 4 && groups <= tx / 2) tx /= 2;
+  while (tx > 8 && (groups + tx / 2 - 1) / (tx / 2) * (tx / 2) < (groups + tx - 1) / tx * tx) tx /= 2;
   const int ty = 256 / tx;
   RowGrid r;
   r.block = dim3(tx, ty);
   const long long gx = (groups + tx - 1) / tx, rows = (static_cast<long long>(q.outer) + ty - 1) / ty;
-  const long long room = std::max(1ll, 32ll * c->sm_count / gx);
+  const long long room = std::max(1ll, 16ll * c->sm_count / gx);
   r.grid = dim3(static_cast<unsigned>(gx), static_cast<unsigned>(std::min(std::min(rows, room), 65535ll)));
   return r;
 }
@@ -288,8 +529,16 @@ RowGrid strided_grid(const BlockView& q, int blocks) {
   return r;
 }
 
-bool vectors(const void* p, long long so, long long sl, int esz) {
-  return sl == 1 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (so * esz) % 16 == 0;
+// rows that start on multiples of `bytes`
+template <typename T>
+bool aligned_rows(const PlainView<T>& a, unsigned bytes) {
+  return (reinterpret_cast<uintptr_t>(a.p) & (bytes - 1)) == 0 && (a.so * static_cast<long long>(sizeof(T))) % bytes == 0;
+}
+
+// outer rows that lie two by two in aligned vectors
+template <typename T>
+bool aligned_pairs(const BlockView& q, const PlainView<T>& a) {
+  return a.so == 1 && q.outer % 2 == 0 && a.sl % 2 == 0 && (reinterpret_cast<uintptr_t>(a.p) & (2 * sizeof(T) - 1)) == 0;
 }
 
 template <typename T, int kFmt>
@@ -297,11 +546,13 @@ int quantize_one(DeviceCtx* c, const BlockView& q, PlainView<const T> a, cudaStr
   const int blocks = (q.inner + BlockFormat<kFmt>::kBlock - 1) / BlockFormat<kFmt>::kBlock;
   if (a.sl == 1) {
     const RowGrid g = row_grid(c, q);
-    if (vectors(a.p, a.so, a.sl, sizeof(T))) quantize_rows_kernel<T, kFmt, true><<<g.grid, g.block, 0, stream>>>(q, a);
+    a.wide = aligned_rows(a, 32);
+    if (aligned_rows(a, 16)) quantize_rows_kernel<T, kFmt, true><<<g.grid, g.block, 0, stream>>>(q, a);
     else quantize_rows_kernel<T, kFmt, false><<<g.grid, g.block, 0, stream>>>(q, a);
   } else {
-    const RowGrid g = strided_grid(q, blocks);
-    quantize_strided_kernel<T, kFmt><<<g.grid, g.block, 0, stream>>>(q, a, blocks);
+    const dim3 grid((q.outer + kStridedRows - 1) / kStridedRows, std::min((blocks + 3) / 4, 65535));
+    if (aligned_pairs(q, a)) quantize_strided_kernel<T, kFmt, true><<<grid, kStridedThreads, 0, stream>>>(q, a, blocks);
+    else quantize_strided_kernel<T, kFmt, false><<<grid, kStridedThreads, 0, stream>>>(q, a, blocks);
   }
   NG_CHECK_LAUNCH();
   return NG_OK;
@@ -312,11 +563,13 @@ int dequantize_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_
   const int blocks = (q.inner + BlockFormat<kFmt>::kBlock - 1) / BlockFormat<kFmt>::kBlock;
   if (a.sl == 1) {
     const RowGrid g = row_grid(c, q);
-    if (vectors(a.p, a.so, a.sl, sizeof(T))) dequantize_rows_kernel<T, kFmt, true><<<g.grid, g.block, 0, stream>>>(q, a);
+    a.wide = aligned_rows(a, 32);
+    if (aligned_rows(a, 16)) dequantize_rows_kernel<T, kFmt, true><<<g.grid, g.block, 0, stream>>>(q, a);
     else dequantize_rows_kernel<T, kFmt, false><<<g.grid, g.block, 0, stream>>>(q, a);
   } else {
-    const RowGrid g = strided_grid(q, blocks);
-    dequantize_strided_kernel<T, kFmt><<<g.grid, g.block, 0, stream>>>(q, a, blocks);
+    const dim3 grid((q.outer + kStridedRows - 1) / kStridedRows, std::min((blocks + 3) / 4, 65535));
+    if (aligned_pairs(q, a)) dequantize_strided_kernel<T, kFmt, true><<<grid, kStridedThreads, 0, stream>>>(q, a, blocks);
+    else dequantize_strided_kernel<T, kFmt, false><<<grid, kStridedThreads, 0, stream>>>(q, a, blocks);
   }
   NG_CHECK_LAUNCH();
   return NG_OK;
@@ -327,7 +580,8 @@ int relu_mask_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_t
   const int blocks = (q.inner + 31) / 32;
   if (a.sl == 1) {
     const RowGrid g = row_grid(c, q);
-    if (vectors(a.p, a.so, a.sl, sizeof(T))) relu_mask_rows_kernel<T, true><<<g.grid, g.block, 0, stream>>>(q, a);
+    a.wide = aligned_rows(a, 32);
+    if (aligned_rows(a, 16)) relu_mask_rows_kernel<T, true><<<g.grid, g.block, 0, stream>>>(q, a);
     else relu_mask_rows_kernel<T, false><<<g.grid, g.block, 0, stream>>>(q, a);
   } else {
     const RowGrid g = strided_grid(q, blocks);

@@ -115,15 +115,29 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t amax_bits, float t) {
   return s;
 }
 
-// 8 numbers of a block to codes: 4 bytes in x (4-bit formats) or 8 in x and y
-template <int kFmt>
+// 8 numbers of a block to codes: 4 bytes in x (4-bit formats) or 8 in x and y. kHalf: they came from fp16.
+template <int kFmt, bool kHalf>
 __device__ __forceinline__ uint2 block_encode8(const float (&x)[8], const BlockScale& s) {
   float y[8];
   uint2 r = make_uint2(0u, 0u);
   if constexpr (BlockFormat<kFmt>::k4) {
+    if constexpr (!BlockFormat<kFmt>::kNv) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = BlockFormat<kFmt>::kNv ? __fdiv_rn(x[i], s.by) : x[i] * s.by;
-    if (!s.nan) r.x = cvt_e2m1x8(y);
+      for (int i = 0; i < 8; ++i) y[i] = x[i] * s.by;
+    } else if constexpr (kHalf) {
+      // An IEEE division per number made this kernel issue-bound (4096 x 9216: 34 us). The product with the
+      // reciprocal is off by 2^-23 of the quotient, which matters on the border between two codes only; rounded to a
+      // multiple of 2^-15 (the sum with 384 has that for its last bit) it is on the border when the quotient is: the
+      // border times the scale has at most 7 bits, and an fp16 number that differs from it does so by 2^-11 of it.
+      const float inv = __frcp_rn(s.by);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = fmaf(x[i], inv, 384.0f) - 384.0f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], s.by);
+    }
+    r.x = cvt_e2m1x8(y);
+    if (s.nan) r.x = 0u;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -135,6 +149,27 @@ __device__ __forceinline__ uint2 block_encode8(const float (&x)[8], const BlockS
     r.y = cvt_e4m3x2(y[4], y[5]) | (cvt_e4m3x2(y[6], y[7]) << 16);
   }
   return r;
+}
+
+// 4 fp16 numbers of a block (two per word) to mxfp8 codes, the same codes as above. `by` as two factors that fp16
+// holds (block_scale_f16): products are exact where they are not below 2^-9, the least that is encoded.
+__device__ __forceinline__ uint32_t block_encode4_f16(uint32_t x0, uint32_t x1, __half2 by0, __half2 by1) {
+  uint32_t r[2];
+  const uint32_t x[2] = {x0, x1};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const __half2 v = *reinterpret_cast<const __half2*>(&x[i]);
+    const __half2 m = __hmax2(__habs2(__hmul2(__hmul2(v, by0), by1)), __half2half2(__ushort_as_half(0x1800)));   // 2^-9
+    const uint32_t y = (*reinterpret_cast<const uint32_t*>(&m) | (x[i] & 0x80008000u)) & __hne2_mask(v, __half2half2(__ushort_as_half(0)));
+    uint16_t c;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(y));
+    r[i] = c;
+  }
+  return r[0] | (r[1] << 16);
+}
+__device__ __forceinline__ void block_scale_f16(float by, __half2& by0, __half2& by1) {
+  by0 = __float2half2_rn(fminf(by, 32768.0f));
+  by1 = __float2half2_rn(fminf(fmaxf(by * (1.0f / 32768.0f), 1.0f), 32768.0f));
 }
 
 // The scale that a stored byte stands for.
@@ -163,6 +198,33 @@ __device__ __forceinline__ void block_decode8(uint2 codes, float scale, float (&
     v[2 * i] = f.x * scale;
     v[2 * i + 1] = f.y * scale;
   }
+}
+
+// 8 codes as fp16 numbers times a scale that fp16 holds and with which nothing leaves its range: one rounding, the
+// same results as in fp32.
+template <int kFmt>
+__device__ __forceinline__ bool block_scale_fits_f16(float scale) {
+  return scale >= 6.103515625e-05f && scale * (BlockFormat<kFmt>::k4 ? 6.0f : 448.0f) <= 65504.0f;
+}
+template <int kFmt>
+__device__ __forceinline__ uint4 block_decode8_f16(uint2 codes, __half2 scale) {
+  __half2 h[4];
+  if (BlockFormat<kFmt>::k4) {
+    half2_of_e2m1x8(codes.x, h);
+  } else {
+    h[0] = half2_of_e4m3x2(codes.x & 0xffffu);
+    h[1] = half2_of_e4m3x2(codes.x >> 16);
+    h[2] = half2_of_e4m3x2(codes.y & 0xffffu);
+    h[3] = half2_of_e4m3x2(codes.y >> 16);
+  }
+  uint4 r;
+  uint32_t* w = &r.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __hmul2(h[i], scale);
+    w[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return r;
 }
 
 // The same for an fp16 result: limited to its largest number (a NaN stays one).

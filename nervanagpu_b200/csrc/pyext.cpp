@@ -22,7 +22,7 @@ namespace {
 constexpr int kMaxDims = 6;
 enum Dtype : int { kF16 = 0, kF32 = 1 };   // positions in the tuple that setup() is given
 
-PyObject *g_tensor_type, *g_node_type, *g_prepare, *g_check, *g_dtypes, *g_ops;
+PyObject *g_tensor_type, *g_node_type, *g_block_type, *g_prepare, *g_check, *g_dtypes, *g_ops;
 PyObject* g_cache;   // expression key -> Launch
 constexpr Py_ssize_t kCacheLimit = 4096;
 constexpr int kMaxArgs = 1024;   // 4 KB of kernel parameters of 4 bytes and more
@@ -560,21 +560,119 @@ PyObject* py_pool(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_TRUE;
 }
 
-// setup(tensor type, node type, prepare, check, dtypes (fp16 and fp32 first), {operation: number})
+// ------------------------------------------------------------------------------------------
+// Matrices in blocks
+// ------------------------------------------------------------------------------------------
+bool read_block(PyObject* o, ng_block_desc& d) {
+  return reinterpret_cast<PyObject*>(Py_TYPE(o)) == g_block_type && read_desc(o, d);
+}
+
+// The plain side of a matrix in blocks: its shape, fp16 or fp32.
+bool plain_matrix(PyObject* o, const ng_block_desc& d, Tensor& t) {
+  return read_tensor(o, t) && t.nd == 2 && t.shape[0] == d.rows && t.shape[1] == d.cols && (t.dtype == kF16 || t.dtype == kF32);
+}
+
+// quantize(backend, A, outs)
+PyObject* py_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  ng_block_desc d[4];
+  Tensor a;
+  void* stream;
+  if (n != 3 || !PyTuple_Check(args[2])) return decline();
+  const Py_ssize_t outs = PyTuple_GET_SIZE(args[2]);
+  if (outs < 1 || outs > 4) return decline();
+  for (Py_ssize_t i = 0; i < outs; ++i)
+    if (!read_block(PyTuple_GET_ITEM(args[2], i), d[i]) || d[i].rows != d[0].rows || d[i].cols != d[0].cols) return decline();
+  if (!plain_matrix(args[1], d[0], a) || !read_stream(args[0], stream)) return decline();
+  const int rc = without_gil([&] {
+    return ng_block_quantize(reinterpret_cast<void*>(a.ptr), a.dtype == kF16 ? 2 : 4, a.strides[0], a.strides[1], d,
+                             static_cast<int>(outs), stream);
+  });
+  if (rc != NG_OK) return failed(rc);
+  Py_RETURN_TRUE;
+}
+
+// block_plain(0 or 1, backend, Q, tensor): dequantize or relu_mask
+PyObject* py_block_plain(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  ng_block_desc d;
+  Tensor t;
+  void* stream;
+  long long what;
+  if (n != 4 || !to_ll(args[0], what) || !read_block(args[2], d) || !plain_matrix(args[3], d, t) || !read_stream(args[1], stream))
+    return decline();
+  if (what == 1 && d.format != NG_BLOCK_MXFP8) return decline();
+  void* p = reinterpret_cast<void*>(t.ptr);
+  const int esz = t.dtype == kF16 ? 2 : 4;
+  const int rc = without_gil([&] {
+    return what == 0 ? ng_block_dequantize(&d, p, esz, t.strides[0], t.strides[1], stream)
+                     : ng_block_relu_mask(&d, p, esz, t.strides[0], t.strides[1], stream);
+  });
+  if (rc != NG_OK) return failed(rc);
+  Py_RETURN_TRUE;
+}
+
+// Leading dimension of a rows x cols matrix with contiguous rows.
+bool row_major(const Tensor& t, int& ld) {
+  if (t.nd != 2 || t.shape[0] < 1 || t.shape[1] < 1 || (t.shape[1] != 1 && t.strides[1] != 1)) return false;
+  const long long v = t.shape[0] > 1 ? t.strides[0] : t.shape[1];
+  ld = static_cast<int>(v);
+  return v >= t.shape[1] && v <= 0x7fffffff;
+}
+
+// block_dot(backend, A, B, C, alpha, beta, relu, stochastic_round)
+PyObject* py_block_dot(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  ng_block_desc da, db;
+  Tensor a = {}, c;
+  float alpha, beta;
+  void* stream;
+  int lda = 0, ldc, sr = 0;
+  if (n != 8 || !read_block(args[2], db) || db.axis != 0 || !read_tensor(args[3], c) || !row_major(c, ldc)) return decline();
+  const bool blocks = reinterpret_cast<PyObject*>(Py_TYPE(args[1])) == g_block_type;
+  long long m, k;
+  if (blocks) {
+    if (!read_desc(args[1], da) || da.axis != 1 || da.format != db.format || db.format == NG_BLOCK_MXFP8) return decline();
+    m = da.rows;
+    k = da.cols;
+  } else {
+    if (db.format != NG_BLOCK_MXFP8 || !read_tensor(args[1], a) || a.dtype != kF16 || !row_major(a, lda)) return decline();
+    m = a.shape[0];
+    k = a.shape[1];
+  }
+  if (k != db.rows || m != c.shape[0] || m > 0x7fffffff || db.cols != c.shape[1] || (c.dtype != kF16 && c.dtype != kF32)) return decline();
+  const bool f32 = c.dtype == kF32;
+  if (!as_float(args[4], alpha) || !as_float(args[5], beta)) return decline();
+  const int relu = PyObject_IsTrue(args[6]);
+  if (relu < 0 || (!(f32 && args[7] == Py_None) && !rounding_bits(args[7], c, sr)) || !read_stream(args[0], stream)) return decline();
+  unsigned long long seed = 0;
+  unsigned off = 0;
+  if (sr != 0) {
+    Ref rs(PyObject_GetAttr(args[0], s_rand_state));
+    if (!rs || !next_random(rs.o, seed, off)) return decline();     // (last: it moves the random stream on)
+  }
+  void* pc = reinterpret_cast<void*>(c.ptr);
+  const int rc = without_gil([&] {
+    if (blocks) return ng_block_dot(&da, &db, pc, ldc, f32, alpha, beta, relu, sr, seed, off, stream);
+    return ng_block_dot_f16(reinterpret_cast<void*>(a.ptr), lda, &db, pc, static_cast<int>(m), ldc, f32, alpha, beta, relu, sr, seed, off, stream);
+  });
+  if (rc != NG_OK) return failed(rc);
+  Py_RETURN_TRUE;
+}
+
+// setup(tensor type, node type, block type, prepare, check, dtypes (fp16 and fp32 first), {operation: number})
 PyObject* py_setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 6 || !PyTuple_Check(args[4]) || !PyDict_Check(args[5])) {
-    PyErr_SetString(PyExc_TypeError, "setup(tensor, node, prepare, check, dtypes, ops)");
+  if (n != 7 || !PyTuple_Check(args[5]) || !PyDict_Check(args[6])) {
+    PyErr_SetString(PyExc_TypeError, "setup(tensor, node, block, prepare, check, dtypes, ops)");
     return nullptr;
   }
-  PyObject** slots[6] = {&g_tensor_type, &g_node_type, &g_prepare, &g_check, &g_dtypes, &g_ops};
-  for (int i = 0; i < 6; ++i) Py_XSETREF(*slots[i], Py_NewRef(args[i]));
+  PyObject** slots[7] = {&g_tensor_type, &g_node_type, &g_block_type, &g_prepare, &g_check, &g_dtypes, &g_ops};
+  for (int i = 0; i < 7; ++i) Py_XSETREF(*slots[i], Py_NewRef(args[i]));
   Py_RETURN_NONE;
 }
 
 #define NG_METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {NG_METHOD("setup", py_setup), NG_METHOD("node", py_node), NG_METHOD("assign", py_assign),
                            NG_METHOD("run", py_run), NG_METHOD("dot", py_dot), NG_METHOD("batched_dot", py_batched_dot),
-                           NG_METHOD("conv", py_conv), NG_METHOD("pool", py_pool), {nullptr, nullptr, 0, nullptr}};
+                           NG_METHOD("conv", py_conv), NG_METHOD("pool", py_pool), NG_METHOD("quantize", py_quantize),
+                           NG_METHOD("block_plain", py_block_plain), NG_METHOD("block_dot", py_block_dot), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

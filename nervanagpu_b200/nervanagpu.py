@@ -782,6 +782,8 @@ class NervanaGPU(object):
         """The numbers of A (fp16 or fp32, any strides), to nearest, into each of up to four matrices in blocks, of
         any formats and axes: a layer's input as an operand of its product and as the record of its backward pass, say.
         A block that holds an infinity or NaN reads back as NaN."""
+        if _native.quantize(self, A, outs):
+            return outs[0] if len(outs) == 1 else outs
         assert 1 <= len(outs) <= 4, "one to four matrices in blocks"
         for Q in outs:
             self._plain_matrix(A, Q)
@@ -794,6 +796,8 @@ class NervanaGPU(object):
 
     def dequantize(self, Q, out):
         """out = the values that Q's codes stand for (fp16: rounded, and limited to +-65504)."""
+        if _native.block_plain(0, self, Q, out):
+            return out
         self._plain_matrix(out, Q)
         _lib.check(self.lib.ng_block_dequantize(Q.desc, out.ptr, out.dtype.itemsize, out.strides[0], out.strides[1], self.stream))
         return out
@@ -802,6 +806,8 @@ class NervanaGPU(object):
         """E = Q > 0 ? E : 0 in place, Q an "mxfp8" record: the mask of the ReLU that Q is the output of, as
         E *= Q > 0 on the plain activation but that what is masked becomes 0 even from an infinity or NaN. A record
         keeps for every number whether it was positive."""
+        if _native.block_plain(1, self, Q, E):
+            return E
         self._plain_matrix(E, Q)
         if Q.format != "mxfp8":
             raise TypeError("only mxfp8 keeps which numbers were positive")
@@ -815,6 +821,8 @@ class NervanaGPU(object):
 
         With X a layer's input (features x images): block_dot(W, X4, Y, relu=True) is its forward product from 4-bit
         weights and inputs, block_dot(E, X8.T, dW) its weight gradient from the input's 8-bit record."""
+        if repeat == 1 and not self.bench and _native.block_dot(self, A, B, C, alpha, beta, relu, stochastic_round):
+            return C
         assert isinstance(B, BlockTensor), "not a matrix in blocks"
         assert A.shape[1] == B.shape[0] and len(C.shape) == 2 and C.shape == (A.shape[0], B.shape[1])
         m, n, k = A.shape[0], B.shape[1], A.shape[1]
@@ -1066,5 +1074,5 @@ class OpTreeNode(tuple):
     def __neg__(self): return _node(_OPS["neg"], self, None)
 
 
-_native.prepare = lambda module: module.setup(GPUTensor, OpTreeNode, prepare_assignment, _lib.check,
+_native.prepare = lambda module: module.setup(GPUTensor, OpTreeNode, BlockTensor, prepare_assignment, _lib.check,
                                               tuple(np.dtype(t) for t in _DTYPES), operation_numbers)
