@@ -13,7 +13,7 @@
 //
 //   warp 0     TMA producer
 //   warp 1     tensor memory, scale copies and MMAs, by one thread
-//   warps 2-5  tensor memory -> shared memory
+//   warps 2-9  tensor memory -> shared memory, two warps per group of 32 lanes
 //   all        sum over the cluster, output stage (epilogue.cuh), stores
 #include <algorithm>
 #include <atomic>
@@ -26,7 +26,7 @@ namespace ngb {
 namespace {
 
 constexpr uint32_t kCodesA = 128u * 128u;       // bytes of a k-block of A
-constexpr int kDotThreads = 192;
+constexpr int kDotThreads = 320;
 constexpr uint32_t kDotSmemLimit = 232448;      // 227 KB
 constexpr uint32_t kDotCtrl = 256;              // barriers, tensor-memory address, abort flag
 constexpr int kDotStages = 8;                   // most
@@ -49,7 +49,8 @@ struct DotTile {
   // partial tiles in shared memory: rows of kN + 4 floats, so that lanes in successive rows meet different banks
   static constexpr int kPitch = kN + 4;
   static constexpr uint32_t kSmem = kStages * kStageBytes + 1024u + kDotCtrl;
-  static_assert(128u * kPitch * 4u <= kStages * kStageBytes, "the partial tile takes the ring's place");
+  // (the partial tile takes the ring's place, and behind it, when it is split, this CTA's share of the sum)
+  static_assert(128u * kPitch * 4u * (kN > 128 ? 1 : 2) <= kStages * kStageBytes, "the ring is smaller than the tile");
 };
 
 struct DotParams {
@@ -110,10 +111,36 @@ __device__ __forceinline__ float4 load_cluster_f4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ float load_cluster_f1(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+// Sum of 4 neighbours over the kParts partial tiles of the cluster, in the order of the partitions; all loads first.
+template <int kParts>
+__device__ __forceinline__ float4 sum_parts(uint32_t at) {
+  float4 x[kParts];
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) x[i] = load_cluster_f4(map_to_cta(at, i));
+#pragma unroll
+  for (int i = 1; i < kParts; ++i) {
+    x[0].x += x[i].x; x[0].y += x[i].y; x[0].z += x[i].z; x[0].w += x[i].w;
+  }
+  return x[0];
+}
+// One output, in fp16 or fp32 (the arithmetic of epi_store8).
+__device__ __forceinline__ void epi_store1(const EpiArgs& e, float acc, void* out, int out_f32, unsigned long long lin) {
+  float c = epi_scale(e, acc);
+  if (out_f32) {
+    float* p = static_cast<float*>(out);
+    if (e.beta != 0.0f) c = fmaf(e.beta, *p, c);
+    *p = c;
+    return;
+  }
+  __half* p = static_cast<__half*>(out);
+  if (e.beta != 0.0f) c = fmaf(e.beta, __half2float(*p), c);
+  if (e.sr_bits) {
+    uint32_t rnd[8];
+    sr_bits8(e, lin >> 3, rnd);
+    *p = f2h_sr(c, rnd[lin & 7ull], e.sr_bits);
+  } else {
+    *p = f2h_rn(c);
+  }
 }
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t n;
@@ -238,18 +265,22 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
     const bool ok = mbar_wait(acc_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
     if (ok && !*abort_flag) {
       tc_fence_after();
-      const int group = warp & 3;
+      const int group = warp & 3, half = (warp - 2) >> 2;
       float* row = reinterpret_cast<float*>(ring_gen) + (group * 32 + lane) * T::kPitch;
       const uint32_t taddr = tmem + (static_cast<uint32_t>(group * 32) << 16);
-      if constexpr (kN < 32) {
-        uint32_t r[16];
-        tc_ld_32x16(taddr, r);
-        tc_wait_ld();
+      if constexpr (kN < 64) {
+        // 16 columns each (a tile of 16: the first of the two warps)
+        if (half * 16 < kN) {
+          uint32_t r[16];
+          tc_ld_32x16(taddr + half * 16, r);
+          tc_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) reinterpret_cast<uint4*>(row)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+          for (int j = 0; j < 4; ++j)
+            reinterpret_cast<uint4*>(row + half * 16)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        }
       } else {
 #pragma unroll 1
-        for (int c = 0; c < kN; c += 32) {
+        for (int c = half * (kN / 2); c < (half + 1) * (kN / 2); c += 32) {
           uint32_t r[32];
           tc_ld_32x32(taddr + c, r);
           tc_wait_ld();
@@ -269,43 +300,61 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
   if (splits > 1) cluster_sync_all();
 
   // This CTA's share of the tile: 128 / splits rows, summed over the cluster.
-  // (a partition that gave up leaves the tile unwritten only in its own share: the status word tells)
-  if (!*abort_flag) {
-    const int rows = 128 / splits, r0 = static_cast<int>(rank) * rows;
-    auto finish = [&](float (&v)[8], long long row, int col, int ncols, int nvalid) {
-      // 8 neighbours of C's row `row` from column `col` on
-      const unsigned long long lin = static_cast<unsigned long long>(row) * ncols + col;
+  // (when a partition gave up, its share is not written and the others hold what was there: the status word tells)
+  const int rows = 128 / splits, r0 = static_cast<int>(rank) * rows;
+  const bool whole = !p.swapped && p.vec_ok;        // rows of whole aligned vectors of C
+  const bool ok = !*abort_flag;
+  const int live = max(0, min(rows, p.M - m0 - r0));
+  auto parts = [&](uint32_t at) {
+    switch (splits) {
+      case 1: return sum_parts<1>(at);
+      case 2: return sum_parts<2>(at);
+      case 4: return sum_parts<4>(at);
+      default: return sum_parts<8>(at);
+    }
+  };
+  if (ok && whole) {
+    for (int i = threadIdx.x; i < live * (kN / 8); i += kDotThreads) {
+      const int r = r0 + i / (kN / 8), c = (i % (kN / 8)) * 8;
+      const int row = m0 + r, col = n0 + c;
+      if (col >= p.N) continue;
+      const uint32_t at = ring + (r * T::kPitch + c) * 4u;
+      const float4 x = parts(at), y = parts(at + 16u);
+      float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      const unsigned long long lin = static_cast<unsigned long long>(row) * p.N + col;
+      const int nvalid = min(8, p.N - col);
       uint8_t* crow = static_cast<uint8_t*>(p.C) + row * p.ldc * (p.out_f32 ? 4 : 2);
-      if (p.out_f32) epi_store8<true>(p.ea, v, crow, crow, col, lin, nvalid, p.vec_ok != 0);
-      else epi_store8<false>(p.ea, v, crow, crow, col, lin, nvalid, p.vec_ok != 0);
-    };
+      if (p.out_f32) epi_store8<true>(p.ea, v, crow, crow, col, lin, nvalid, true);
+      else epi_store8<false>(p.ea, v, crow, crow, col, lin, nvalid, true);
+    }
+  } else if (ok) {
+    // C's rows are at any address, or run down the tile: one output per lane and access
+    uint32_t at0 = ring + r0 * T::kPitch * 4u;
+    const float* sum = reinterpret_cast<const float*>(ring_gen) + r0 * T::kPitch;
+    if (splits > 1) {
+      sum = reinterpret_cast<const float*>(ring_gen) + 128 * T::kPitch;
+      for (int i = threadIdx.x; i < live * (kN / 4); i += kDotThreads) {
+        const int off = i / (kN / 4) * T::kPitch + i % (kN / 4) * 4;
+        *reinterpret_cast<float4*>(const_cast<float*>(sum) + off) = parts(at0 + off * 4u);
+      }
+      __syncthreads();
+    }
+    const int cols = min(kN, p.N - n0);
     if (!p.swapped) {
-      for (int i = threadIdx.x; i < rows * (kN / 8); i += kDotThreads) {
-        const int r = r0 + i / (kN / 8), c = (i % (kN / 8)) * 8;
-        const int row = m0 + r, col = n0 + c;
-        if (row >= p.M || col >= p.N) continue;
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        const uint32_t at = ring + (r * T::kPitch + c) * 4u;
-        for (uint32_t s = 0; s < splits; ++s) {
-          const uint32_t src = map_to_cta(at, s);
-          const float4 x = load_cluster_f4(src), y = load_cluster_f4(src + 16u);
-          v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-          v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-        }
-        finish(v, row, col, p.N, min(8, p.N - col));
+      for (int i = threadIdx.x; i < live * kN; i += kDotThreads) {
+        const int r = i / kN, c = i % kN;
+        const long long row = m0 + r0 + r;
+        if (c < cols)
+          epi_store1(p.ea, sum[r * T::kPitch + c], static_cast<uint8_t*>(p.C) + (row * p.ldc + n0 + c) * (p.out_f32 ? 4 : 2), p.out_f32,
+                     static_cast<unsigned long long>(row) * p.N + n0 + c);
       }
     } else {
-      for (int i = threadIdx.x; i < kN * (rows / 8); i += kDotThreads) {
-        const int c = i / (rows / 8), r = r0 + (i % (rows / 8)) * 8;
-        const int row = n0 + c, col = m0 + r;      // of C
-        if (row >= p.N || col >= p.M) continue;
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t s = 0; s < splits; ++s) {
-          const uint32_t src = map_to_cta(ring + (r * T::kPitch + c) * 4u, s);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] += load_cluster_f1(src + j * T::kPitch * 4u);
-        }
-        finish(v, row, col, p.M, min(8, p.M - col));
+      for (int i = threadIdx.x; i < cols * rows; i += kDotThreads) {
+        const int c = i / rows, r = i - c * rows;       // (a row and a column of C)
+        const long long row = n0 + c;
+        if (r < live)
+          epi_store1(p.ea, sum[r * T::kPitch + c], static_cast<uint8_t*>(p.C) + (row * p.ldc + m0 + r0 + r) * (p.out_f32 ? 4 : 2), p.out_f32,
+                     static_cast<unsigned long long>(row) * p.M + m0 + r0 + r);
       }
     }
   }
@@ -413,7 +462,7 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   if (cols > 128) cols = static_cast<long long>(p.tiles_m) * ((p.N + 255) / 256) >= c->sm_count ? 256 : 128;
   const long long tiles = static_cast<long long>(p.tiles_m) * ((p.N + cols - 1) / cols);
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= c->sm_count && p.num_kb >= splits * 4) splits *= 2;
+  while (splits < 8 && tiles * splits * 2 <= c->sm_count && p.num_kb >= splits * 2) splits *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define NG_DOT(kn) (nv ? launch_dot<kn, true>(c, a, b, p, splits, s) : launch_dot<kn, false>(c, a, b, p, splits, s))
   switch (cols) {

@@ -31,6 +31,10 @@ __device__ __forceinline__ void from_f32(float v, __half& x) { x = __float2half_
 __device__ __forceinline__ void from_f32(float v, float& x) { x = v; }
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+#define NG_DEPENDENT_PROLOGUE(early) \
+  grid_dependency_wait();            \
+  if (early) grid_launch_dependents()
+
 // ---- rows form: 16 numbers per lane ------------------------------------------------------------------
 constexpr int kLane = 16;
 
@@ -157,7 +161,8 @@ __device__ __forceinline__ void warp_store(T* base, long long so, long long o_fi
   const long long step = static_cast<long long>(gridDim.y) * blockDim.y
 
 template <typename T, int kFmt, bool kVec>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(BlockView q, PlainView<const T> a) {
+__global__ void __launch_bounds__(256) quantize_rows_kernel(BlockView q, PlainView<const T> a, int early) {
+  NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
   NG_ROWS_PROLOGUE(T);
   constexpr int kUnroll = kVec ? 2 : 1;       // rows whose loads are in flight together
@@ -217,7 +222,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(BlockView q, PlainVi
 }
 
 template <typename T, int kFmt, bool kVec>
-__global__ void __launch_bounds__(256) dequantize_rows_kernel(BlockView q, PlainView<T> a) {
+__global__ void __launch_bounds__(256) dequantize_rows_kernel(BlockView q, PlainView<T> a, int early) {
+  NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
   NG_ROWS_PROLOGUE(T);
   constexpr int kShare = F::kNv ? 1 : 2;
@@ -271,7 +277,8 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(BlockView q, Plain
 __device__ __forceinline__ bool not_positive(uint32_t code) { return code - 1u >= 0x7fu; }
 
 template <typename T, bool kVec>
-__global__ void __launch_bounds__(256) relu_mask_rows_kernel(BlockView q, PlainView<T> a) {
+__global__ void __launch_bounds__(256) relu_mask_rows_kernel(BlockView q, PlainView<T> a, int early) {
+  NG_DEPENDENT_PROLOGUE(early);
   const int tid = threadIdx.x + threadIdx.y * blockDim.x, lane = tid & 31;
   const int log_tx = min(31 - __clz(blockDim.x), 5);
   const int g = blockIdx.x * blockDim.x + threadIdx.x, n = q.inner - g * kLane;
@@ -372,7 +379,8 @@ __device__ __forceinline__ int strided_row(int j) {
 }
 
 template <typename T, int kFmt, bool kVec>
-__global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(BlockView q, PlainView<const T> a, int blocks) {
+__global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(BlockView q, PlainView<const T> a, int early, int blocks) {
+  NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
   using S = StridedTile<kFmt>;
   using P = Pair<T>;
@@ -439,7 +447,8 @@ __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(Block
 
 // (codes are read block by block: the four warps of a CTA find each other's neighbours in the L1 cache)
 template <typename T, int kFmt, bool kVec>
-__global__ void __launch_bounds__(kStridedThreads) dequantize_strided_kernel(BlockView q, PlainView<T> a, int blocks) {
+__global__ void __launch_bounds__(kStridedThreads) dequantize_strided_kernel(BlockView q, PlainView<T> a, int early, int blocks) {
+  NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
   using S = StridedTile<kFmt>;
   using P = Pair<T>;
@@ -489,7 +498,8 @@ __global__ void __launch_bounds__(kStridedThreads) dequantize_strided_kernel(Blo
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) relu_mask_strided_kernel(BlockView q, PlainView<T> a, int blocks) {
+__global__ void __launch_bounds__(256) relu_mask_strided_kernel(BlockView q, PlainView<T> a, int early, int blocks) {
+  NG_DEPENDENT_PROLOGUE(early);
   const int o = blockIdx.x * 32 + threadIdx.x;
   if (o >= q.outer) return;
   for (int b = blockIdx.y * 8 + threadIdx.y; b < blocks; b += gridDim.y * 8) {
@@ -508,6 +518,32 @@ __global__ void __launch_bounds__(256) relu_mask_strided_kernel(BlockView q, Pla
 struct RowGrid {
   dim3 grid, block;
 };
+template <typename K, typename V>
+cudaError_t launch_with(const cudaLaunchConfig_t& cfg, K kernel, int early, const BlockView& q, const V& a) {
+  return cudaLaunchKernelEx(&cfg, kernel, q, a, early);
+}
+template <typename K, typename V>
+cudaError_t launch_with(const cudaLaunchConfig_t& cfg, K kernel, int early, const BlockView& q, const V& a, int blocks) {
+  return cudaLaunchKernelEx(&cfg, kernel, q, a, early, blocks);
+}
+// Set up while the kernel before it in the stream drains; the kernel after it may do the same at once (`early`) where
+// this one's blocks are all resident from the start, so that the next one's take no room from those still to come.
+template <typename... P, typename... A>
+int launch(const DeviceCtx* c, void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t stream, const BlockView& q, A... rest) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = tuning().dependent_launch != 0 ? 1 : 0;
+  const int early = static_cast<long long>(grid.x) * grid.y <= 2ll * c->sm_count;
+  NG_CUDA(launch_with(cfg, kernel, early, q, rest...));
+  NG_CHECK_LAUNCH();
+  return NG_OK;
+}
 // Lanes per row: its groups of 16 numbers, rounded up to 8 (four blocks of 32, whose scales leave together), over
 // CTAs of 256 threads with as few idle lanes as a power of two allows; the other threads take other rows.
 RowGrid row_grid(const DeviceCtx* c, const BlockView& q) {
@@ -544,51 +580,51 @@ bool aligned_pairs(const BlockView& q, const PlainView<T>& a) {
 template <typename T, int kFmt>
 int quantize_one(DeviceCtx* c, const BlockView& q, PlainView<const T> a, cudaStream_t stream) {
   const int blocks = (q.inner + BlockFormat<kFmt>::kBlock - 1) / BlockFormat<kFmt>::kBlock;
+  int rc;
   if (a.sl == 1) {
     const RowGrid g = row_grid(c, q);
     a.wide = aligned_rows(a, 32);
-    if (aligned_rows(a, 16)) quantize_rows_kernel<T, kFmt, true><<<g.grid, g.block, 0, stream>>>(q, a);
-    else quantize_rows_kernel<T, kFmt, false><<<g.grid, g.block, 0, stream>>>(q, a);
+    if (aligned_rows(a, 16)) rc = launch(c, quantize_rows_kernel<T, kFmt, true>, g.grid, g.block, stream, q, a);
+    else rc = launch(c, quantize_rows_kernel<T, kFmt, false>, g.grid, g.block, stream, q, a);
   } else {
     const dim3 grid((q.outer + kStridedRows - 1) / kStridedRows, std::min((blocks + 3) / 4, 65535));
-    if (aligned_pairs(q, a)) quantize_strided_kernel<T, kFmt, true><<<grid, kStridedThreads, 0, stream>>>(q, a, blocks);
-    else quantize_strided_kernel<T, kFmt, false><<<grid, kStridedThreads, 0, stream>>>(q, a, blocks);
+    if (aligned_pairs(q, a)) rc = launch(c, quantize_strided_kernel<T, kFmt, true>, grid, dim3(kStridedThreads), stream, q, a, blocks);
+    else rc = launch(c, quantize_strided_kernel<T, kFmt, false>, grid, dim3(kStridedThreads), stream, q, a, blocks);
   }
-  NG_CHECK_LAUNCH();
-  return NG_OK;
+  return rc;
 }
 
 template <typename T, int kFmt>
 int dequantize_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_t stream) {
   const int blocks = (q.inner + BlockFormat<kFmt>::kBlock - 1) / BlockFormat<kFmt>::kBlock;
+  int rc;
   if (a.sl == 1) {
     const RowGrid g = row_grid(c, q);
     a.wide = aligned_rows(a, 32);
-    if (aligned_rows(a, 16)) dequantize_rows_kernel<T, kFmt, true><<<g.grid, g.block, 0, stream>>>(q, a);
-    else dequantize_rows_kernel<T, kFmt, false><<<g.grid, g.block, 0, stream>>>(q, a);
+    if (aligned_rows(a, 16)) rc = launch(c, dequantize_rows_kernel<T, kFmt, true>, g.grid, g.block, stream, q, a);
+    else rc = launch(c, dequantize_rows_kernel<T, kFmt, false>, g.grid, g.block, stream, q, a);
   } else {
     const dim3 grid((q.outer + kStridedRows - 1) / kStridedRows, std::min((blocks + 3) / 4, 65535));
-    if (aligned_pairs(q, a)) dequantize_strided_kernel<T, kFmt, true><<<grid, kStridedThreads, 0, stream>>>(q, a, blocks);
-    else dequantize_strided_kernel<T, kFmt, false><<<grid, kStridedThreads, 0, stream>>>(q, a, blocks);
+    if (aligned_pairs(q, a)) rc = launch(c, dequantize_strided_kernel<T, kFmt, true>, grid, dim3(kStridedThreads), stream, q, a, blocks);
+    else rc = launch(c, dequantize_strided_kernel<T, kFmt, false>, grid, dim3(kStridedThreads), stream, q, a, blocks);
   }
-  NG_CHECK_LAUNCH();
-  return NG_OK;
+  return rc;
 }
 
 template <typename T>
 int relu_mask_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_t stream) {
   const int blocks = (q.inner + 31) / 32;
+  int rc;
   if (a.sl == 1) {
     const RowGrid g = row_grid(c, q);
     a.wide = aligned_rows(a, 32);
-    if (aligned_rows(a, 16)) relu_mask_rows_kernel<T, true><<<g.grid, g.block, 0, stream>>>(q, a);
-    else relu_mask_rows_kernel<T, false><<<g.grid, g.block, 0, stream>>>(q, a);
+    if (aligned_rows(a, 16)) rc = launch(c, relu_mask_rows_kernel<T, true>, g.grid, g.block, stream, q, a);
+    else rc = launch(c, relu_mask_rows_kernel<T, false>, g.grid, g.block, stream, q, a);
   } else {
     const RowGrid g = strided_grid(q, blocks);
-    relu_mask_strided_kernel<T><<<g.grid, g.block, 0, stream>>>(q, a, blocks);
+    rc = launch(c, relu_mask_strided_kernel<T>, g.grid, g.block, stream, q, a, blocks);
   }
-  NG_CHECK_LAUNCH();
-  return NG_OK;
+  return rc;
 }
 
 #define NG_BY_FORMAT(fmt, call)                                   \
