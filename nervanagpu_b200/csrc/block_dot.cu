@@ -2,16 +2,17 @@
 //
 // 4-bit x 4-bit (block_dot_kernel): C = epilogue(sum_k A[i,k] B[k,j]) on tcgen05.mma.kind::mxf4nvf4, which takes the
 // packed codes from shared memory and the scales of both operands from tensor memory, multiplies each block's
-// products by its two scales and accumulates in fp32. Both operands lie along the sum in rows of 128-byte units, so
-// one TMA box of [rows][128 bytes] is a k-block of 256 numbers (four MMAs of 64), and its scales, laid out at
-// quantisation as tensor memory holds them, are one plain bulk copy into shared memory and one tcgen05.cp per 512
-// bytes from there.
+// products by its two scales and accumulates in fp32. Both operands lie in memory as shared memory holds them: a k-block
+// of 256 numbers (four MMAs of 64) of 128 rows is one bulk copy of 16 KB, its scales one of 1 or 2 KB, and a tcgen05.cp
+// per 512 bytes takes these to tensor memory.
 //
 // A CTA computes a tile of 128 rows x kN columns (kN from 16 to 256). Few tiles are split along the sum over the
-// CTAs of a thread-block cluster, which add their partial tiles up over distributed shared memory in the order of the
-// partitions: one launch, no scratch memory, the same bits every time.
+// CTAs of a thread-block cluster. Each of them then gets a share of the tile's rows from all the others by bulk copies
+// between their shared memories and adds them up in the order of the partitions: one launch, no scratch memory, the
+// same bits every time. (Fetched by loads from the others' shared memory instead, the partial tiles of 4096 x 128 x
+// 9216 took 3.8 us of 12.2.)
 //
-//   warp 0     TMA producer
+//   warp 0     producer (the first loads leave before tensor memory is allocated)
 //   warp 1     tensor memory, scale copies and MMAs, by one thread
 //   warps 2-9  tensor memory -> shared memory, two warps per group of 32 lanes
 //   all        sum over the cluster, output stage (epilogue.cuh), stores
@@ -57,9 +58,12 @@ struct DotParams {
   int M, N;                  // rows of the two operands
   int num_kb;
   int tiles_m;
+  const uint8_t *ca, *cb;    // codes
   const uint8_t *sa, *sb;    // scales
+  long long pitch_a, pitch_b;    // bytes of a row of tiles of codes
+  int tile_a, tile_b;        // bytes of a tile of codes
   long long spitch;          // bytes of a row of scale tiles (the same for both: one format, one length)
-  int sa_tiles, sb_tiles;    // rows of scale tiles that exist
+  int b_tiles;               // rows of tiles of B that exist
   uint32_t idesc;
   void* C;
   long long ldc;
@@ -106,23 +110,14 @@ __device__ __forceinline__ void tc_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ float4 load_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
+// bytes of this CTA's shared memory to another's (or its own), counted on a barrier there
+__device__ __forceinline__ void bulk_push(uint32_t dst_cluster, uint32_t src, uint32_t bytes, uint32_t bar_cluster) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst_cluster),
+               "r"(src), "r"(bytes), "r"(bar_cluster)
+               : "memory");
 }
-// Sum of 4 neighbours over the kParts partial tiles of the cluster, in the order of the partitions; all loads first.
-template <int kParts>
-__device__ __forceinline__ float4 sum_parts(uint32_t at) {
-  float4 x[kParts];
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) x[i] = load_cluster_f4(map_to_cta(at, i));
-#pragma unroll
-  for (int i = 1; i < kParts; ++i) {
-    x[0].x += x[i].x; x[0].y += x[i].y; x[0].z += x[i].z; x[0].w += x[i].w;
-  }
-  return x[0];
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // One output, in fp16 or fp32 (the arithmetic of epi_store8).
 __device__ __forceinline__ void epi_store1(const EpiArgs& e, float acc, void* out, int out_f32, unsigned long long lin) {
   float c = epi_scale(e, acc);
@@ -149,9 +144,7 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 
 template <int kN, bool kNv>
-__global__ void __launch_bounds__(kDotThreads, 1)
-block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
-                 const __grid_constant__ DotParams p) {
+__global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_constant__ DotParams p) {
   using T = DotTile<kN, kNv>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -159,29 +152,54 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
   uint8_t* ring_gen = smem_raw + (ring - smem_u32(smem_raw));
   auto full_bar = [&](int s) { return ctrl + 8u * s; };
   auto empty_bar = [&](int s) { return ctrl + 8u * (kDotStages + s); };
-  const uint32_t acc_bar = ctrl + 8u * (2 * kDotStages);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_gen + T::kStages * T::kStageBytes + 8 * (2 * kDotStages + 1));
+  const uint32_t acc_bar = ctrl + 8u * (2 * kDotStages), part_bar = acc_bar + 8u;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_gen + T::kStages * T::kStageBytes + 8 * (2 * kDotStages + 2));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t splits = cluster_size(), rank = cluster_cta_rank();
+  const int splits = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_cta_rank());
   const int tile = blockIdx.x / splits;
   const int m0 = (tile % p.tiles_m) * 128, n0 = (tile / p.tiles_m) * kN;
   const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * rank / splits);
   const int count = static_cast<int>(static_cast<long long>(p.num_kb) * (rank + 1) / splits) - kb0;
+  // this CTA's share of the tile, and where the partitions' parts of it arrive (behind the tile itself)
+  const int rows = 128 / splits, r0 = rank * rows;
+  const uint32_t share_bytes = static_cast<uint32_t>(rows) * T::kPitch * 4u;
+  const uint32_t parts = ring + 128u * T::kPitch * 4u;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < T::kStages; ++s) {
-      mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+  // k-block i of this partition into slot i % kStages
+  const int rt = m0 / 128, ct = n0 / 128;
+  const int ct_live = min(T::kRowTiles, p.b_tiles - ct);    // (the last column tile may reach beyond B's rows)
+  auto load_kb = [&](int i) {
+    const int s = i % T::kStages;
+    const uint32_t a = ring + s * T::kStageBytes, b = a + kCodesA, sa = b + T::kCodesB, sb = sa + T::kScalesA;
+    const long long kb = kb0 + i;
+    constexpr uint32_t kB = (kN < 128 ? kN : 128) * 128u;      // (a tile of B: with up to 64 columns, B has as many rows as they are padded to)
+    mbar_expect_tx(full_bar(s), p.tile_a + T::kScalesA + ct_live * (kB + T::kScalesA));
+    bulk_load(a, p.ca + rt * p.pitch_a + kb * p.tile_a, p.tile_a, full_bar(s));
+    bulk_load(sa, p.sa + rt * p.spitch + kb * T::kScalesA, T::kScalesA, full_bar(s));
+    for (int c = 0; c < ct_live; ++c) {
+      bulk_load(b + c * kB, p.cb + (ct + c) * p.pitch_b + kb * p.tile_b, kB, full_bar(s));
+      bulk_load(sb + c * T::kScalesA, p.sb + (ct + c) * p.spitch + kb * T::kScalesA, T::kScalesA, full_bar(s));
     }
-    mbar_init(acc_bar, 1);
-    *abort_flag = 0;
-    mbar_fence_init();
-    tma_prefetch_desc(&mapA);
-    tma_prefetch_desc(&mapB);
-  }
-  if (warp == 1) {
+  };
+  const int first = min(count, T::kStages);      // k-blocks that need no free slot
+  if (warp == 0) {
+    if (elect_one()) {
+      for (int s = 0; s < T::kStages; ++s) {
+        mbar_init(full_bar(s), 1);
+        mbar_init(empty_bar(s), 1);
+      }
+      mbar_init(acc_bar, 1);
+      mbar_init(part_bar, 1);
+      *abort_flag = 0;
+      mbar_fence_init();
+      if (splits > 1) mbar_expect_tx(part_bar, (splits - 1) * share_bytes);
+      grid_dependency_wait();
+      for (int i = 0; i < first; ++i) load_kb(i);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), T::kCols);
     tmem_relinquish();
   }
@@ -193,31 +211,16 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
 
   if (warp == 0) {
     if (elect_one()) {
-      const int rt = m0 / 128, ct = n0 / 128;
-      const int ct_live = min(T::kRowTiles, p.sb_tiles - ct);    // (the last column tile may reach beyond B's scales)
-      const uint32_t tx = kCodesA + T::kCodesB + T::kScalesA * (1 + ct_live);
-      int i = 0;
-      bool ok = true;
+      int i = first;
       for (; i < count; ++i) {
-        const int s = i % T::kStages, lap = i / T::kStages;
-        if (lap > 0 && !mbar_wait(empty_bar(s), (lap - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns)) {
-          ok = false;
+        if (!mbar_wait(empty_bar(i % T::kStages), (i / T::kStages - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns)) {
+          // given up: the loads in flight must land before the CTA may end
+          int none = 0;
+          for (int j = i - T::kStages; j < i; ++j)
+            mbar_wait(full_bar(j % T::kStages), (j / T::kStages) & 1, &none, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns);
           break;
         }
-        const uint32_t a = ring + s * T::kStageBytes, b = a + kCodesA, sa = b + T::kCodesB, sb = sa + T::kScalesA;
-        const int kb = kb0 + i;
-        mbar_expect_tx(full_bar(s), tx);
-        tma_load_5d(a, &mapA, full_bar(s), kb * 64, m0, 0, 0, 0);
-        tma_load_5d(b, &mapB, full_bar(s), kb * 64, n0, 0, 0, 0);
-        const long long koff = static_cast<long long>(kb) * T::kScalesA;
-        bulk_load(sa, p.sa + rt * p.spitch + koff, T::kScalesA, full_bar(s));
-        for (int c = 0; c < ct_live; ++c) bulk_load(sb + c * T::kScalesA, p.sb + (ct + c) * p.spitch + koff, T::kScalesA, full_bar(s));
-      }
-      // given up: the loads in flight must land before the CTA may end
-      if (!ok) {
-        int none = 0;
-        for (int j = max(0, i - T::kStages); j < i; ++j)
-          mbar_wait(full_bar(j % T::kStages), (j / T::kStages) & 1, &none, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns);
+        load_kb(i);
       }
     }
     __syncwarp();
@@ -225,7 +228,6 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
     if (elect_one()) {
       const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);     // 8 rows of 128 bytes apart, version 1, 128-byte swizzle
       const uint32_t scales = tmem + T::kAccCols;
-      const uint32_t b_shift = static_cast<uint32_t>(n0 % 128) / 32u;   // columns of the scale tile before this tile's first
       bool ok = true;
       for (int i = 0; i < count; ++i) {
         const int s = i % T::kStages;
@@ -249,7 +251,7 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
           const uint64_t db = (static_cast<uint64_t>(hi) << 32) | (1u << 16) | ((b + 32u * j) >> 4);
           const int t = kNv ? j : j / 2;
           const uint32_t id = kNv ? 0u : (j & 1) * 2u;       // which of the tile's four scales are this MMA's first
-          tc_mma_blocks<kNv>(tmem, da, db, p.idesc | (id << 4) | (id << 29), ta + t * 4, tb + t * T::kRowTiles * 4 + b_shift,
+          tc_mma_blocks<kNv>(tmem, da, db, p.idesc | (id << 4) | (id << 29), ta + t * 4, tb + t * T::kRowTiles * 4,
                              (i | j) != 0);
         }
         tc_commit(empty_bar(s));
@@ -261,9 +263,14 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
       }
     }
     __syncwarp();
+  }
+  if (warp < 2) {
+    if (splits > 1) cluster_arrive();
   } else {
-    const bool ok = mbar_wait(acc_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
-    if (ok && !*abort_flag) {
+    const bool done = mbar_wait(acc_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
+    __syncwarp();
+    if (splits > 1) cluster_arrive();      // (with everybody's: all rings are idle, parts may arrive there)
+    if (done && !*abort_flag) {
       tc_fence_after();
       const int group = warp & 3, half = (warp - 2) >> 2;
       float* row = reinterpret_cast<float*>(ring_gen) + (group * 32 + lane) * T::kPitch;
@@ -291,35 +298,51 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
       }
       tc_fence_before();
     }
+    fence_async_smem();      // (the parts leave by bulk copies)
   }
   __syncthreads();
+  if (splits > 1) {
+    cluster_wait();
+    if (warp == 0 && elect_one()) {
+      for (int d = 1; d < splits; ++d) {
+        const int to = (rank + d) % splits;
+        bulk_push(map_to_cta(parts + rank * share_bytes, to), ring + to * share_bytes, share_bytes, map_to_cta(part_bar, to));
+      }
+    }
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, T::kCols);
   }
-  if (splits > 1) cluster_sync_all();
+  if (splits > 1) {
+    mbar_wait(part_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
+    __syncwarp();
+    cluster_arrive();        // (with everybody's: all parts have arrived, nobody's tile is read any more)
+    __syncthreads();         // the abort flag is final
+  }
 
-  // This CTA's share of the tile: 128 / splits rows, summed over the cluster.
-  // (when a partition gave up, its share is not written and the others hold what was there: the status word tells)
-  const int rows = 128 / splits, r0 = static_cast<int>(rank) * rows;
+  // The sum over the partitions, in their order, and the output stage. (When a partition gave up, the others' shares
+  // hold what was there: the status word tells.)
   const bool whole = !p.swapped && p.vec_ok;        // rows of whole aligned vectors of C
-  const bool ok = !*abort_flag;
   const int live = max(0, min(rows, p.M - m0 - r0));
-  auto parts = [&](uint32_t at) {
-    switch (splits) {
-      case 1: return sum_parts<1>(at);
-      case 2: return sum_parts<2>(at);
-      case 4: return sum_parts<4>(at);
-      default: return sum_parts<8>(at);
+  const float* own = reinterpret_cast<const float*>(ring_gen) + r0 * T::kPitch;
+  const float* others = reinterpret_cast<const float*>(ring_gen) + 128 * T::kPitch;
+  auto sum4 = [&](int off) {
+    float4 v = *reinterpret_cast<const float4*>((rank == 0 ? own : others) + off);
+    for (int s = 1; s < splits; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>((s == rank ? own : others + s * rows * T::kPitch) + off);
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
     }
+    return v;
   };
-  if (ok && whole) {
+  if (*abort_flag) {
+  } else if (whole) {
     for (int i = threadIdx.x; i < live * (kN / 8); i += kDotThreads) {
-      const int r = r0 + i / (kN / 8), c = (i % (kN / 8)) * 8;
-      const int row = m0 + r, col = n0 + c;
+      const int r = i / (kN / 8), c = (i % (kN / 8)) * 8;
+      const int col = n0 + c;
+      const long long row = m0 + r0 + r;
       if (col >= p.N) continue;
-      const uint32_t at = ring + (r * T::kPitch + c) * 4u;
-      const float4 x = parts(at), y = parts(at + 16u);
+      const float4 x = sum4(r * T::kPitch + c), y = sum4(r * T::kPitch + c + 4);
       float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
       const unsigned long long lin = static_cast<unsigned long long>(row) * p.N + col;
       const int nvalid = min(8, p.N - col);
@@ -327,15 +350,12 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
       if (p.out_f32) epi_store8<true>(p.ea, v, crow, crow, col, lin, nvalid, true);
       else epi_store8<false>(p.ea, v, crow, crow, col, lin, nvalid, true);
     }
-  } else if (ok) {
+  } else {
     // C's rows are at any address, or run down the tile: one output per lane and access
-    uint32_t at0 = ring + r0 * T::kPitch * 4u;
-    const float* sum = reinterpret_cast<const float*>(ring_gen) + r0 * T::kPitch;
     if (splits > 1) {
-      sum = reinterpret_cast<const float*>(ring_gen) + 128 * T::kPitch;
       for (int i = threadIdx.x; i < live * (kN / 4); i += kDotThreads) {
         const int off = i / (kN / 4) * T::kPitch + i % (kN / 4) * 4;
-        *reinterpret_cast<float4*>(const_cast<float*>(sum) + off) = parts(at0 + off * 4u);
+        *reinterpret_cast<float4*>(const_cast<float*>(own) + off) = sum4(off);
       }
       __syncthreads();
     }
@@ -345,7 +365,7 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
         const int r = i / kN, c = i % kN;
         const long long row = m0 + r0 + r;
         if (c < cols)
-          epi_store1(p.ea, sum[r * T::kPitch + c], static_cast<uint8_t*>(p.C) + (row * p.ldc + n0 + c) * (p.out_f32 ? 4 : 2), p.out_f32,
+          epi_store1(p.ea, own[r * T::kPitch + c], static_cast<uint8_t*>(p.C) + (row * p.ldc + n0 + c) * (p.out_f32 ? 4 : 2), p.out_f32,
                      static_cast<unsigned long long>(row) * p.N + n0 + c);
       }
     } else {
@@ -353,30 +373,18 @@ block_dot_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
         const int c = i / rows, r = i - c * rows;       // (a row and a column of C)
         const long long row = n0 + c;
         if (r < live)
-          epi_store1(p.ea, sum[r * T::kPitch + c], static_cast<uint8_t*>(p.C) + (row * p.ldc + m0 + r0 + r) * (p.out_f32 ? 4 : 2), p.out_f32,
+          epi_store1(p.ea, own[r * T::kPitch + c], static_cast<uint8_t*>(p.C) + (row * p.ldc + m0 + r0 + r) * (p.out_f32 ? 4 : 2), p.out_f32,
                      static_cast<unsigned long long>(row) * p.M + m0 + r0 + r);
       }
     }
   }
-  if (splits > 1) cluster_sync_all();     // the others may still be reading this CTA's partial tile
-}
-
-// [rows][128 bytes] boxes of a matrix's codes (as 16-bit units), zeros beyond its last row
-int codes_map(CUtensorMap* map, const BlockView& v, int box_rows) {
-  const uint64_t dims[5] = {static_cast<uint64_t>(v.pitch / 2), static_cast<uint64_t>(v.outer), 1, 1, 1};
-  const uint64_t all = static_cast<uint64_t>(v.pitch) * v.outer;
-  const uint64_t strides[4] = {static_cast<uint64_t>(v.pitch), all, all, all};
-  const uint32_t box[5] = {64, static_cast<uint32_t>(box_rows), 1, 1, 1};
-  return make_tensor_map(map, v.codes, dims, strides, box);
+  __syncwarp();
+  if (splits > 1) cluster_wait();
 }
 
 template <int kN, bool kNv>
-int launch_dot(DeviceCtx* c, const BlockView& a, const BlockView& b, DotParams& p, int splits, cudaStream_t stream) {
+int launch_dot(DeviceCtx* c, DotParams& p, int splits, cudaStream_t stream) {
   using T = DotTile<kN, kNv>;
-  CUtensorMap mapA, mapB;
-  int rc = codes_map(&mapA, a, 128);
-  if (rc == NG_OK) rc = codes_map(&mapB, b, kN);
-  if (rc != NG_OK) return rc;
   // E2M1 operands, N >> 3, scales E4M3 or E8M0, M >> 4
   p.idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(kN >> 3) << 17) | ((kNv ? 0u : 1u) << 23) | ((128u >> 4) << 24);
   const long long tiles = static_cast<long long>(p.tiles_m) * ((p.N + kN - 1ll) / kN);
@@ -400,12 +408,12 @@ int launch_dot(DeviceCtx* c, const BlockView& a, const BlockView& b, DotParams& 
     NG_CUDA(cudaFuncSetAttribute(block_dot_kernel<kN, kNv>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
     ready.fetch_or(1ull << c->device, std::memory_order_relaxed);
   }
-  NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_kernel<kN, kNv>, mapA, mapB, p));
+  NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_kernel<kN, kNv>, p));
   NG_CHECK_LAUNCH();
   return NG_OK;
 }
 
-int pad_columns(int n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : (n + 127) / 128 * 128; }
+int pad_columns(int n) { return n <= 64 ? block_tile_rows(n) : (n + 127) / 128 * 128; }
 
 int check_output(const void* C, int ldc, int n, int sr_bits, int out_f32) {
   if (!C) return fail(NG_ERR_INVALID_ARG, "null operand");
@@ -454,9 +462,10 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   if (p.swapped) std::swap(a, b);
   p.M = a.outer; p.N = b.outer;
   p.tiles_m = (p.M + 127) / 128;
-  p.num_kb = static_cast<int>(a.pitch / kRowPad);
+  p.num_kb = (a.inner + 255) / 256;
+  p.ca = a.codes; p.cb = b.codes; p.pitch_a = a.pitch; p.pitch_b = b.pitch; p.tile_a = a.tile; p.tile_b = b.tile;
   p.sa = a.scales; p.sb = b.scales; p.spitch = a.spitch;
-  p.sa_tiles = (a.outer + 127) / 128; p.sb_tiles = (b.outer + 127) / 128;
+  p.b_tiles = (b.outer + 127) / 128;
   p.status = c->status; p.wait_limit_ns = c->wait_limit_ns;
   int cols = pad_columns(p.N);
   if (cols > 128) cols = static_cast<long long>(p.tiles_m) * ((p.N + 255) / 256) >= c->sm_count ? 256 : 128;
@@ -464,7 +473,7 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   int splits = 1;
   while (splits < 8 && tiles * splits * 2 <= c->sm_count && p.num_kb >= splits * 2) splits *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define NG_DOT(kn) (nv ? launch_dot<kn, true>(c, a, b, p, splits, s) : launch_dot<kn, false>(c, a, b, p, splits, s))
+#define NG_DOT(kn) (nv ? launch_dot<kn, true>(c, p, splits, s) : launch_dot<kn, false>(c, p, splits, s))
   switch (cols) {
     case 16: return NG_DOT(16);
     case 32: return NG_DOT(32);

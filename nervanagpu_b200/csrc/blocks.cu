@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(BlockView q, PlainVi
       word |= __shfl_xor_sync(0xffffffffu, word, kShare);
       word |= __shfl_xor_sync(0xffffffffu, word, 2 * kShare);
       if (live) {
-        uint8_t* dst = q.codes + o * q.pitch + static_cast<long long>(g) * (2 * F::kBytes8);
+        uint8_t* dst = q.codes + F::code_at(q, static_cast<int>(o), static_cast<long long>(g) * (2 * F::kBytes8));
         if (F::k4) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0].x, c[1].x);
         else *reinterpret_cast<uint4*>(dst) = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
         if (g % (4 * kShare) == 0)
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(BlockView q, Plain
       codes[u] = make_uint4(0u, 0u, 0u, 0u);
       byte[u] = 0u;
       if (o < q.outer && n > 0) {
-        const uint8_t* src = q.codes + o * q.pitch + static_cast<long long>(g) * (2 * F::kBytes8);
+        const uint8_t* src = q.codes + F::code_at(q, static_cast<int>(o), static_cast<long long>(g) * (2 * F::kBytes8));
         if (F::k4) {
           const uint2 c = *reinterpret_cast<const uint2*>(src);
           codes[u].x = c.x;
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(Block
     for (int i = threadIdx.x; i < kStridedRows * (S::kRow / 16); i += kStridedThreads) {
       const int row = i / (S::kRow / 16), c = i % (S::kRow / 16);
       if (o0 + row < q.outer)
-        *reinterpret_cast<uint4*>(q.codes + (o0 + row) * q.pitch + static_cast<long long>(b0) * S::kBytes + c * 16) =
+        *reinterpret_cast<uint4*>(q.codes + F::code_at(q, o0 + row, static_cast<long long>(b0) * S::kBytes + c * 16)) =
             *reinterpret_cast<const uint4*>(codes + row * S::kPitch + c * 16);
     }
     const uint32_t* words = reinterpret_cast<const uint32_t*>(scales);
@@ -460,10 +460,10 @@ __global__ void __launch_bounds__(kStridedThreads) dequantize_strided_kernel(Blo
     float scale[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint2* src = reinterpret_cast<const uint2*>(q.codes + r[j] * q.pitch + static_cast<long long>(b) * S::kBytes);
 #pragma unroll
       for (int i = 0; i < S::kBytes / 8; ++i) {
-        const uint2 c = r[j] < q.outer ? src[i] : make_uint2(0u, 0u);
+        uint2 c = make_uint2(0u, 0u);
+        if (r[j] < q.outer) c = *reinterpret_cast<const uint2*>(q.codes + F::code_at(q, r[j], static_cast<long long>(b) * S::kBytes + 8 * i));
         w[j][2 * i] = c.x;
         w[j][2 * i + 1] = c.y;
       }
@@ -636,15 +636,22 @@ int relu_mask_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_t
 
 }  // namespace
 
-// rows of codes and of scales, in bytes
-static void block_pitches(const ng_block_desc& d, long long& pitch, long long& spitch) {
-  const long long inner = d.axis ? d.cols : d.rows;
+// rows of a tile of a 4-bit format
+int block_tile_rows(int outer) { return outer <= 16 ? 16 : outer <= 32 ? 32 : outer <= 64 ? 64 : 128; }
+
+// what the sizes give, in bytes
+static void block_pitches(const ng_block_desc& d, BlockView& v) {
+  v.outer = d.axis ? d.rows : d.cols;
+  v.inner = d.axis ? d.cols : d.rows;
   if (d.format == NG_BLOCK_MXFP8) {
-    pitch = (inner + kRowPad - 1) / kRowPad * kRowPad;
-    spitch = pitch / 32;
+    v.tile = 0;
+    v.pitch = (v.inner + kRowPad - 1ll) / kRowPad * kRowPad;
+    v.spitch = v.pitch / 32;
   } else {
-    pitch = (inner + 2 * kRowPad - 1) / (2 * kRowPad) * kRowPad;
-    spitch = pitch * 2 / (d.format == NG_BLOCK_NVFP4 ? 64 : 128) * kScaleTile;
+    const long long kbs = (v.inner + 255ll) / 256;
+    v.tile = block_tile_rows(v.outer) * kRowPad;
+    v.pitch = kbs * v.tile;
+    v.spitch = kbs * (d.format == NG_BLOCK_NVFP4 ? 4 : 2) * kScaleTile;
   }
 }
 
@@ -671,11 +678,9 @@ int block_view(const DeviceCtx* c, const ng_block_desc* d, BlockView& v) {
   if ((reinterpret_cast<uintptr_t>(d->codes) | reinterpret_cast<uintptr_t>(d->scales)) & (kRowPad - 1))
     return fail(NG_ERR_INVALID_ARG, "codes and scales must be 128-byte aligned");
   if (d->device != c->device) return fail(NG_ERR_INVALID_ARG, "block matrix of device %d, the current device is %d", d->device, c->device);
-  block_pitches(*d, v.pitch, v.spitch);
+  block_pitches(*d, v);
   v.codes = static_cast<uint8_t*>(d->codes);
   v.scales = static_cast<uint8_t*>(d->scales);
-  v.outer = d->axis ? d->rows : d->cols;
-  v.inner = d->axis ? d->cols : d->rows;
   v.t = d->scale;
   return NG_OK;
 }
@@ -696,11 +701,11 @@ int ng_block_bytes(const ng_block_desc* desc, size_t* codes_bytes, size_t* scale
   const int rc = check_shape(desc);
   if (rc != NG_OK) return rc;
   if (!codes_bytes || !scales_bytes) return fail(NG_ERR_INVALID_ARG, "no place for the sizes");
-  long long pitch, spitch;
-  block_pitches(*desc, pitch, spitch);
-  const long long outer = desc->axis ? desc->rows : desc->cols;
-  *codes_bytes = static_cast<size_t>(pitch) * outer;
-  *scales_bytes = static_cast<size_t>(spitch) * (desc->format == NG_BLOCK_MXFP8 ? outer : (outer + 127) / 128);
+  BlockView v = {};
+  block_pitches(*desc, v);
+  const size_t rows = desc->format == NG_BLOCK_MXFP8 ? v.outer : (v.outer + 127ll) / 128;
+  *codes_bytes = static_cast<size_t>(v.pitch) * rows;
+  *scales_bytes = static_cast<size_t>(v.spitch) * rows;
   return NG_OK;
 }
 

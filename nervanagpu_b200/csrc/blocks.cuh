@@ -17,26 +17,31 @@
 // A block with an infinity or a NaN has the scale NaN (0xff, or 0x7f in E4M3): all of it reads back as NaN. A
 // product sums over the block, so its result is lost either way. mxfp8 codes keep the signs in such blocks too.
 //
-// Layout. The matrix is stored along its blocked axis ("inner"), one row of codes per index of the other axis
-// ("outer"), two 4-bit codes per byte (the even one in the low half). Rows are padded with zeros to 128 bytes:
-// every row can be addressed by TMA, and a product's k-block of 128 bytes needs no case for the end of the row.
-// 4-bit scales lie as the tensor cores take them: tiles of 512 bytes hold 4 consecutive blocks of 128 outer rows,
-// byte (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4, so that a tile goes to tensor memory in one copy.
-// mxfp8 scales lie row by row. Scales are padded with zeros too (2^-127 or 0: with the zero codes they give zero).
+// Layout. The matrix is stored along its blocked axis ("inner"), a row of codes per index of the other axis ("outer"),
+// two 4-bit codes per byte (the even one in the low half).
+//   mxfp8: rows of codes one behind the other, padded with zeros to 128 bytes; rows of scales likewise (4 per 128).
+//   4-bit formats: as shared and tensor memory hold them, so that a product's operands are plain contiguous copies,
+//   without a tensor map to build and fetch and without a stride between their rows. Tiles of 128 outer rows (fewer
+//   in a matrix of at most 64: 16, 32 or 64) x 128 bytes = 256 numbers, the tiles of 128 rows along the inner axis
+//   one behind the other; the 16-byte pieces of row r are exchanged as the 128-byte swizzle wants it, piece c
+//   at c ^ (r % 8). Scales: tiles of 512 bytes with 4 consecutive blocks of 128 outer rows, byte
+//   (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4.
+// Tiles are padded with zeros, which no call overwrites (a scale of 2^-127 or 0 with the code 0 gives zero).
 #pragma once
 #include "../../include/nervana_b200.h"
 #include "common.cuh"
 
 namespace ngb {
 
-constexpr int kRowPad = 128;        // bytes: rows of codes are multiples of this
+constexpr int kRowPad = 128;        // bytes: mxfp8 rows are multiples of this, tiles' rows have as many
 constexpr int kScaleTile = 512;     // bytes of a tile of 4-bit formats' scales
 
 // What a kernel needs to know of a matrix in blocks.
 struct BlockView {
   uint8_t* codes;
   uint8_t* scales;
-  long long pitch;        // bytes from one row of codes to the next
+  long long pitch;        // bytes from one row (mxfp8) or one row of tiles of codes to the next
+  int tile;               // 4-bit formats: bytes of a tile of codes
   long long spitch;       // bytes from one row (mxfp8) or one row of tiles (4-bit formats) of scales to the next
   int outer, inner;
   float t;                // nvfp4: the matrix's power of two
@@ -49,6 +54,12 @@ struct BlockFormat {
   static constexpr int kBlock = kNv ? 16 : 32;
   static constexpr int kBytes8 = k4 ? 4 : 8;      // bytes of 8 codes
 
+  // byte `at` of row o of the codes, within an aligned 16 bytes
+  static __device__ __forceinline__ long long code_at(const BlockView& v, int o, long long at) {
+    if (!k4) return o * v.pitch + at;
+    const int b = static_cast<int>(at) & 127;
+    return (o >> 7) * v.pitch + (at >> 7) * v.tile + (o & 127) * 128 + (b ^ ((o & 7) << 4));
+  }
   static __device__ __forceinline__ long long scale_at(const BlockView& v, int o, int b) {
     if (!k4) return o * v.spitch + b;
     return (o >> 7) * v.spitch + (b >> 2) * kScaleTile + (o & 31) * 16 + ((o >> 5) & 3) * 4 + (b & 3);

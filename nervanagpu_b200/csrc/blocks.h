@@ -7,6 +7,8 @@ namespace ngb {
 
 // Checks what a descriptor says, without a device.
 int check_shape(const ng_block_desc* d);
+// Rows of a tile of codes in a 4-bit matrix of so many outer rows (128 from 65 on).
+int block_tile_rows(int outer);
 // Checks a descriptor against the current device and fills in what the kernels need.
 int block_view(const DeviceCtx* c, const ng_block_desc* d, BlockView& v);
 // The values of a checked matrix as rows of `ld` fp16 numbers along its blocked axis.

@@ -166,17 +166,17 @@ def test_several_matrices_from_one_call_and_the_same_buffer_again(ng):
             assert np.array_equal(t, got.T) and q.T.T.axis == q.axis
 
 
-def test_padding_stays_zero(ng):
-    """Products read whole k-blocks and scale tiles: what lies behind a row's or the matrix's end is zero."""
-    x = np.full((130, 70), 3.0, np.float16)
+@pytest.mark.parametrize("shape", [(130, 70), (20, 300), (1, 1), (65, 256)])
+def test_padding_stays_zero(ng, shape):
+    """Products read whole tiles of codes and scales: what lies behind a row's or the matrix's end is zero."""
+    x = np.full(shape, 3.0, np.float16)
     for fmt in ("mxfp4", "nvfp4"):
-        q = filled(ng, x, fmt, 1)
-        codes = q.codes.get().reshape(130, 128)
-        assert (codes[:, :35] != 0).all() and (codes[:, 35:] == 0).all()
-        per = 512 // 4
-        scales = q.scales.get()
-        blocks = -(-70 // (16 if fmt == "nvfp4" else 32))
-        assert (scales != 0).sum() == 130 * blocks and scales.size % (4 * per) == 0
+        for axis in (0, 1):
+            q = filled(ng, x if axis else x.T, fmt, axis)
+            codes, scales = q.codes.get(), q.scales.get()
+            odd = shape[1] % 2 * shape[0]
+            assert (codes != 0).sum() == shape[0] * ((shape[1] + 1) // 2) and ((codes >> 4) != 0).sum() == (codes != 0).sum() - odd
+            assert (scales != 0).sum() == shape[0] * -(-shape[1] // (16 if fmt == "nvfp4" else 32))
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
