@@ -501,18 +501,10 @@ int ng_block_dot_f16(const void* A, int lda, const ng_block_desc* B, void* C, in
   BlockView b;
   rc = block_view(c, B, b);
   if (rc != NG_OK) return rc;
-  AuxClaim room;
-  void* plain = nullptr;
-  const long long ld = (k + 7ll) / 8 * 8;
-  rc = room.room(c, static_cast<cudaStream_t>(stream), static_cast<size_t>(ld) * n * 2, &plain);
-  if (rc != NG_OK) return rc;
-  rc = dequantize_f16(c, *B, b, static_cast<__half*>(plain), ld, static_cast<cudaStream_t>(stream));
-  if (rc != NG_OK) return rc;
-  GemmCall g = {};
-  g.A = A; g.B = plain; g.C = C; g.b_t = 1; g.m = m; g.n = n; g.k = k;
-  g.lda = lda; g.ldb = ld; g.ldc = ldc; g.alpha = alpha; g.beta = beta; g.relu = relu; g.sr_bits = sr_bits;
-  g.seed = seed; g.rng_offset = rng_offset; g.batch = 1; g.loops = 1; g.out_f32 = out_f32;
-  return run_gemm(g, static_cast<cudaStream_t>(stream));
+  EpiArgs ea;
+  ea.alpha = alpha; ea.beta = beta; ea.relu = relu; ea.sr_bits = sr_bits;
+  ea.seed_lo = static_cast<uint32_t>(seed); ea.seed_hi = static_cast<uint32_t>(seed >> 32); ea.rng_offset = rng_offset;
+  return run_block_dot_f16(c, A, lda, *B, b, C, m, ldc, out_f32, ea, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,506 @@
+// Products of a plain fp16 matrix with one in mxfp8 (blocks.cuh): the weight gradient of a fully-connected layer from
+// its deltas (m x k, k images) and the 8-bit record of its input (n x k along the images).
+//
+//   C[i,j] = epilogue(sum_k A[i,k] X[j,k]),   X[j,k] = code * 2^e, an fp16 number when it was made from one
+//
+// block_dot_f16_kernel multiplies in fp16 on tcgen05 with fp32 accumulation. The record is brought to fp16 on its way
+// into shared memory: its codes come by TMA, eight warps take 64 of each row per k-block, convert them, scale them by
+// their power of two (exact) and store them where the 128-byte swizzle wants them; no fp16 copy of the record is ever
+// in memory. A's tiles come by TMA, or, from rows that TMA cannot address, through the same warps. A CTA
+// computes tiles of 128 x kN, one after the other, with two accumulators, so that the output stage of one tile runs
+// beside the products of the next: with few images the time is that of writing C.
+//
+//   warp 0       TMA producer
+//   warp 1       tensor memory, MMAs
+//   warps 2-9    output stage: two warps per group of 32 lanes, each half of the columns
+//   warps 10-17  the record to fp16
+#include <algorithm>
+#include <atomic>
+
+#include "blocks.h"
+#include "epilogue.cuh"
+
+namespace ngb {
+
+namespace {
+
+constexpr int kMixEpi = 8, kMixConv = 8;                  // warps
+constexpr int kMixThreads = 32 * (2 + kMixEpi + kMixConv);
+constexpr uint32_t kMixA = 128u * 128u;                   // a k-block of A: 128 rows of 64 fp16 numbers
+constexpr uint32_t kMixStage = kMixEpi * 4096u;           // output staging: [32 rows][128 bytes] per warp
+constexpr int kMixRaw = 3;                                // slots of codes
+constexpr uint32_t kMixCtrl = 256;
+constexpr uint32_t kMixSmemLimit = 232448;
+
+template <int kN>
+struct MixTile {
+  static constexpr uint32_t kB = kN * 128u;
+  static constexpr uint32_t kSlot = kMixA + kB;
+  static constexpr uint32_t kRaw = kN * 64u;              // a k-block of codes
+  static constexpr int kRoom = static_cast<int>((kMixSmemLimit - 1024u - kMixCtrl - kMixStage - kMixRaw * kRaw) / kSlot);
+  static constexpr int kStages = kRoom < 6 ? kRoom : 6;
+  static constexpr uint32_t kSmem = kStages * kSlot + kMixRaw * kRaw + kMixStage + kMixCtrl + 1024u;
+  static constexpr uint32_t kCols = 2 * kN;               // of tensor memory: two accumulators
+  static constexpr int kEpiCols = kN > 64 ? kN / 2 : 64;  // columns of an output-stage warp (64: one of the two has them all)
+};
+
+struct MixParams {
+  const __half* A;
+  long long lda;
+  int a_tma;
+  int M, N, K;
+  int tiles_n, tiles, num_kb;
+  BlockView x;
+  void* C;
+  long long ldc;
+  int out_f32, store;        // store: 1 = TMA, 0 = one number per lane and access
+  EpiArgs ea;
+  int* status;
+  unsigned long long wait_limit_ns;
+};
+
+// kLean: fp16 outputs rounded to nearest with nothing added; the other instance does all.
+template <int kN, bool kLean>
+__global__ void __launch_bounds__(kMixThreads, 1)
+block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapX,
+                     const __grid_constant__ CUtensorMap mapC, const __grid_constant__ MixParams p) {
+  using T = MixTile<kN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* ring_gen = smem_raw + (ring - smem_u32(smem_raw));
+  const uint32_t raw = ring + T::kStages * T::kSlot, staging = raw + kMixRaw * T::kRaw;
+  const uint32_t ctrl = staging + kMixStage;
+  auto full_bar = [&](int s) { return ctrl + 8u * s; };
+  auto empty_bar = [&](int s) { return ctrl + 8u * (6 + s); };
+  auto accf_bar = [&](int a) { return ctrl + 8u * (12 + a); };
+  auto acce_bar = [&](int a) { return ctrl + 8u * (14 + a); };
+  auto rawf_bar = [&](int s) { return ctrl + 8u * (16 + s); };
+  auto rawe_bar = [&](int s) { return ctrl + 8u * (19 + s); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_gen + (ctrl - ring) + 8 * 22);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < T::kStages; ++s) {
+      mbar_init(full_bar(s), kMixConv + (p.a_tma ? 1 : 0));
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(accf_bar(a), 1);
+      mbar_init(acce_bar(a), kMixEpi);
+    }
+    for (int s = 0; s < kMixRaw; ++s) {
+      mbar_init(rawf_bar(s), 1);
+      mbar_init(rawe_bar(s), kMixConv);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    if (p.a_tma) tma_prefetch_desc(&mapA);
+    tma_prefetch_desc(&mapX);
+    if (p.store) tma_prefetch_desc(&mapC);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), T::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+
+  // (slots are counted over all tiles of this CTA: `it` = k-blocks so far)
+  if (warp == 0) {
+    if (elect_one()) {
+      int it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+        const int m0 = t / p.tiles_n * 128, n0 = t % p.tiles_n * kN;
+        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+          const int s = it % T::kStages, x = it % kMixRaw;
+          if (it >= kMixRaw && !mbar_wait(rawe_bar(x), (it / kMixRaw - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(rawf_bar(x), T::kRaw);
+          tma_load_5d(raw + x * T::kRaw, &mapX, rawf_bar(x), kb * 32, n0, 0, 0, 0);
+          if (!p.a_tma) continue;
+          if (it >= T::kStages && !mbar_wait(empty_bar(s), (it / T::kStages - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(full_bar(s), kMixA);
+          tma_load_5d(ring + s * T::kSlot, &mapA, full_bar(s), kb * 64, m0, 0, 0, 0);
+        }
+      }
+      if (!ok) {
+        // Given up: the loads in flight must land before the CTA may end. Their barriers may never complete, the
+        // other arrivals missing, so this waits for time instead, which no copy inside the device takes.
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29), lo = 1u << 16;
+      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(kN >> 3) << 17) | ((128u >> 4) << 24);
+      int it = 0, local = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x, ++local) {
+        const int acc = local & 1;
+        if (local >= 2 && !mbar_wait(acce_bar(acc), (local / 2 - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_ACC, p.wait_limit_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+          const int s = it % T::kStages;
+          if (!mbar_wait(full_bar(s), (it / T::kStages) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_MMA, p.wait_limit_ns)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = ring + s * T::kSlot;
+          tc_mma_f16_run<false, 4>(tmem + acc * kN, lo | (a >> 4), hi, lo | ((a + kMixA) >> 4), hi, idesc, kb != 0, 2u, 2u);
+          tc_commit(empty_bar(s));
+        }
+        if (ok) tc_commit(accf_bar(acc));
+      }
+      if (!ok) {   // what was issued must end before tensor memory is given back (a fresh use of a barrier is not at hand)
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 2 + kMixEpi) {
+    const int group = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t stage = staging + (warp - 2) * 4096u;
+    uint8_t* stage_gen = ring_gen + (stage - ring);
+    const bool f32 = !kLean && p.out_f32;
+    const int esz = f32 ? 4 : 2;
+    const int box = 128 / esz;                       // columns of a staged box
+    int local = 0;
+    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++local) {
+      const int acc = local & 1;
+      const bool ok = mbar_wait(accf_bar(acc), (local / 2) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
+      if (__any_sync(0xffffffffu, !ok)) break;
+      tc_fence_after();
+      const int m0 = t / p.tiles_n * 128 + group * 32, n0 = t % p.tiles_n * kN + half * T::kEpiCols;
+      const long long row = m0 + lane;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(group * 32) << 16) + acc * kN + half * T::kEpiCols;
+      if (half * T::kEpiCols >= kN) {
+        if (lane == 0) mbar_arrive(acce_bar(acc));
+        continue;
+      }
+      if constexpr (kLean) {
+        const bool as_is = p.ea.alpha == 1.0f && !p.ea.relu;
+#pragma unroll 1
+        for (int c = 0; c < T::kEpiCols; c += 64) {
+          uint32_t r[2][32];
+          tc_ld_32x32(taddr + c, r[0]);
+          tc_ld_32x32(taddr + c + 32, r[1]);
+          tc_wait_ld();
+          if (c + 64 >= T::kEpiCols) {     // the accumulator has been read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acce_bar(acc));
+          }
+          if (m0 >= p.M || n0 + c >= p.N) continue;
+          uint4 w[8];
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            __half2* h = reinterpret_cast<__half2*>(&w[g]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float a = __uint_as_float(r[g / 4][g % 4 * 8 + 2 * i]), b = __uint_as_float(r[g / 4][g % 4 * 8 + 2 * i + 1]);
+              if (!as_is) {
+                a = epi_scale(p.ea, a);
+                b = epi_scale(p.ea, b);
+              }
+              h[i] = __floats2half2_rn(a, b);
+            }
+          }
+          if (lane == 0) tma_store_wait_read<0>();       // (the box before must have left)
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < 8; ++g) *reinterpret_cast<uint4*>(stage_gen + lane * 128 + ((g ^ (lane & 7)) << 4)) = w[g];
+          if (p.store) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_5d(&mapC, stage, n0 + c, m0, 0, 0, 0);
+              tma_store_commit();
+            }
+          } else {
+            // rows at any address: a row at a time, two numbers per lane
+            __syncwarp();
+            __half* out = static_cast<__half*>(p.C) + m0 * p.ldc + n0 + c + lane;
+            const int rows = min(32, p.M - m0), cols = p.N - n0 - c - lane;
+#pragma unroll 8
+            for (int i = 0; i < rows; ++i, out += p.ldc) {
+              const uint8_t* src = stage_gen + i * 128 + ((lane * 2) & 15);
+              if (cols > 0) out[0] = *reinterpret_cast<const __half*>(src + (((lane >> 3) ^ (i & 7)) << 4));
+              if (cols > 32) out[32] = *reinterpret_cast<const __half*>(src + (((4 + (lane >> 3)) ^ (i & 7)) << 4));
+            }
+            __syncwarp();
+          }
+        }
+        continue;
+      }
+#pragma unroll 1
+      for (int c = 0; c < T::kEpiCols; c += 32) {
+        uint32_t r[32];
+        tc_ld_32x32(taddr + c, r);
+        tc_wait_ld();
+        if (c + 32 >= T::kEpiCols) {     // the accumulator has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acce_bar(acc));
+        }
+        if (m0 >= p.M || n0 + c >= p.N) continue;
+        // into this lane's row of the staged box: 32 columns are 64 bytes of fp16 (half a row) or 128 of fp32
+        const int at = f32 ? 0 : (c & 32) * 2;
+        if (at == 0) {                   // (the box before must have left)
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+        }
+        uint8_t* dst = stage_gen + lane * 128;
+        const uint32_t sw = (lane & 7) << 4;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[8 * g + i]);
+          uint4 lo, hi;
+          {
+            const int col = n0 + c + 8 * g;
+            const int nvalid = row < p.M ? max(0, min(8, p.N - col)) : 0;
+            const unsigned long long lin = static_cast<unsigned long long>(row) * p.N + col;
+            const void* oldp = nvalid > 0 ? static_cast<const uint8_t*>(p.C) + (row * p.ldc + col) * esz : nullptr;
+            if (f32) epi_pack8<true>(p.ea, v, oldp, lin, lo, hi, max(nvalid, 1));
+            else epi_pack8<false>(p.ea, v, oldp, lin, lo, hi, max(nvalid, 1));
+          }
+          if (f32) {
+            *reinterpret_cast<uint4*>(dst + ((32 * g) ^ sw)) = lo;
+            *reinterpret_cast<uint4*>(dst + ((32 * g + 16) ^ sw)) = hi;
+          } else {
+            *reinterpret_cast<uint4*>(dst + ((at + 16 * g) ^ sw)) = lo;
+          }
+        }
+        if (!f32 && at == 0 && n0 + c + 32 < p.N) continue;    // the other half of the box comes next
+        const int col0 = n0 + (f32 ? c : c & ~63);
+        if (p.store) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_5d(&mapC, stage, col0, m0, 0, 0, 0);
+            tma_store_commit();
+          }
+        } else {
+          __syncwarp();
+          const int rows = min(32, p.M - m0), cols = min(box, p.N - col0);
+          for (int i = 0; i < rows; ++i) {
+            uint8_t* out = static_cast<uint8_t*>(p.C) + ((m0 + i) * p.ldc + col0) * esz;
+            for (int j = lane; j < cols; j += 32) {
+              const uint8_t* src = stage_gen + i * 128 + (((j * esz) & 112) ^ ((i & 7) << 4)) + ((j * esz) & 15);
+              if (f32) reinterpret_cast<float*>(out)[j] = *reinterpret_cast<const float*>(src);
+              else reinterpret_cast<__half*>(out)[j] = *reinterpret_cast<const __half*>(src);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait_all();
+    __syncwarp();
+  } else {
+    // ---- the record to fp16: a thread has a row of the tile per k-block, or (128 or 64 columns) half or a quarter of one
+    constexpr int kPer = 32 * kMixConv / kN;            // threads that share a row
+    constexpr int kPieces = 4 / kPer;                   // 16 codes of a k-block each
+    const int tid = threadIdx.x - 32 * (2 + kMixEpi);
+    const int r = tid / kPer, part = tid % kPer;
+    int it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+      const int m0 = t / p.tiles_n * 128, j = t % p.tiles_n * kN + r;
+      // the scales of 128 codes are a word
+      const uint8_t* scales = p.x.scales + static_cast<long long>(j) * p.x.spitch;
+      uint32_t word = j < p.N ? *reinterpret_cast<const uint32_t*>(scales) : 0u;
+      for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+        const int s = it % T::kStages, x = it % kMixRaw;
+        ok = mbar_wait(rawf_bar(x), (it / kMixRaw) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns) &&
+             (it < T::kStages || mbar_wait(empty_bar(s), (it / T::kStages - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns));
+        if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+        const uint8_t* src = ring_gen + (raw - ring) + x * T::kRaw + r * 64;
+        uint8_t* b = ring_gen + s * T::kSlot + kMixA + r * 128;
+        uint4 w[kPieces];
+        float scale[(kPieces + 1) / 2];
+        bool fits = true;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int piece = part * kPieces + i;                // swizzled by 64 bytes as TMA left them
+          w[i] = *reinterpret_cast<const uint4*>(src + ((piece ^ (r >> 1 & 3)) << 4));
+          if (i % 2 == 0) {
+            scale[i / 2] = block_scale_value<NG_BLOCK_MXFP8>(word >> ((kb & 1) * 16 + (piece >> 1) * 8) & 0xffu, 1.0f);
+            fits = fits && block_scale_fits_f16<NG_BLOCK_MXFP8>(scale[i / 2]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int piece = part * kPieces + i;
+          uint4 v[2];
+          if (fits) {
+            const __half2 by = __float2half2_rn(scale[i / 2]);
+            v[0] = block_decode8_f16<NG_BLOCK_MXFP8>(make_uint2(w[i].x, w[i].y), by);
+            v[1] = block_decode8_f16<NG_BLOCK_MXFP8>(make_uint2(w[i].z, w[i].w), by);
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float f[8];
+              block_decode8<NG_BLOCK_MXFP8>(h ? make_uint2(w[i].z, w[i].w) : make_uint2(w[i].x, w[i].y), scale[i / 2], f);
+              block_limit_f16<NG_BLOCK_MXFP8>(scale[i / 2], f);
+              __half2* o = reinterpret_cast<__half2*>(&v[h]);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) o[y] = __floats2half2_rn(f[2 * y], f[2 * y + 1]);
+            }
+          }
+          *reinterpret_cast<uint4*>(b + (((2 * piece) ^ (r & 7)) << 4)) = v[0];
+          *reinterpret_cast<uint4*>(b + (((2 * piece + 1) ^ (r & 7)) << 4)) = v[1];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(rawe_bar(x));
+        if ((kb & 1) && kb + 1 < p.num_kb && j < p.N) word = *reinterpret_cast<const uint32_t*>(scales + (kb + 1) * 2ll);
+        if (!p.a_tma) {
+          // 16 rows of A per warp, two numbers per lane and row
+          const int cw = warp - 2 - kMixEpi, k0 = kb * 64 + lane;
+          uint8_t* a = ring_gen + s * T::kSlot;
+#pragma unroll
+          for (int i = 0; i < 128 / kMixConv; ++i) {
+            const int ar = cw * (128 / kMixConv) + i;
+            const __half* src = p.A + static_cast<long long>(m0 + ar) * p.lda + k0;
+            const bool row_ok = m0 + ar < p.M;
+            const __half lo = row_ok && k0 < p.K ? src[0] : __half(0.0f), hi = row_ok && k0 + 32 < p.K ? src[32] : __half(0.0f);
+            const int at = lane * 2, sw = (ar & 7) << 4;
+            *reinterpret_cast<__half*>(a + ar * 128 + ((at & 112) ^ sw) + (at & 15)) = lo;
+            *reinterpret_cast<__half*>(a + ar * 128 + (((at + 64) & 112) ^ sw) + (at & 15)) = hi;
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full_bar(s));
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, T::kCols);
+  }
+}
+
+// rank-2 boxes of a row-major matrix
+int plain_map(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_cols, int box_rows, int esz) {
+  const uint64_t dims[5] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows), 1, 1, 1};
+  const uint64_t row = static_cast<uint64_t>(ld) * esz, all = row * rows;
+  const uint64_t strides[4] = {row, all, all, all};
+  const uint32_t box[5] = {static_cast<uint32_t>(box_cols), static_cast<uint32_t>(box_rows), 1, 1, 1};
+  return make_tensor_map(map, base, dims, strides, box, esz);
+}
+
+template <int kN, bool kLean>
+int launch_mix(DeviceCtx* c, MixParams& p, cudaStream_t stream) {
+  using T = MixTile<kN>;
+  p.tiles_n = (p.N + kN - 1) / kN;
+  const long long tiles = static_cast<long long>(p.tiles_n) * ((p.M + 127ll) / 128);
+  if (tiles > 0x3fffffffll) return fail(NG_ERR_TOO_LARGE, "too many tiles");
+  p.tiles = static_cast<int>(tiles);
+  CUtensorMap mapA = {}, mapX, mapC = {};
+  int rc = NG_OK;
+  if (p.a_tma) rc = plain_map(&mapA, p.A, p.M, p.K, p.lda, 64, 128, 2);
+  // (codes as 16-bit units; zeros beyond the last row)
+  if (rc == NG_OK) rc = plain_map(&mapX, p.x.codes, p.N, p.x.pitch / 2, p.x.pitch / 2, 32, kN, 2);
+  if (rc == NG_OK && p.store) rc = plain_map(&mapC, p.C, p.M, p.N, p.ldc, p.out_f32 ? 32 : 64, 32, p.out_f32 ? 4 : 2);
+  if (rc != NG_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, c->sm_count)));
+  cfg.blockDim = dim3(kMixThreads);
+  cfg.dynamicSmemBytes = T::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = tuning().dependent_launch != 0 ? 1 : 0;
+  static std::atomic<unsigned long long> ready{0};
+  if (!(ready.load(std::memory_order_relaxed) >> c->device & 1u)) {
+    NG_CUDA(cudaFuncSetAttribute(block_dot_f16_kernel<kN, kLean>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
+    ready.fetch_or(1ull << c->device, std::memory_order_relaxed);
+  }
+  NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_f16_kernel<kN, kLean>, mapA, mapX, mapC, p));
+  NG_CHECK_LAUNCH();
+  return NG_OK;
+}
+
+}  // namespace
+
+// Long sums: the record as fp16 rows in scratch memory, then the product of two fp16 matrices. False when there is no
+// room for them.
+static bool from_scratch(DeviceCtx* c, const void* A, int lda, const ng_block_desc& d, const BlockView& x, void* C, int m, int ldc,
+                         int out_f32, const EpiArgs& ea, cudaStream_t stream, int& rc) {
+  AuxClaim room;
+  void* plain = nullptr;
+  const long long ld = (x.inner + 7ll) / 8 * 8;
+  if (room.room(c, stream, static_cast<size_t>(ld) * x.outer * 2, &plain) != NG_OK) {
+    cudaGetLastError();
+    return false;
+  }
+  rc = dequantize_f16(c, d, x, static_cast<__half*>(plain), ld, stream);
+  if (rc != NG_OK) return true;
+  GemmCall g = {};
+  g.A = A; g.B = plain; g.C = C; g.b_t = 1; g.m = m; g.n = x.outer; g.k = x.inner;
+  g.lda = lda; g.ldb = ld; g.ldc = ldc; g.alpha = ea.alpha; g.beta = ea.beta; g.relu = ea.relu; g.sr_bits = ea.sr_bits;
+  g.seed = static_cast<unsigned long long>(ea.seed_hi) << 32 | ea.seed_lo; g.rng_offset = ea.rng_offset;
+  g.batch = 1; g.loops = 1; g.out_f32 = out_f32;
+  rc = run_gemm(g, stream);
+  return true;
+}
+
+int run_block_dot_f16(DeviceCtx* c, const void* A, int lda, const ng_block_desc& d, const BlockView& x, void* C, int m, int ldc,
+                      int out_f32, const EpiArgs& ea, cudaStream_t stream) {
+  MixParams p = {};
+  p.A = static_cast<const __half*>(A); p.lda = lda;
+  p.a_tma = (reinterpret_cast<uintptr_t>(A) & 15u) == 0 && lda % 8 == 0;
+  p.M = m; p.N = x.outer; p.K = x.inner;
+  p.num_kb = (x.inner + 63) / 64;
+  p.x = x;
+  p.C = C; p.ldc = ldc; p.out_f32 = out_f32;
+  p.store = (reinterpret_cast<uintptr_t>(C) & 15u) == 0 && ldc % (out_f32 ? 4 : 8) == 0;
+  p.ea = ea;
+  p.status = c->status; p.wait_limit_ns = c->wait_limit_ns;
+  const bool lean = !out_f32 && ea.beta == 0.0f && ea.sr_bits == 0;
+  // Columns of a tile: what takes the SMs least time, a tile of n columns counted as n + 64 (its rows of A, its start
+  // and its end). 1001 x 4097 x 125: one round of 136 tiles of 256 columns, or four of 520 tiles of 64.
+  const long long row_tiles = (m + 127ll) / 128;
+  int cols = 256;
+  long long best = 0;
+  for (int n = 256; n >= 64; n /= 2) {
+    const long long tiles = row_tiles * ((p.N + n - 1ll) / n), cost = (tiles + c->sm_count - 1) / c->sm_count * (n + 64);
+    if (best == 0 || cost < best) {
+      best = cost;
+      cols = n;
+    }
+  }
+  // Converting on the way costs a k-block of a 256-column tile 0.66 us where its products take 0.27, so longer sums are
+  // better off with an fp16 copy, which costs a launch and its traffic but leaves the product alone: here / from
+  // scratch, us: 1024 x 1024 x 1024 9.4 / 14.6, 4096 x 4096 x 256 18.2 / 17.1, x 512 28.9 / 24.6, x 1024 50.7 / 35.5,
+  // 512 x 512 x 8192 55 / 17, 1000 x 4096 x 2000 27.0 / 24.0. Two k-blocks are always within the time of writing C.
+  const long long rounds = best / (cols + 64);
+  int rc;
+  if (p.num_kb > 2 && rounds * p.num_kb > 16 && from_scratch(c, A, lda, d, x, C, m, ldc, out_f32, ea, stream, rc)) return rc;
+#define NG_MIX(kn) (lean ? launch_mix<kn, true>(c, p, stream) : launch_mix<kn, false>(c, p, stream))
+  return cols == 256 ? NG_MIX(256) : cols == 128 ? NG_MIX(128) : NG_MIX(64);
+#undef NG_MIX
+}
+
+}  // namespace ngb

@@ -215,7 +215,8 @@ __device__ __forceinline__ void block_decode8(uint2 codes, float scale, float (&
 // same results as in fp32.
 template <int kFmt>
 __device__ __forceinline__ bool block_scale_fits_f16(float scale) {
-  return scale >= 6.103515625e-05f && scale * (BlockFormat<kFmt>::k4 ? 6.0f : 448.0f) <= 65504.0f;
+  // (below 2^-40 fp16 holds neither the scale nor any of the values: both are zero)
+  return (scale >= 6.103515625e-05f || scale <= 9.094947e-13f) && scale * (BlockFormat<kFmt>::k4 ? 6.0f : 448.0f) <= 65504.0f;
 }
 template <int kFmt>
 __device__ __forceinline__ uint4 block_decode8_f16(uint2 codes, __half2 scale) {

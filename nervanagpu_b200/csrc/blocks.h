@@ -1,6 +1,7 @@
 // Host-side view of matrices in blocks, shared by the element-wise kernels and the products on them.
 #pragma once
 #include "blocks.cuh"
+#include "epilogue.cuh"
 #include "host.h"
 
 namespace ngb {
@@ -13,5 +14,9 @@ int block_tile_rows(int outer);
 int block_view(const DeviceCtx* c, const ng_block_desc* d, BlockView& v);
 // The values of a checked matrix as rows of `ld` fp16 numbers along its blocked axis.
 int dequantize_f16(DeviceCtx* c, const ng_block_desc& d, const BlockView& q, __half* out, long long ld, cudaStream_t stream);
+
+// The product of block_dot_f16.cu, from checked operands.
+int run_block_dot_f16(DeviceCtx* c, const void* A, int lda, const ng_block_desc& d, const BlockView& x, void* C, int m, int ldc,
+                      int out_f32, const EpiArgs& ea, cudaStream_t stream);
 
 }  // namespace ngb

@@ -214,7 +214,7 @@ def operands(rng, fmt, m, n, k):
 
 
 SIZES = [(1, 1, 1), (1, 1, 16), (3, 5, 33), (16, 1, 256), (128, 128, 256), (130, 17, 300), (257, 33, 1000), (1001, 125, 4097),
-         (64, 300, 513), (200, 129, 64), (384, 65, 2048), (5, 1000, 640), (1, 4096, 512), (4096, 1, 4096), (640, 520, 768)]
+         (64, 300, 513), (200, 129, 64), (384, 65, 2048), (5, 1000, 640), (1, 4096, 512), (4096, 1, 4096), (640, 520, 768), (2500, 2304, 512)]
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
@@ -285,7 +285,8 @@ def test_product_output_stage(ng, m, n, k, mixed):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (2, 3, 31), (128, 64, 32), (33, 17, 125), (130, 257, 300), (1001, 515, 125),
-                                   (64, 256, 2048), (300, 200, 64), (16, 1000, 128), (257, 9, 4100)])
+                                   (64, 256, 2048), (300, 200, 64), (16, 1000, 128), (257, 9, 4100),
+                                   (2048, 1301, 70), (2496, 2304, 96), (2400, 2311, 33), (19000, 65, 40)])
 @pytest.mark.parametrize("shift", [0, 1])
 def test_block_dot_f16(ng, m, n, k, shift):
     """The weight gradient: plain fp16 deltas (also at odd addresses and in rows of a wider matrix) with an 8-bit record."""
