@@ -14,7 +14,7 @@ EXT = os.path.join(HERE, "_native.so")     # CPython module: the native half of 
 EXT_SOURCE = os.path.join(CSRC, "pyext.cpp")
 
 SOURCES = ["runtime.cu", "tc_host.cu", "gemm.cu", "conv.cu", "pool.cu", "ew_rt.cu", "legacy_api.cu", "comm.cu",
-           "blocks.cu", "block_dot.cu", "block_dot_f16.cu"]
+           "blocks.cu", "block_dot.cu", "block_dot_pair.cu", "block_dot_f16.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

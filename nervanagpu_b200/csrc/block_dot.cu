@@ -6,7 +6,7 @@
 // of 256 numbers (four MMAs of 64) of 128 rows is one bulk copy of 16 KB, its scales one of 1 or 2 KB, and a tcgen05.cp
 // per 512 bytes takes these to tensor memory.
 //
-// A CTA computes a tile of 128 rows x kN columns (kN from 16 to 256). Few tiles are split along the sum over the
+// A CTA computes a tile of 128 rows x kN columns (kN from 16 to 128). Few tiles are split along the sum over the
 // CTAs of a thread-block cluster. Each of them then gets a share of the tile's rows from all the others by bulk copies
 // between their shared memories and adds them up in the order of the partitions: one launch, no scratch memory, the
 // same bits every time. (Fetched by loads from the others' shared memory instead, the partial tiles of 4096 x 128 x
@@ -19,8 +19,8 @@
 #include <algorithm>
 #include <atomic>
 
+#include "block_mma.cuh"
 #include "blocks.h"
-#include "epilogue.cuh"
 
 namespace ngb {
 
@@ -36,22 +36,21 @@ constexpr int kDotStages = 8;                   // most
 template <int kN, bool kNv>
 struct DotTile {
   static constexpr int kScaleTiles = kNv ? 4 : 2;            // 512-byte scale tiles per k-block and 128 rows
-  static constexpr int kRowTiles = (kN + 127) / 128;         // of B's scales
   static constexpr uint32_t kCodesB = kN * 128u;
-  static constexpr uint32_t kScalesA = kScaleTiles * kScaleTile;
-  static constexpr uint32_t kStageBytes = (kCodesA + kCodesB + kScalesA * (1 + kRowTiles) + 1023u) & ~1023u;
+  static constexpr uint32_t kScales = kScaleTiles * kScaleTile;      // of 128 rows
+  static constexpr uint32_t kStageBytes = (kCodesA + kCodesB + 2 * kScales + 1023u) & ~1023u;
   static constexpr int kStages =
       static_cast<int>((kDotSmemLimit - 1024u - kDotCtrl) / kStageBytes) < kDotStages ? static_cast<int>((kDotSmemLimit - 1024u - kDotCtrl) / kStageBytes) : kDotStages;
   // tensor memory: the accumulator, then two buffers of scales, A's before B's
   static constexpr int kAccCols = kN < 32 ? 32 : kN;
-  static constexpr int kScaleCols = kScaleTiles * 4 * (1 + kRowTiles);
+  static constexpr int kScaleCols = kScaleTiles * 8;
   static constexpr int kColsUsed = kAccCols + 2 * kScaleCols;
-  static constexpr uint32_t kCols = kColsUsed <= 128 ? 128 : (kColsUsed <= 256 ? 256 : 512);
+  static constexpr uint32_t kCols = kColsUsed <= 128 ? 128 : 256;
   // partial tiles in shared memory: rows of kN + 4 floats, so that lanes in successive rows meet different banks
   static constexpr int kPitch = kN + 4;
   static constexpr uint32_t kSmem = kStages * kStageBytes + 1024u + kDotCtrl;
   // (the partial tile takes the ring's place, and behind it, when it is split, this CTA's share of the sum)
-  static_assert(128u * kPitch * 4u * (kN > 128 ? 1 : 2) <= kStages * kStageBytes, "the ring is smaller than the tile");
+  static_assert(2 * 128u * kPitch * 4u <= kStages * kStageBytes, "the ring is smaller than the tile");
 };
 
 struct DotParams {
@@ -61,10 +60,8 @@ struct DotParams {
   const uint8_t *ca, *cb;    // codes
   const uint8_t *sa, *sb;    // scales
   long long pitch_a, pitch_b;    // bytes of a row of tiles of codes
-  int tile_a, tile_b;        // bytes of a tile of codes
+  int tile_a;                // bytes of a tile of A's codes
   long long spitch;          // bytes of a row of scale tiles (the same for both: one format, one length)
-  int b_tiles;               // rows of tiles of B that exist
-  uint32_t idesc;
   void* C;
   long long ldc;
   int out_f32, vec_ok;
@@ -74,33 +71,6 @@ struct DotParams {
   unsigned long long wait_limit_ns;
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-// 32 rows of 16 bytes in shared memory to 4 columns of tensor memory, the same in each of the four groups of 32 lanes
-__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint32_t smem) {
-  const uint64_t desc = (static_cast<uint64_t>((128u >> 4) | (1u << 14)) << 32) | (1u << 16) | (smem >> 4);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-template <bool kNv>
-__device__ __forceinline__ void tc_mma_blocks(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
-                                              uint32_t accumulate) {
-  if (kNv) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
-  } else {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
-  }
-}
 __device__ __forceinline__ void tc_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -169,19 +139,17 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
 
   // k-block i of this partition into slot i % kStages
   const int rt = m0 / 128, ct = n0 / 128;
-  const int ct_live = min(T::kRowTiles, p.b_tiles - ct);    // (the last column tile may reach beyond B's rows)
   auto load_kb = [&](int i) {
     const int s = i % T::kStages;
-    const uint32_t a = ring + s * T::kStageBytes, b = a + kCodesA, sa = b + T::kCodesB, sb = sa + T::kScalesA;
+    const uint32_t a = ring + s * T::kStageBytes, b = a + kCodesA, sa = b + T::kCodesB, sb = sa + T::kScales;
     const long long kb = kb0 + i;
-    constexpr uint32_t kB = (kN < 128 ? kN : 128) * 128u;      // (a tile of B: with up to 64 columns, B has as many rows as they are padded to)
-    mbar_expect_tx(full_bar(s), p.tile_a + T::kScalesA + ct_live * (kB + T::kScalesA));
+    // (A may have tiles of fewer rows: what the MMA then reads behind them ends in rows that are not stored. B's have
+    // as many as the tile has columns.)
+    mbar_expect_tx(full_bar(s), p.tile_a + T::kCodesB + 2 * T::kScales);
     bulk_load(a, p.ca + rt * p.pitch_a + kb * p.tile_a, p.tile_a, full_bar(s));
-    bulk_load(sa, p.sa + rt * p.spitch + kb * T::kScalesA, T::kScalesA, full_bar(s));
-    for (int c = 0; c < ct_live; ++c) {
-      bulk_load(b + c * kB, p.cb + (ct + c) * p.pitch_b + kb * p.tile_b, kB, full_bar(s));
-      bulk_load(sb + c * T::kScalesA, p.sb + (ct + c) * p.spitch + kb * T::kScalesA, T::kScalesA, full_bar(s));
-    }
+    bulk_load(sa, p.sa + rt * p.spitch + kb * T::kScales, T::kScales, full_bar(s));
+    bulk_load(b, p.cb + ct * p.pitch_b + kb * T::kCodesB, T::kCodesB, full_bar(s));
+    bulk_load(sb, p.sb + ct * p.spitch + kb * T::kScales, T::kScales, full_bar(s));
   };
   const int first = min(count, T::kStages);      // k-blocks that need no free slot
   if (warp == 0) {
@@ -226,7 +194,6 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
     __syncwarp();
   } else if (warp == 1) {
     if (elect_one()) {
-      const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);     // 8 rows of 128 bytes apart, version 1, 128-byte swizzle
       const uint32_t scales = tmem + T::kAccCols;
       bool ok = true;
       for (int i = 0; i < count; ++i) {
@@ -236,24 +203,8 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
           break;
         }
         tc_fence_after();
-        const uint32_t a = ring + s * T::kStageBytes, b = a + kCodesA, sa = b + T::kCodesB, sb = sa + T::kScalesA;
-        const uint32_t ta = scales + (i & 1) * T::kScaleCols, tb = ta + T::kScaleTiles * 4;
-#pragma unroll
-        for (int t = 0; t < T::kScaleTiles; ++t) {
-          tc_copy_scales(ta + t * 4, sa + t * kScaleTile);
-#pragma unroll
-          for (int c = 0; c < T::kRowTiles; ++c)
-            tc_copy_scales(tb + (t * T::kRowTiles + c) * 4, sb + c * T::kScalesA + t * kScaleTile);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint64_t da = (static_cast<uint64_t>(hi) << 32) | (1u << 16) | ((a + 32u * j) >> 4);
-          const uint64_t db = (static_cast<uint64_t>(hi) << 32) | (1u << 16) | ((b + 32u * j) >> 4);
-          const int t = kNv ? j : j / 2;
-          const uint32_t id = kNv ? 0u : (j & 1) * 2u;       // which of the tile's four scales are this MMA's first
-          tc_mma_blocks<kNv>(tmem, da, db, p.idesc | (id << 4) | (id << 29), ta + t * 4, tb + t * T::kRowTiles * 4,
-                             (i | j) != 0);
-        }
+        const uint32_t a = ring + s * T::kStageBytes, b = a + kCodesA, sa = b + T::kCodesB, sb = sa + T::kScales;
+        mma_kblock<kNv, false, 1>(tmem, a, b, sa, sb, scales + (i & 1) * T::kScaleCols, block_idesc(128, kN, kNv), i == 0);
         tc_commit(empty_bar(s));
       }
       tc_commit(acc_bar);
@@ -385,8 +336,6 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
 template <int kN, bool kNv>
 int launch_dot(DeviceCtx* c, DotParams& p, int splits, cudaStream_t stream) {
   using T = DotTile<kN, kNv>;
-  // E2M1 operands, N >> 3, scales E4M3 or E8M0, M >> 4
-  p.idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(kN >> 3) << 17) | ((kNv ? 0u : 1u) << 23) | ((128u >> 4) << 24);
   const long long tiles = static_cast<long long>(p.tiles_m) * ((p.N + kN - 1ll) / kN);
   if (tiles * splits > 0x7fffffffll) return fail(NG_ERR_TOO_LARGE, "too many tiles");
   cudaLaunchConfig_t cfg = {};
@@ -463,23 +412,30 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   p.M = a.outer; p.N = b.outer;
   p.tiles_m = (p.M + 127) / 128;
   p.num_kb = (a.inner + 255) / 256;
-  p.ca = a.codes; p.cb = b.codes; p.pitch_a = a.pitch; p.pitch_b = b.pitch; p.tile_a = a.tile; p.tile_b = b.tile;
+  p.ca = a.codes; p.cb = b.codes; p.pitch_a = a.pitch; p.pitch_b = b.pitch; p.tile_a = a.tile;
   p.sa = a.scales; p.sb = b.scales; p.spitch = a.spitch;
-  p.b_tiles = (b.outer + 127) / 128;
   p.status = c->status; p.wait_limit_ns = c->wait_limit_ns;
-  int cols = pad_columns(p.N);
-  if (cols > 128) cols = static_cast<long long>(p.tiles_m) * ((p.N + 255) / 256) >= c->sm_count ? 256 : 128;
+  const int cols = p.N > 64 ? 128 : pad_columns(p.N);
   const long long tiles = static_cast<long long>(p.tiles_m) * ((p.N + cols - 1) / cols);
   int splits = 1;
   while (splits < 8 && tiles * splits * 2 <= c->sm_count && p.num_kb >= splits * 2) splits *= 2;
+  // Or pairs of SMs on tiles of 256 x 256 (block_dot_pair.cu), by the sum of what both take in us: a start, and per round
+  // of tiles its k-blocks and its output stage. Here / pairs, nvfp4: 8192^3 235 / 162, 4096^3 49 / 34, 2048^3 13.9 / 9.8,
+  // 8192 x 512 x 8192 25.0 / 18.4, 1000^3 6.9 / 7.0, 1536 x 1536 x 4096 9.2 / 11.9, 4096 x 128 x 9216 10.4 / 16.4.
+  const long long pair_tiles = ((m + 255ll) / 256) * ((n + 255ll) / 256);
+  const double here = 4.5 + (tiles + c->sm_count - 1) / c->sm_count * (0.25 * p.num_kb / splits + 1.5) + (splits > 1 ? 2.0 : 0.0);
+  const double pairs = 5.5 + (pair_tiles + c->sm_count / 2 - 1) / (c->sm_count / 2) * (0.33 * p.num_kb + 0.7);
+  if (m > 64 && n > 64 && pairs < here) {
+    if (p.swapped) std::swap(a, b);
+    return run_block_dot_pair(c, a, b, nv, make_out(C, m, n, ldc, out_f32, p.ea), static_cast<cudaStream_t>(stream));
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define NG_DOT(kn) (nv ? launch_dot<kn, true>(c, p, splits, s) : launch_dot<kn, false>(c, p, splits, s))
   switch (cols) {
     case 16: return NG_DOT(16);
     case 32: return NG_DOT(32);
     case 64: return NG_DOT(64);
-    case 128: return NG_DOT(128);
-    default: return NG_DOT(256);
+    default: return NG_DOT(128);
   }
 #undef NG_DOT
 }

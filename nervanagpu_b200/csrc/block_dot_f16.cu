@@ -18,7 +18,6 @@
 #include <atomic>
 
 #include "blocks.h"
-#include "epilogue.cuh"
 
 namespace ngb {
 
@@ -51,10 +50,7 @@ struct MixParams {
   int M, N, K;
   int tiles_n, tiles, num_kb;
   BlockView x;
-  void* C;
-  long long ldc;
-  int out_f32, store;        // store: 1 = TMA, 0 = one number per lane and access
-  EpiArgs ea;
+  OutParams out;
   int* status;
   unsigned long long wait_limit_ns;
 };
@@ -97,7 +93,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     mbar_fence_init();
     if (p.a_tma) tma_prefetch_desc(&mapA);
     tma_prefetch_desc(&mapX);
-    if (p.store) tma_prefetch_desc(&mapC);
+    if (p.out.store) tma_prefetch_desc(&mapC);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), T::kCols);
@@ -177,9 +173,6 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     const int group = warp & 3, half = (warp - 2) >> 2;
     const uint32_t stage = staging + (warp - 2) * 4096u;
     uint8_t* stage_gen = ring_gen + (stage - ring);
-    const bool f32 = !kLean && p.out_f32;
-    const int esz = f32 ? 4 : 2;
-    const int box = 128 / esz;                       // columns of a staged box
     int local = 0;
     for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++local) {
       const int acc = local & 1;
@@ -187,130 +180,11 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
       if (__any_sync(0xffffffffu, !ok)) break;
       tc_fence_after();
       const int m0 = t / p.tiles_n * 128 + group * 32, n0 = t % p.tiles_n * kN + half * T::kEpiCols;
-      const long long row = m0 + lane;
       const uint32_t taddr = tmem + (static_cast<uint32_t>(group * 32) << 16) + acc * kN + half * T::kEpiCols;
-      if (half * T::kEpiCols >= kN) {
-        if (lane == 0) mbar_arrive(acce_bar(acc));
-        continue;
-      }
-      if constexpr (kLean) {
-        const bool as_is = p.ea.alpha == 1.0f && !p.ea.relu;
-#pragma unroll 1
-        for (int c = 0; c < T::kEpiCols; c += 64) {
-          uint32_t r[2][32];
-          tc_ld_32x32(taddr + c, r[0]);
-          tc_ld_32x32(taddr + c + 32, r[1]);
-          tc_wait_ld();
-          if (c + 64 >= T::kEpiCols) {     // the accumulator has been read
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acce_bar(acc));
-          }
-          if (m0 >= p.M || n0 + c >= p.N) continue;
-          uint4 w[8];
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            __half2* h = reinterpret_cast<__half2*>(&w[g]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float a = __uint_as_float(r[g / 4][g % 4 * 8 + 2 * i]), b = __uint_as_float(r[g / 4][g % 4 * 8 + 2 * i + 1]);
-              if (!as_is) {
-                a = epi_scale(p.ea, a);
-                b = epi_scale(p.ea, b);
-              }
-              h[i] = __floats2half2_rn(a, b);
-            }
-          }
-          if (lane == 0) tma_store_wait_read<0>();       // (the box before must have left)
-          __syncwarp();
-#pragma unroll
-          for (int g = 0; g < 8; ++g) *reinterpret_cast<uint4*>(stage_gen + lane * 128 + ((g ^ (lane & 7)) << 4)) = w[g];
-          if (p.store) {
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_5d(&mapC, stage, n0 + c, m0, 0, 0, 0);
-              tma_store_commit();
-            }
-          } else {
-            // rows at any address: a row at a time, two numbers per lane
-            __syncwarp();
-            __half* out = static_cast<__half*>(p.C) + m0 * p.ldc + n0 + c + lane;
-            const int rows = min(32, p.M - m0), cols = p.N - n0 - c - lane;
-#pragma unroll 8
-            for (int i = 0; i < rows; ++i, out += p.ldc) {
-              const uint8_t* src = stage_gen + i * 128 + ((lane * 2) & 15);
-              if (cols > 0) out[0] = *reinterpret_cast<const __half*>(src + (((lane >> 3) ^ (i & 7)) << 4));
-              if (cols > 32) out[32] = *reinterpret_cast<const __half*>(src + (((4 + (lane >> 3)) ^ (i & 7)) << 4));
-            }
-            __syncwarp();
-          }
-        }
-        continue;
-      }
-#pragma unroll 1
-      for (int c = 0; c < T::kEpiCols; c += 32) {
-        uint32_t r[32];
-        tc_ld_32x32(taddr + c, r);
-        tc_wait_ld();
-        if (c + 32 >= T::kEpiCols) {     // the accumulator has been read
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(acce_bar(acc));
-        }
-        if (m0 >= p.M || n0 + c >= p.N) continue;
-        // into this lane's row of the staged box: 32 columns are 64 bytes of fp16 (half a row) or 128 of fp32
-        const int at = f32 ? 0 : (c & 32) * 2;
-        if (at == 0) {                   // (the box before must have left)
-          if (lane == 0) tma_store_wait_read<0>();
-          __syncwarp();
-        }
-        uint8_t* dst = stage_gen + lane * 128;
-        const uint32_t sw = (lane & 7) << 4;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[8 * g + i]);
-          uint4 lo, hi;
-          {
-            const int col = n0 + c + 8 * g;
-            const int nvalid = row < p.M ? max(0, min(8, p.N - col)) : 0;
-            const unsigned long long lin = static_cast<unsigned long long>(row) * p.N + col;
-            const void* oldp = nvalid > 0 ? static_cast<const uint8_t*>(p.C) + (row * p.ldc + col) * esz : nullptr;
-            if (f32) epi_pack8<true>(p.ea, v, oldp, lin, lo, hi, max(nvalid, 1));
-            else epi_pack8<false>(p.ea, v, oldp, lin, lo, hi, max(nvalid, 1));
-          }
-          if (f32) {
-            *reinterpret_cast<uint4*>(dst + ((32 * g) ^ sw)) = lo;
-            *reinterpret_cast<uint4*>(dst + ((32 * g + 16) ^ sw)) = hi;
-          } else {
-            *reinterpret_cast<uint4*>(dst + ((at + 16 * g) ^ sw)) = lo;
-          }
-        }
-        if (!f32 && at == 0 && n0 + c + 32 < p.N) continue;    // the other half of the box comes next
-        const int col0 = n0 + (f32 ? c : c & ~63);
-        if (p.store) {
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_5d(&mapC, stage, col0, m0, 0, 0, 0);
-            tma_store_commit();
-          }
-        } else {
-          __syncwarp();
-          const int rows = min(32, p.M - m0), cols = min(box, p.N - col0);
-          for (int i = 0; i < rows; ++i) {
-            uint8_t* out = static_cast<uint8_t*>(p.C) + ((m0 + i) * p.ldc + col0) * esz;
-            for (int j = lane; j < cols; j += 32) {
-              const uint8_t* src = stage_gen + i * 128 + (((j * esz) & 112) ^ ((i & 7) << 4)) + ((j * esz) & 15);
-              if (f32) reinterpret_cast<float*>(out)[j] = *reinterpret_cast<const float*>(src);
-              else reinterpret_cast<__half*>(out)[j] = *reinterpret_cast<const __half*>(src);
-            }
-          }
-          __syncwarp();
-        }
-      }
+      auto release = [&] { if (lane == 0) mbar_arrive(acce_bar(acc)); };
+      if (half * T::kEpiCols >= kN) release();
+      else if constexpr (kLean) out_lean<T::kEpiCols>(p.out, &mapC, taddr, stage, stage_gen, m0, n0, release);
+      else out_any<T::kEpiCols>(p.out, &mapC, taddr, stage, stage_gen, m0, n0, release);
     }
     if (lane == 0) tma_store_wait_all();
     __syncwarp();
@@ -399,15 +273,6 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
   }
 }
 
-// rank-2 boxes of a row-major matrix
-int plain_map(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_cols, int box_rows, int esz) {
-  const uint64_t dims[5] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows), 1, 1, 1};
-  const uint64_t row = static_cast<uint64_t>(ld) * esz, all = row * rows;
-  const uint64_t strides[4] = {row, all, all, all};
-  const uint32_t box[5] = {static_cast<uint32_t>(box_cols), static_cast<uint32_t>(box_rows), 1, 1, 1};
-  return make_tensor_map(map, base, dims, strides, box, esz);
-}
-
 template <int kN, bool kLean>
 int launch_mix(DeviceCtx* c, MixParams& p, cudaStream_t stream) {
   using T = MixTile<kN>;
@@ -420,7 +285,7 @@ int launch_mix(DeviceCtx* c, MixParams& p, cudaStream_t stream) {
   if (p.a_tma) rc = plain_map(&mapA, p.A, p.M, p.K, p.lda, 64, 128, 2);
   // (codes as 16-bit units; zeros beyond the last row)
   if (rc == NG_OK) rc = plain_map(&mapX, p.x.codes, p.N, p.x.pitch / 2, p.x.pitch / 2, 32, kN, 2);
-  if (rc == NG_OK && p.store) rc = plain_map(&mapC, p.C, p.M, p.N, p.ldc, p.out_f32 ? 32 : 64, 32, p.out_f32 ? 4 : 2);
+  if (rc == NG_OK && p.out.store) rc = out_map(&mapC, p.out);
   if (rc != NG_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, c->sm_count)));
@@ -474,11 +339,9 @@ int run_block_dot_f16(DeviceCtx* c, const void* A, int lda, const ng_block_desc&
   p.M = m; p.N = x.outer; p.K = x.inner;
   p.num_kb = (x.inner + 63) / 64;
   p.x = x;
-  p.C = C; p.ldc = ldc; p.out_f32 = out_f32;
-  p.store = (reinterpret_cast<uintptr_t>(C) & 15u) == 0 && ldc % (out_f32 ? 4 : 8) == 0;
-  p.ea = ea;
+  p.out = make_out(C, m, x.outer, ldc, out_f32, ea);
   p.status = c->status; p.wait_limit_ns = c->wait_limit_ns;
-  const bool lean = !out_f32 && ea.beta == 0.0f && ea.sr_bits == 0;
+  const bool lean = out_is_lean(p.out);
   // Columns of a tile: what takes the SMs least time, a tile of n columns counted as n + 64 (its rows of A, its start
   // and its end). 1001 x 4097 x 125: one round of 136 tiles of 256 columns, or four of 520 tiles of 64.
   const long long row_tiles = (m + 127ll) / 128;

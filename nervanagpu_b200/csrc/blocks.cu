@@ -685,6 +685,25 @@ int block_view(const DeviceCtx* c, const ng_block_desc* d, BlockView& v) {
   return NG_OK;
 }
 
+int plain_map(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_cols, int box_rows, int esz) {
+  const uint64_t dims[5] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows), 1, 1, 1};
+  const uint64_t row = static_cast<uint64_t>(ld) * esz, all = row * rows;
+  const uint64_t strides[4] = {row, all, all, all};
+  const uint32_t box[5] = {static_cast<uint32_t>(box_cols), static_cast<uint32_t>(box_rows), 1, 1, 1};
+  return make_tensor_map(map, base, dims, strides, box, esz);
+}
+
+OutParams make_out(void* C, int m, int n, int ldc, int out_f32, const EpiArgs& ea) {
+  OutParams out = {};
+  out.M = m; out.N = n; out.C = C; out.ldc = ldc; out.out_f32 = out_f32; out.ea = ea;
+  out.store = (reinterpret_cast<uintptr_t>(C) & 15u) == 0 && ldc % (out_f32 ? 4 : 8) == 0;
+  return out;
+}
+
+int out_map(CUtensorMap* map, const OutParams& out) {
+  return plain_map(map, out.C, out.M, out.N, out.ldc, out.out_f32 ? 32 : 64, 32, out.out_f32 ? 4 : 2);
+}
+
 int dequantize_f16(DeviceCtx* c, const ng_block_desc& d, const BlockView& q, __half* out, long long ld, cudaStream_t stream) {
   PlainView<__half> a = {out, ld, 1};
   NG_BY_FORMAT(d.format, return (dequantize_one<__half, kF>(c, q, a, stream)));

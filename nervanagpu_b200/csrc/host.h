@@ -101,9 +101,9 @@ class AuxClaim {
 };
 
 // Rank-5 tiled tensor map over fp16 (elem_bytes 2) data. dims[0] is the contiguous dimension;
-// strides_bytes[i] is the byte stride of dims[i+1]. Swizzle is chosen from the inner box width.
+// strides_bytes[i] is the byte stride of dims[i+1]. Swizzle is chosen from the inner box width, none if `plain`.
 int make_tensor_map(CUtensorMap* out, const void* base, const uint64_t dims[5], const uint64_t strides_bytes[4],
-                    const uint32_t box[5], int elem_bytes = 2);
+                    const uint32_t box[5], int elem_bytes = 2, bool plain = false);
 
 // Fill the MMA/ring fields of a parameter block and launch the tensor-core kernel (+ split-K reduce).
 struct TcOperandLayout {

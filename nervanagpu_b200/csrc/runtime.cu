@@ -186,7 +186,7 @@ static EncodeTiledFn get_encode_fn() {
 }
 
 int make_tensor_map(CUtensorMap* out, const void* base, const uint64_t dims[5], const uint64_t strides_bytes[4],
-                    const uint32_t box[5], int elem_bytes) {
+                    const uint32_t box[5], int elem_bytes, bool plain) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return fail(NG_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available from the driver");
   cuuint64_t gdim[5], gstr[4];
@@ -199,7 +199,8 @@ int make_tensor_map(CUtensorMap* out, const void* base, const uint64_t dims[5], 
   for (int i = 0; i < 4; ++i) gstr[i] = strides_bytes[i];
   const uint32_t inner_bytes = box[0] * elem_bytes;
   CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_NONE;
-  if (inner_bytes == 128) sw = CU_TENSOR_MAP_SWIZZLE_128B;
+  if (plain) sw = CU_TENSOR_MAP_SWIZZLE_NONE;
+  else if (inner_bytes == 128) sw = CU_TENSOR_MAP_SWIZZLE_128B;
   else if (inner_bytes == 64) sw = CU_TENSOR_MAP_SWIZZLE_64B;
   else if (inner_bytes == 32) sw = CU_TENSOR_MAP_SWIZZLE_32B;
   CUtensorMapDataType dt = elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;

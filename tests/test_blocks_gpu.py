@@ -214,7 +214,7 @@ def operands(rng, fmt, m, n, k):
 
 
 SIZES = [(1, 1, 1), (1, 1, 16), (3, 5, 33), (16, 1, 256), (128, 128, 256), (130, 17, 300), (257, 33, 1000), (1001, 125, 4097),
-         (64, 300, 513), (200, 129, 64), (384, 65, 2048), (5, 1000, 640), (1, 4096, 512), (4096, 1, 4096), (640, 520, 768), (2500, 2304, 512)]
+         (64, 300, 513), (200, 129, 64), (384, 65, 2048), (5, 1000, 640), (1, 4096, 512), (4096, 1, 4096), (640, 520, 768), (2500, 2304, 512), (2049, 2101, 1030), (2304, 2048, 2300)]
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
@@ -238,7 +238,7 @@ def test_block_dot(ng, fmt, m, n, k):
     assert np.array_equal(first, F.get())
 
 
-@pytest.mark.parametrize("m,n,k", [(70, 50, 100), (200, 300, 513), (9, 700, 96), (256, 128, 1024)])
+@pytest.mark.parametrize("m,n,k", [(70, 50, 100), (200, 300, 513), (9, 700, 96), (256, 128, 1024), (2100, 2061, 300)])
 @pytest.mark.parametrize("mixed", [False, True])
 def test_product_output_stage(ng, m, n, k, mixed):
     """alpha, ReLU, what is added to, rounding to nearest and stochastically, rows inside a wider matrix."""
