@@ -1,13 +1,16 @@
 """Whole-network forward / backward timing through the Layer classes.
 
     python -m nervanagpu_b200.convnet_benchmarks [--nets Alexnet,VGG] [--loops 10] [--layer-bench] [--stats]
+                                                 [--checkpoint] [--products mxfp4|nvfp4]
 
 The counterpart of the reference's benchmarks/convnet-benchmarks.py:250-403: each network is a list
 of layer configurations turned into Layer objects by Layer.create, delta buffers are shared between
 alternating layers, the initial weights are scaled so that activations stay near 1, and `loops`
 iterations of fprop over all layers and bprop (deltas, weight update and SGD step, in reverse) are
 timed with events. Output lines have the reference's form ("Avg(10) fprop: ... msecs ... gflops"),
-flops per layer from Layer.flops with the backward pass counted twice.
+flops per layer from Layer.flops with the backward pass counted twice. --checkpoint keeps the inputs of
+convolutions and fully-connected layers as 8-bit records for the backward pass and lets their fp16 forms share two
+buffers; --products takes the fully-connected layers' forward products from 4-bit blocks.
 
 Networks: the convolution/pooling/fully-connected stacks of AlexNet (one-column variant), Overfeat
 (fast), VGG model A and VGG model E as the public convnet-benchmarks lists them, and GoogLeNet (v1,
@@ -20,7 +23,7 @@ import ctypes
 import numpy as np
 
 from . import NervanaGPU, _lib
-from .layers import ConvLayer, DataLayer, FullLayer, Inception, Layer, PoolLayer
+from .layers import ConvLayer, DataLayer, FullLayer, Inception, Layer, PoolLayer, link_records
 
 
 def _conv(K, R, pad=0, stride=1):
@@ -104,10 +107,14 @@ class _Stopwatch(object):
         return ms.value
 
 
-def build_network(ng, confs, dtype=np.float16, zeros=False, seed=0):
+def build_network(ng, confs, dtype=np.float16, zeros=False, seed=0, checkpoint=False, products=None):
     """Layer objects with activations, weights and (shared) delta buffers in place."""
     layers, prev = [], None
     for conf in confs:
+        if checkpoint and conf["layer"] in (ConvLayer, FullLayer) and type(prev) is not DataLayer:   # (data stays)
+            conf = dict(conf, checkpoint=True)
+        if products and conf["layer"] is FullLayer:
+            conf = dict(conf, products=products)
         prev = Layer.create(ng, conf, prev, dtype)
         layers.append(prev)
     # the two largest delta buffers and the largest weight-gradient buffer are shared by all layers
@@ -115,9 +122,19 @@ def build_network(ng, confs, dtype=np.float16, zeros=False, seed=0):
     widest = max(layers, key=lambda l: l.sizeF)
     shared_deltas = [ng.empty(deltas.dimI, dtype=deltas.dtype), ng.empty(deltas.dimI, dtype=deltas.dtype)]
     shared_updates = ng.empty(widest.dimF, dtype=np.float32)
+    released = link_records(layers)
+    shared_acts = shared_inputs = None
+    if any(released):
+        largest = max((l for l, r in zip(layers, released) if r), key=lambda l: l.sizeO)
+        shared_acts = [ng.empty(largest.dimO, dtype=largest.dtype), ng.empty(largest.dimO, dtype=largest.dtype)]
+    recorded = [l for l in layers if l.checkpoint and isinstance(l, ConvLayer)]
+    if recorded:
+        shared_inputs = ng.empty(max(recorded, key=lambda l: l.sizeI).dimI, dtype=dtype)
+        for layer in recorded:
+            layer.init_restored(shared_inputs)
     rng = np.random.RandomState(seed)
     for i, layer in enumerate(layers):
-        layer.init_activations()
+        layer.init_activations(shared_acts if released[i] else None)
         layer.init_weights(shared=shared_updates, zeros=zeros, rng=rng)
         if i > 1:
             layer.init_deltas(shared=shared_deltas)
@@ -133,13 +150,13 @@ def build_network(ng, confs, dtype=np.float16, zeros=False, seed=0):
     return layers
 
 
-def run_network(ng, name, loops=10, stats=False, zeros=False, out=print):
+def run_network(ng, name, loops=10, stats=False, zeros=False, out=print, checkpoint=False, products=None):
     warmup, confs = NETWORKS[name]
     title = "%s (dtype=float16, N=%d)" % (name, confs[0]["N"])
     out("------------------------------------------------")
     out("Benchmarking: " + title)
     out("------------------------------------------------")
-    layers = build_network(ng, confs, zeros=zeros)
+    layers = build_network(ng, confs, zeros=zeros, checkpoint=checkpoint, products=products)
     watch = _Stopwatch(ng)
     totals = {"fprop": [0.0, 0.0], "bprop": [0.0, 0.0]}
     for it in range(loops + warmup):
@@ -189,12 +206,15 @@ def main():
     ap.add_argument("--layer-bench", action="store_true", help="print the time of every conv / pool / GEMM call")
     ap.add_argument("--stats", action="store_true", help="print activation / delta / update statistics per layer")
     ap.add_argument("--zeros", action="store_true", help="all-zero data and weights")
+    ap.add_argument("--checkpoint", action="store_true", help="8-bit records of layer inputs for the backward pass")
+    ap.add_argument("--products", choices=("mxfp4", "nvfp4"), help="fully-connected products from 4-bit blocks")
     args = ap.parse_args()
     ng = NervanaGPU(stochastic_round=False, bench=args.layer_bench)
     for name in args.nets.split(","):
         if name not in NETWORKS:
             raise SystemExit("unknown network %s (have: %s)" % (name, ", ".join(sorted(NETWORKS))))
-        run_network(ng, name, loops=args.loops, stats=args.stats, zeros=args.zeros)
+        run_network(ng, name, loops=args.loops, stats=args.stats, zeros=args.zeros, checkpoint=args.checkpoint,
+                    products=args.products)
 
 
 if __name__ == "__main__":

@@ -426,11 +426,11 @@ __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(Block
       scales[row * 4 + which] = n > 0 && o0 + row < q.outer ? static_cast<uint8_t>(s.byte) : 0;
     }
     __syncthreads();
-    // (a group of four blocks is whole within a row's padding; what lies behind the last number is zero)
+    // (what lies behind the last number is zero; 4-bit rows are padded to four blocks and more, mxfp8 rows to one)
 #pragma unroll
     for (int i = threadIdx.x; i < kStridedRows * (S::kRow / 16); i += kStridedThreads) {
       const int row = i / (S::kRow / 16), c = i % (S::kRow / 16);
-      if (o0 + row < q.outer)
+      if (o0 + row < q.outer && (F::k4 || b0 * S::kBytes + c * 16ll < q.pitch))
         *reinterpret_cast<uint4*>(q.codes + F::code_at(q, o0 + row, static_cast<long long>(b0) * S::kBytes + c * 16)) =
             *reinterpret_cast<const uint4*>(codes + row * S::kPitch + c * 16);
     }
@@ -645,11 +645,11 @@ static void block_pitches(const ng_block_desc& d, BlockView& v) {
   v.inner = d.axis ? d.cols : d.rows;
   if (d.format == NG_BLOCK_MXFP8) {
     v.tile = 0;
-    v.pitch = (v.inner + kRowPad - 1ll) / kRowPad * kRowPad;
-    v.spitch = v.pitch / 32;
+    v.pitch = (v.inner + 31ll) / 32 * 32;
+    v.spitch = (v.inner + 127ll) / 128 * 4;
   } else {
     const long long kbs = (v.inner + 255ll) / 256;
-    v.tile = block_tile_rows(v.outer) * kRowPad;
+    v.tile = block_tile_rows(v.outer) * kTileRow;
     v.pitch = kbs * v.tile;
     v.spitch = kbs * (d.format == NG_BLOCK_NVFP4 ? 4 : 2) * kScaleTile;
   }
@@ -675,7 +675,7 @@ int block_view(const DeviceCtx* c, const ng_block_desc* d, BlockView& v) {
   const int rc = check_shape(d);
   if (rc != NG_OK) return rc;
   if (!d->codes || !d->scales) return fail(NG_ERR_INVALID_ARG, "block matrix without memory");
-  if ((reinterpret_cast<uintptr_t>(d->codes) | reinterpret_cast<uintptr_t>(d->scales)) & (kRowPad - 1))
+  if ((reinterpret_cast<uintptr_t>(d->codes) | reinterpret_cast<uintptr_t>(d->scales)) & 127)
     return fail(NG_ERR_INVALID_ARG, "codes and scales must be 128-byte aligned");
   if (d->device != c->device) return fail(NG_ERR_INVALID_ARG, "block matrix of device %d, the current device is %d", d->device, c->device);
   block_pitches(*d, v);

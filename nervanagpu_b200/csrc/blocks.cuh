@@ -19,7 +19,7 @@
 //
 // Layout. The matrix is stored along its blocked axis ("inner"), a row of codes per index of the other axis ("outer"),
 // two 4-bit codes per byte (the even one in the low half).
-//   mxfp8: rows of codes one behind the other, padded with zeros to 128 bytes; rows of scales likewise (4 per 128).
+//   mxfp8: rows of codes one behind the other, padded with zeros to whole blocks; rows of scales likewise, to 4.
 //   4-bit formats: as shared and tensor memory hold them, so that a product's operands are plain contiguous copies,
 //   without a tensor map to build and fetch and without a stride between their rows. Tiles of 128 outer rows (fewer
 //   in a matrix of at most 64: 16, 32 or 64) x 128 bytes = 256 numbers, the tiles of 128 rows along the inner axis
@@ -33,7 +33,7 @@
 
 namespace ngb {
 
-constexpr int kRowPad = 128;        // bytes: mxfp8 rows are multiples of this, tiles' rows have as many
+constexpr int kTileRow = 128;       // bytes of a row of a tile of 4-bit codes
 constexpr int kScaleTile = 512;     // bytes of a tile of 4-bit formats' scales
 
 // What a kernel needs to know of a matrix in blocks.

@@ -38,9 +38,19 @@ class Layer(object):
         self.fprop_out = None
         self.bprop_out = None
         self.learning_rate = 0.0
+        # 8-bit records (see record_input): whether this layer keeps one of its input and masks the deltas it passes
+        # down by it, and whether the layer above does that for this one
+        self.checkpoint = False
+        self.record = None
+        self.masks_below = self.masked_above = False
 
-    def init_activations(self):
-        self.fprop_out = self.lib.empty(self.dimO, dtype=self.dtype)
+    def init_activations(self, shared=None):
+        """shared: two buffers that layers take in turn (their outputs are then gone when the next but one runs)."""
+        if shared is None:
+            self.fprop_out = self.lib.empty(self.dimO, dtype=self.dtype)
+        else:
+            self.fprop_out = shared[0].share(self.dimO)
+            shared.reverse()
         self.act_stats = self.lib.empty((self.dimO2[0], 1), dtype=np.float32)
 
     def init_deltas(self, shared=None):
@@ -76,7 +86,27 @@ class Layer(object):
     def bprop(self, bprop_in):
         return bprop_in
 
+    def record_input(self, fprop_in, *operands):
+        """Quantise the input into this layer's 8-bit record, for its backward pass, and into any operands of its
+        product, in one call. With a record, a layer needs its input no more after its forward pass: the weight
+        gradient is taken from the record, and so is the mask of the ReLU below. (An extension: the reference keeps
+        every activation in fp16, nervanagpu/layers.py:64-70.)"""
+        outs = list(operands)
+        if self.checkpoint:
+            if self.record is None:
+                self.record = self.lib.block_empty(self.dimI2, "mxfp8")
+            outs.append(self.record)
+        if outs:
+            self.lib.quantize(fprop_in.reshape(self.dimI2), *outs)
+
+    def mask_below(self):
+        """The ReLU mask of the layer below on the deltas this layer passes down."""
+        if self.masks_below and self.bprop_out is not None:
+            self.lib.relu_mask(self.record, self.bprop_out.reshape(self.dimI2))
+
     def bprop_relu(self, bprop_in):
+        if self.masked_above:
+            return bprop_in
         # the forward ReLU is fused into the conv / GEMM epilogue; its gradient is a mask
         bprop_in *= self.fprop_out > 0
         return bprop_in
@@ -187,8 +217,18 @@ class DataLayer(Layer):
 
 
 class FullLayer(Layer):
-    def __init__(self, lib, dtype, N, nIn, nOut):
+    """products: "mxfp4" or "nvfp4" for a forward product from weights and inputs in 4-bit blocks (block_dot); the
+    backward pass multiplies with the fp16 weights. scales: the powers of two of nvfp4 weights and inputs. The weights are
+    quantised in every forward pass, as they change in every step, or once by fix_weights, for inference.
+    checkpoint: keep the input as an 8-bit record for the backward pass (see Layer.record_input)."""
+
+    def __init__(self, lib, dtype, N, nIn, nOut, products=None, scales=(2.0 ** -10, 2.0 ** -2), checkpoint=False):
         super(FullLayer, self).__init__(lib, dtype, N)
+        if products not in (None, "mxfp4", "nvfp4"):
+            raise ValueError("products are fp16 (None), mxfp4 or nvfp4, not %r" % (products,))
+        self.products, self.scales, self.checkpoint = products, scales, bool(checkpoint)
+        self.weight_blocks = self.input_blocks = None
+        self.weights_fixed = False
         self.nIn, self.nOut = nIn, nOut
         self.flops = N * nIn * nOut * 2.0
         self.dimI = self.dimI2 = (nIn, N)
@@ -196,9 +236,38 @@ class FullLayer(Layer):
         self.dimF = self.dimF2 = (nOut, nIn)
         self.sizeI, self.sizeO, self.sizeF = nIn * N, nOut * N, nIn * nOut
 
+    def quantize_weights(self):
+        if self.weight_blocks is None:
+            ws, xs = self.scales if self.products == "nvfp4" else (1.0, 1.0)
+            self.weight_blocks = self.lib.block_empty(self.dimF, self.products, axis=1, scale=ws)
+            self.input_blocks = self.lib.block_empty(self.dimI, self.products, axis=0, scale=xs)
+        self.lib.quantize(self.weights, self.weight_blocks)
+
+    def fix_weights(self):
+        """Quantise the weights now and no more until the next descent: for inference. A program that writes `weights`
+        itself calls this again."""
+        if self.products:
+            self.quantize_weights()
+            self.weights_fixed = True
+
+    def grad_descent(self):
+        super(FullLayer, self).grad_descent()
+        self.weights_fixed = False
+
+    def scale_weights(self, scale):
+        super(FullLayer, self).scale_weights(scale)
+        self.weights_fixed = False
+
     def fprop(self, fprop_in, scale_weights=0):
         fprop_in = super(FullLayer, self).fprop(fprop_in)
-        self.lib.dot(self.weights, fprop_in, self.fprop_out, relu=True)
+        if self.products:
+            if not self.weights_fixed:
+                self.quantize_weights()
+            self.record_input(fprop_in, self.input_blocks)
+            self.lib.block_dot(self.weight_blocks, self.input_blocks, self.fprop_out, relu=True)
+        else:
+            self.record_input(fprop_in)
+            self.lib.dot(self.weights, fprop_in, self.fprop_out, relu=True)
         if scale_weights:
             self.scale_weights(scale_weights)
             self.fprop(fprop_in)
@@ -207,21 +276,31 @@ class FullLayer(Layer):
     def bprop(self, bprop_in):
         self.bprop_relu(bprop_in)
         self.lib.dot(self.weights.T, bprop_in, self.bprop_out)
-        self.lib.dot(bprop_in, self.fprop_in.T, self.updat_out)
+        if self.checkpoint:
+            self.lib.block_dot(bprop_in, self.record.T, self.updat_out)
+        else:
+            self.lib.dot(bprop_in, self.fprop_in.T, self.updat_out)
         self.grad_descent()
+        self.mask_below()
         return self.bprop_out
 
     def __str__(self):
-        return "FullLayer: N, nIn, nOut: (%d, %d, %d)" % (self.N, self.nIn, self.nOut)
+        extra = (" products: %s" % self.products if self.products else "") + (" checkpoint" if self.checkpoint else "")
+        return "FullLayer: N, nIn, nOut: (%d, %d, %d)%s" % (self.N, self.nIn, self.nOut, extra)
 
 
 class ConvLayer(Layer):
-    """Convolution parameters: I (C,D,H,W,N) * F (C,T,R,S,K) -> O (K,M,P,Q,N)."""
+    """Convolution parameters: I (C,D,H,W,N) * F (C,T,R,S,K) -> O (K,M,P,Q,N).
+
+    checkpoint: keep the input as an 8-bit record for the backward pass (see Layer.record_input), which brings it back into
+    `restored`, a buffer that layers can share (init_restored)."""
 
     def __init__(self, lib, dtype, N, C, K, D=1, H=1, W=1, T=1, R=1, S=1, pad_d=0, pad_h=0, pad_w=0,
-                 str_d=1, str_h=1, str_w=1, grid_P=0, grid_Q=0, update_size=None):
+                 str_d=1, str_h=1, str_w=1, grid_P=0, grid_Q=0, update_size=None, checkpoint=False):
         # weight gradients are produced in fp32 (nervanagpu/layers.py:289)
         super(ConvLayer, self).__init__(lib, dtype, N, np.float32)
+        self.checkpoint = bool(checkpoint)
+        self.restored = None
         assert N % 8 == 0, "N dim must be multiple of 8"
         assert K % 8 == 0, "K dim must be multiple of 8"
 
@@ -254,6 +333,7 @@ class ConvLayer(Layer):
 
     def fprop(self, fprop_in, scale_weights=0):
         fprop_in = super(ConvLayer, self).fprop(fprop_in)
+        self.record_input(fprop_in)
         self.lib.fprop_conv(self, fprop_in, self.weights, self.fprop_out, relu=True)
         if scale_weights:
             self.scale_weights(scale_weights)
@@ -264,9 +344,19 @@ class ConvLayer(Layer):
         self.bprop_relu(bprop_in)
         if self.bprop_out is not None:
             self.lib.bprop_conv(self, self.weights, bprop_in, self.bprop_out)
-        self.lib.update_conv(self, self.fprop_in, bprop_in, self.updat_out)
+        inputs = self.fprop_in
+        if self.checkpoint:
+            if self.restored is None:
+                self.init_restored()
+            inputs = self.restored
+            self.lib.dequantize(self.record, inputs.reshape(self.dimI2))
+        self.lib.update_conv(self, inputs, bprop_in, self.updat_out)
         self.grad_descent()
+        self.mask_below()
         return self.bprop_out
+
+    def init_restored(self, shared=None):
+        self.restored = self.lib.empty(self.dimI, dtype=self.dtype) if shared is None else shared.share(self.dimI)
 
     def __str__(self):
         return ("ConvLayer: NCK: (%d, %d, %d) DHW:%s TRS:%s MPQ:%s" %
@@ -292,7 +382,7 @@ class DeconvLayer(ConvLayer):
         self.lib.bprop_conv(self, self.weights, self.fprop_in, self.fprop_out)
         return self.fprop_out
 
-    def init_activations(self):
+    def init_activations(self, shared=None):
         self.fprop_out = self.lib.empty(self.dimI, dtype=self.dtype)
         self.act_stats = self.lib.empty((self.dimI2[0], 1), dtype=np.float32)
 
@@ -397,7 +487,7 @@ class Inception(Layer):
         if self.sizeF:
             self.dimF = widest.dimF
 
-    def init_activations(self):
+    def init_activations(self, shared=None):
         super(Inception, self).init_activations()
         k0 = 0
         for part in self.partitions:
@@ -457,3 +547,20 @@ class Inception(Layer):
             lines.append("  Part%d:" % (i + 1))
             lines.extend("    %s" % layer for layer in part)
         return "\n".join(lines)
+
+
+def link_records(layers):
+    """For a chain of layers some of which keep 8-bit records of their inputs: such a layer masks the deltas that it
+    passes to a convolution or fully-connected layer below by that layer's ReLU, which then does not do it itself.
+    Returns, for each layer, whether its output is not needed any more once the layer above has run (the backward pass
+    of a pooling layer reads its input, not its output): these outputs can share buffers (init_activations(shared))."""
+    released = [False] * len(layers)
+    for i in range(len(layers) - 1):
+        below, above = layers[i], layers[i + 1]
+        if not above.checkpoint:
+            continue
+        relu = type(below) in (ConvLayer, FullLayer)
+        if relu:
+            above.masks_below = below.masked_above = True
+        released[i] = relu or type(below) is PoolLayer
+    return released

@@ -108,9 +108,9 @@ def test_c_entries_refuse_before_they_touch_a_device(lib):
 
 
 @pytest.mark.parametrize("fmt,axis,shape,codes,scales", [
-    ("mxfp4", 1, (1, 1), 2048, 1024), ("nvfp4", 1, (1, 1), 2048, 2048), ("mxfp8", 1, (1, 1), 128, 4),
+    ("mxfp4", 1, (1, 1), 2048, 1024), ("nvfp4", 1, (1, 1), 2048, 2048), ("mxfp8", 1, (1, 1), 32, 4), ("mxfp8", 1, (100, 64), 6400, 400), ("mxfp8", 1, (100, 129), 16000, 800),
     ("nvfp4", 1, (20, 257), 32 * 256, 4096), ("mxfp4", 1, (64, 256), 64 * 128, 1024), ("mxfp4", 1, (65, 256), 128 * 128, 1024),
-    ("nvfp4", 1, (129, 257), 256 * 256, 2 * 4096), ("mxfp4", 0, (257, 129), 256 * 256, 2 * 2048), ("mxfp8", 0, (257, 129), 129 * 384, 129 * 12),
+    ("nvfp4", 1, (129, 257), 256 * 256, 2 * 4096), ("mxfp4", 0, (257, 129), 256 * 256, 2 * 2048), ("mxfp8", 0, (257, 129), 129 * 288, 129 * 12),
     ("nvfp4", 1, (70000, 70000), 547 * 274 * 16384, 547 * 274 * 2048)])
 def test_sizes(lib, fmt, axis, shape, codes, scales):
     a, b = ctypes.c_size_t(), ctypes.c_size_t()
