@@ -25,8 +25,6 @@ struct PlainView {
   bool wide;        // rows form: every row starts on 32 bytes
 };
 
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ void from_f32(float v, __half& x) { x = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(float v, float& x) { x = v; }
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -85,6 +83,25 @@ struct Raw {
     }
   }
 };
+
+// the h-th 8 of them in fp32
+__device__ __forceinline__ void to_f32x8(const Raw<__half>& r, int h, float (&x)[8]) {
+  const uint32_t w[4] = {r.v[h].x, r.v[h].y, r.v[h].z, r.v[h].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void to_f32x8(const Raw<float>& r, int h, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint4 w = r.v[2 * h + i];
+    x[4 * i] = __uint_as_float(w.x); x[4 * i + 1] = __uint_as_float(w.y);
+    x[4 * i + 2] = __uint_as_float(w.z); x[4 * i + 3] = __uint_as_float(w.w);
+  }
+}
 
 // Largest magnitude, as the bits of an fp32 number (above those of infinity for a NaN).
 __device__ __forceinline__ uint32_t top_bits(const Raw<__half>& r) {
@@ -161,7 +178,7 @@ __device__ __forceinline__ void warp_store(T* base, long long so, long long o_fi
   const long long step = static_cast<long long>(gridDim.y) * blockDim.y
 
 template <typename T, int kFmt, bool kVec>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(BlockView q, PlainView<const T> a, int early) {
+__global__ void __launch_bounds__(256, !kVec && sizeof(T) == 4 ? 6 : 4) quantize_rows_kernel(BlockView q, PlainView<const T> a, int early) {
   NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
   NG_ROWS_PROLOGUE(T);
@@ -185,7 +202,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(BlockView q, PlainVi
       const bool live = o < q.outer && n > 0;
       uint32_t top = top_bits(raw[u]);
       if (!F::kNv) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      const BlockScale s = block_scale<kFmt>(top, q.t);
+      const BlockScale s = block_scale<kFmt, sizeof(T) == 2>(top, q.t);
       uint2 c[2];
       // (by up to 2^30 is two fp16 factors; a block of zeros needs none)
       if (!F::k4 && sizeof(T) == 2 && !s.nan && (s.by <= 1073741824.0f || top == 0u)) {
@@ -200,8 +217,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(BlockView q, PlainVi
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float x[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = to_f32(raw[u].at()[8 * h + i]);
+          to_f32x8(raw[u], h, x);
           c[h] = block_encode8<kFmt, sizeof(T) == 2>(x, s);
         }
       }
@@ -345,7 +361,10 @@ template <>
 struct Pair<__half> {
   using Vec = uint32_t;
   static __device__ __forceinline__ Vec of(__half a, __half b) { return __half_as_ushort(a) | static_cast<uint32_t>(__half_as_ushort(b)) << 16; }
-  static __device__ __forceinline__ float get(Vec v, int j) { return __half2float(__ushort_as_half(static_cast<uint16_t>(j ? v >> 16 : v & 0xffffu))); }
+  static __device__ __forceinline__ float get(Vec v, int j) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&v);
+    return j ? __high2float(h) : __low2float(h);
+  }
 };
 template <>
 struct Pair<float> {
@@ -412,7 +431,7 @@ __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(Block
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int row = strided_row<kVec>(j);
-      const BlockScale s = block_scale<kFmt>(top[j], q.t);
+      const BlockScale s = block_scale<kFmt, sizeof(T) == 2>(top[j], q.t);
       uint8_t* dst = codes + row * S::kPitch + which * S::kBytes;
 #pragma unroll
       for (int h = 0; h < F::kBlock / 8; ++h) {

@@ -105,14 +105,25 @@ struct BlockScale {
   float by;
   bool nan;
 };
-template <int kFmt>
+// 1 / x to within 2^-22 of it, for a normal x
+__device__ __forceinline__ float rcp_near(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// kHalf: the numbers came from fp16.
+template <int kFmt, bool kHalf>
 __device__ __forceinline__ BlockScale block_scale(uint32_t amax_bits, float t) {
   BlockScale s;
   s.nan = amax_bits >= 0x7f800000u;
   if (BlockFormat<kFmt>::kNv) {
-    // (amax / 6t is rounded to fp32 first. That cannot put it on the border between two E4M3 numbers, 5 bits long:
-    // an fp32 number next to 6 t * border is more than half an ulp of the quotient away from it.)
-    s.byte = s.nan ? 0x7fu : cvt_e4m3x2(__fdiv_rn(__uint_as_float(amax_bits), 6.0f * t), 0.0f);
+    // amax / 6t is rounded before it is rounded to E4M3. Neither way can that put it on the border between two of
+    // those, 5 bits long, or off it: an fp32 number next to 6 t * border is more than half an ulp of the quotient away
+    // from it; fp16 numbers are 2^-11 of it away, and their quotients, off by 2^-21 at most, are rounded to 16 bits.
+    float quotient;
+    if (kHalf) quotient = __uint_as_float((__float_as_uint(__uint_as_float(amax_bits) * rcp_near(6.0f * t)) + 0x40u) & ~0x7fu);
+    else quotient = __fdiv_rn(__uint_as_float(amax_bits), 6.0f * t);
+    s.byte = s.nan ? 0x7fu : cvt_e4m3x2(quotient, 0.0f);
     if (s.byte == 0u) s.byte = 1u;
     s.by = __low2float(half2_of_e4m3x2(s.byte)) * t;
   } else {
@@ -137,15 +148,23 @@ __device__ __forceinline__ uint2 block_encode8(const float (&x)[8], const BlockS
       for (int i = 0; i < 8; ++i) y[i] = x[i] * s.by;
     } else if constexpr (kHalf) {
       // An IEEE division per number made this kernel issue-bound (4096 x 9216: 34 us). The product with the
-      // reciprocal is off by 2^-23 of the quotient, which matters on the border between two codes only; rounded to a
+      // reciprocal is off by 2^-21 of the quotient, which matters on the border between two codes only; rounded to a
       // multiple of 2^-15 (the sum with 384 has that for its last bit) it is on the border when the quotient is: the
       // border times the scale has at most 7 bits, and an fp16 number that differs from it does so by 2^-11 of it.
-      const float inv = __frcp_rn(s.by);
+      const float inv = rcp_near(s.by);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = fmaf(x[i], inv, 384.0f) - 384.0f;
     } else {
+      // An fp32 number may be closer to a border. The multiple of 2^-15 is then the border itself, its product with the
+      // scale is exact, and the sign of what it leaves of x tells the side: a step of up to 2^-17 that way. (A number
+      // that leaves something leaves at least 2^-26 of the scale there; elsewhere the next border is 2^-15 away, the
+      // quotient's own error, 2^-21 of up to 6.5, less than half of that.)
+      const float inv = rcp_near(s.by), sure = inv * 1024.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], s.by);
+      for (int i = 0; i < 8; ++i) {
+        const float q = fmaf(x[i], inv, 384.0f) - 384.0f;
+        y[i] = q + fminf(fmaxf(fmaf(-q, s.by, x[i]) * sure, -7.62939453125e-06f), 7.62939453125e-06f);
+      }
     }
     r.x = cvt_e2m1x8(y);
     if (s.nan) r.x = 0u;
