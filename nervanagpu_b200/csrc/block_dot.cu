@@ -18,6 +18,7 @@
 //   all        sum over the cluster, output stage (epilogue.cuh), stores
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "block_mma.cuh"
 #include "blocks.h"
@@ -39,18 +40,19 @@ struct DotTile {
   static constexpr uint32_t kCodesB = kN * 128u;
   static constexpr uint32_t kScales = kScaleTiles * kScaleTile;      // of 128 rows
   static constexpr uint32_t kStageBytes = (kCodesA + kCodesB + 2 * kScales + 1023u) & ~1023u;
-  static constexpr int kStages =
-      static_cast<int>((kDotSmemLimit - 1024u - kDotCtrl) / kStageBytes) < kDotStages ? static_cast<int>((kDotSmemLimit - 1024u - kDotCtrl) / kStageBytes) : kDotStages;
+  // partial tiles in shared memory: rows of kN + 4 floats, so that lanes in successive rows meet different banks
+  static constexpr int kPitch = kN + 4;
+  static constexpr uint32_t kParts = 128u * kPitch * 4u;
+  static constexpr int kRoom = static_cast<int>((kDotSmemLimit - 1024u - kDotCtrl - kParts) / kStageBytes);
+  static constexpr int kStages = kRoom < kDotStages ? kRoom : kDotStages;
   // tensor memory: the accumulator, then two buffers of scales, A's before B's
   static constexpr int kAccCols = kN < 32 ? 32 : kN;
   static constexpr int kScaleCols = kScaleTiles * 8;
   static constexpr int kColsUsed = kAccCols + 2 * kScaleCols;
   static constexpr uint32_t kCols = kColsUsed <= 128 ? 128 : 256;
-  // partial tiles in shared memory: rows of kN + 4 floats, so that lanes in successive rows meet different banks
-  static constexpr int kPitch = kN + 4;
-  static constexpr uint32_t kSmem = kStages * kStageBytes + 1024u + kDotCtrl;
-  // (the partial tile takes the ring's place, and behind it, when it is split, this CTA's share of the sum)
-  static_assert(2 * 128u * kPitch * 4u <= kStages * kStageBytes, "the ring is smaller than the tile");
+  static constexpr uint32_t kSmem = kStages * kStageBytes + kParts + kDotCtrl + 1024u;
+  // (this CTA's tile takes the ring's place when its products are done; the others' parts of its share have their own)
+  static_assert(kParts <= kStages * kStageBytes, "the ring is smaller than the tile");
 };
 
 struct DotParams {
@@ -86,7 +88,9 @@ __device__ __forceinline__ void bulk_push(uint32_t dst_cluster, uint32_t src, ui
                "r"(src), "r"(bytes), "r"(bar_cluster)
                : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+// (relaxed: neither arrival publishes memory. The barriers that the first tells of are fenced when they are made, the second
+// only says that nobody reads this CTA's tile any more. As a release each took half a microsecond.)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // One output, in fp16 or fp32 (the arithmetic of epi_store8).
 __device__ __forceinline__ void epi_store1(const EpiArgs& e, float acc, void* out, int out_f32, unsigned long long lin) {
@@ -118,12 +122,12 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
   using T = DotTile<kN, kNv>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t ctrl = ring + T::kStages * T::kStageBytes;
+  const uint32_t parts = ring + T::kStages * T::kStageBytes, ctrl = parts + T::kParts;
   uint8_t* ring_gen = smem_raw + (ring - smem_u32(smem_raw));
   auto full_bar = [&](int s) { return ctrl + 8u * s; };
   auto empty_bar = [&](int s) { return ctrl + 8u * (kDotStages + s); };
   const uint32_t acc_bar = ctrl + 8u * (2 * kDotStages), part_bar = acc_bar + 8u;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_gen + T::kStages * T::kStageBytes + 8 * (2 * kDotStages + 2));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_gen + (ctrl - ring) + 8 * (2 * kDotStages + 2));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -132,10 +136,9 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
   const int m0 = (tile % p.tiles_m) * 128, n0 = (tile / p.tiles_m) * kN;
   const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * rank / splits);
   const int count = static_cast<int>(static_cast<long long>(p.num_kb) * (rank + 1) / splits) - kb0;
-  // this CTA's share of the tile, and where the partitions' parts of it arrive (behind the tile itself)
+  // this CTA's share of the tile
   const int rows = 128 / splits, r0 = rank * rows;
   const uint32_t share_bytes = static_cast<uint32_t>(rows) * T::kPitch * 4u;
-  const uint32_t parts = ring + 128u * T::kPitch * 4u;
 
   // k-block i of this partition into slot i % kStages
   const int rt = m0 / 128, ct = n0 / 128;
@@ -143,8 +146,8 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
     const int s = i % T::kStages;
     const uint32_t a = ring + s * T::kStageBytes, b = a + kCodesA, sa = b + T::kCodesB, sb = sa + T::kScales;
     const long long kb = kb0 + i;
-    // (A may have tiles of fewer rows: what the MMA then reads behind them ends in rows that are not stored. B's have
-    // as many as the tile has columns.)
+    // (A may have tiles of fewer rows: what the MMA then reads behind them ends in rows that are not stored. B's tiles have
+    // as many as this tile has columns.)
     mbar_expect_tx(full_bar(s), p.tile_a + T::kCodesB + 2 * T::kScales);
     bulk_load(a, p.ca + rt * p.pitch_a + kb * p.tile_a, p.tile_a, full_bar(s));
     bulk_load(sa, p.sa + rt * p.spitch + kb * T::kScales, T::kScales, full_bar(s));
@@ -174,6 +177,7 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (splits > 1) cluster_arrive();      // (this CTA's barriers exist)
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
 
@@ -215,12 +219,9 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
     }
     __syncwarp();
   }
-  if (warp < 2) {
-    if (splits > 1) cluster_arrive();
-  } else {
+  if (warp >= 2) {
     const bool done = mbar_wait(acc_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
     __syncwarp();
-    if (splits > 1) cluster_arrive();      // (with everybody's: all rings are idle, parts may arrive there)
     if (done && !*abort_flag) {
       tc_fence_after();
       const int group = warp & 3, half = (warp - 2) >> 2;
@@ -253,13 +254,12 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
   }
   __syncthreads();
   if (splits > 1) {
-    cluster_wait();
-    if (warp == 0 && elect_one()) {
-      for (int d = 1; d < splits; ++d) {
-        const int to = (rank + d) % splits;
-        bulk_push(map_to_cta(parts + rank * share_bytes, to), ring + to * share_bytes, share_bytes, map_to_cta(part_bar, to));
-      }
+    cluster_wait();          // (with everybody's arrival long ago: the barriers that the parts count on exist)
+    if (warp == 0 && lane > 0 && lane < splits) {
+      const int to = (rank + lane) % splits;
+      bulk_push(map_to_cta(parts + rank * share_bytes, to), ring + to * share_bytes, share_bytes, map_to_cta(part_bar, to));
     }
+    __syncwarp();
   }
   if (warp == 1) {
     tc_fence_after();
@@ -277,23 +277,26 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
   const bool whole = !p.swapped && p.vec_ok;        // rows of whole aligned vectors of C
   const int live = max(0, min(rows, p.M - m0 - r0));
   const float* own = reinterpret_cast<const float*>(ring_gen) + r0 * T::kPitch;
-  const float* others = reinterpret_cast<const float*>(ring_gen) + 128 * T::kPitch;
-  auto sum4 = [&](int off) {
-    float4 v = *reinterpret_cast<const float4*>((rank == 0 ? own : others) + off);
-    for (int s = 1; s < splits; ++s) {
-      const float4 x = *reinterpret_cast<const float4*>((s == rank ? own : others + s * rows * T::kPitch) + off);
-      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+  const float* others = reinterpret_cast<const float*>(ring_gen + (parts - ring));
+  auto part = [&](int s) { return s == rank ? own : others + s * rows * T::kPitch; };
+  auto sum4 = [&](auto n, int off) {
+    constexpr int kParts = decltype(n)::value;
+    float4 x[kParts];
+#pragma unroll
+    for (int s = 0; s < kParts; ++s) x[s] = *reinterpret_cast<const float4*>(part(s) + off);
+#pragma unroll
+    for (int s = 1; s < kParts; ++s) {
+      x[0].x += x[s].x; x[0].y += x[s].y; x[0].z += x[s].z; x[0].w += x[s].w;
     }
-    return v;
+    return x[0];
   };
-  if (*abort_flag) {
-  } else if (whole) {
+  auto store_whole = [&](auto n) {
     for (int i = threadIdx.x; i < live * (kN / 8); i += kDotThreads) {
       const int r = i / (kN / 8), c = (i % (kN / 8)) * 8;
       const int col = n0 + c;
       const long long row = m0 + r0 + r;
       if (col >= p.N) continue;
-      const float4 x = sum4(r * T::kPitch + c), y = sum4(r * T::kPitch + c + 4);
+      const float4 x = sum4(n, r * T::kPitch + c), y = sum4(n, r * T::kPitch + c + 4);
       float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
       const unsigned long long lin = static_cast<unsigned long long>(row) * p.N + col;
       const int nvalid = min(8, p.N - col);
@@ -301,34 +304,47 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
       if (p.out_f32) epi_store8<true>(p.ea, v, crow, crow, col, lin, nvalid, true);
       else epi_store8<false>(p.ea, v, crow, crow, col, lin, nvalid, true);
     }
-  } else {
-    // C's rows are at any address, or run down the tile: one output per lane and access
-    if (splits > 1) {
-      for (int i = threadIdx.x; i < live * (kN / 4); i += kDotThreads) {
-        const int off = i / (kN / 4) * T::kPitch + i % (kN / 4) * 4;
-        *reinterpret_cast<float4*>(const_cast<float*>(own) + off) = sum4(off);
-      }
-      __syncthreads();
+  };
+  auto sum_in_place = [&](auto n) {
+    for (int i = threadIdx.x; i < live * (kN / 4); i += kDotThreads) {
+      const int off = i / (kN / 4) * T::kPitch + i % (kN / 4) * 4;
+      *reinterpret_cast<float4*>(const_cast<float*>(own) + off) = sum4(n, off);
     }
+    __syncthreads();
+  };
+#define NG_BY_PARTS(call, from)                                                 \
+  switch (splits) {                                                             \
+    case 1: if (from <= 1) call(std::integral_constant<int, 1>()); break;       \
+    case 2: call(std::integral_constant<int, 2>()); break;                      \
+    case 4: call(std::integral_constant<int, 4>()); break;                      \
+    default: call(std::integral_constant<int, 8>()); break;                     \
+  }
+  if (*abort_flag) {
+  } else if (whole) {
+    NG_BY_PARTS(store_whole, 1)
+  } else {
+    // C's rows are at any address, or run down the tile: one output per lane and access, neighbours in lanes
+    NG_BY_PARTS(sum_in_place, 2)
     const int cols = min(kN, p.N - n0);
-    if (!p.swapped) {
-      for (int i = threadIdx.x; i < live * kN; i += kDotThreads) {
-        const int r = i / kN, c = i % kN;
-        const long long row = m0 + r0 + r;
-        if (c < cols)
-          epi_store1(p.ea, own[r * T::kPitch + c], static_cast<uint8_t*>(p.C) + (row * p.ldc + n0 + c) * (p.out_f32 ? 4 : 2), p.out_f32,
-                     static_cast<unsigned long long>(row) * p.N + n0 + c);
-      }
-    } else {
-      for (int i = threadIdx.x; i < cols * rows; i += kDotThreads) {
-        const int c = i / rows, r = i - c * rows;       // (a row and a column of C)
-        const long long row = n0 + c;
-        if (r < live)
-          epi_store1(p.ea, own[r * T::kPitch + c], static_cast<uint8_t*>(p.C) + (row * p.ldc + m0 + r0 + r) * (p.out_f32 ? 4 : 2), p.out_f32,
-                     static_cast<unsigned long long>(row) * p.M + m0 + r0 + r);
+    const int runs = p.swapped ? cols : live, len = p.swapped ? live : cols;       // rows of C that have some, and how many
+    const int run_step = p.swapped ? 1 : T::kPitch, step = p.swapped ? T::kPitch : 1;
+    const long long row0 = p.swapped ? n0 : m0 + r0, col0 = p.swapped ? m0 + r0 : n0;
+    const int width = p.swapped ? p.M : p.N;
+    const bool plain = p.ea.beta == 0.0f && p.ea.sr_bits == 0 && !p.out_f32;
+    for (int u = warp; u < runs; u += kDotThreads / 32) {
+      const long long row = row0 + u;
+      uint8_t* out = static_cast<uint8_t*>(p.C) + (row * p.ldc + col0) * (p.out_f32 ? 4 : 2);
+      const float* src = own + u * run_step;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = j * 32 + lane;
+        if (i >= len) break;
+        if (plain) reinterpret_cast<__half*>(out)[i] = f2h_rn(epi_scale(p.ea, src[i * step]));
+        else epi_store1(p.ea, src[i * step], out + i * (p.out_f32 ? 4 : 2), p.out_f32, static_cast<unsigned long long>(row) * width + col0 + i);
       }
     }
   }
+#undef NG_BY_PARTS
   __syncwarp();
   if (splits > 1) cluster_wait();
 }
@@ -360,6 +376,33 @@ int launch_dot(DeviceCtx* c, DotParams& p, int splits, cudaStream_t stream) {
   NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_kernel<kN, kNv>, p));
   NG_CHECK_LAUNCH();
   return NG_OK;
+}
+
+// CTAs that run at the same time in clusters of 2^log: larger ones leave SMs of their GPCs over (132 in clusters of 4, 120
+// in clusters of 8; 2048 x 128 x 2048 as 128 CTAs in clusters of 8 took two rounds, 12.0 us).
+int cluster_room(const DeviceCtx* c, int log) {
+  static std::atomic<int> known[64][4];
+  int n = known[c->device][log].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  using T = DotTile<128, true>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(c->sm_count >> log << log));
+  cfg.blockDim = dim3(kDotThreads);
+  cfg.dynamicSmemBytes = T::kSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1u << log;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaFuncSetAttribute(block_dot_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, block_dot_kernel<128, true>, &cfg) != cudaSuccess)
+    cudaGetLastError();
+  n = std::max(1, clusters << log);
+  known[c->device][log].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 int pad_columns(int n) { return n <= 64 ? block_tile_rows(n) : (n + 127) / 128 * 128; }
@@ -415,15 +458,26 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   p.ca = a.codes; p.cb = b.codes; p.pitch_a = a.pitch; p.pitch_b = b.pitch; p.tile_a = a.tile;
   p.sa = a.scales; p.sb = b.scales; p.spitch = a.spitch;
   p.status = c->status; p.wait_limit_ns = c->wait_limit_ns;
+  // Columns of a tile: B's rows padded, as its scales lie; a column of more has its tile in the middle of a scale tile, which
+  // tensor memory cannot address. Partitions of the sum, by what they take in us: per round of tiles, the k-blocks at 135
+  // bytes/ns and the output stage; when split, the exchange, at 30 bytes/ns of what each CTA gets.
   const int cols = p.N > 64 ? 128 : pad_columns(p.N);
   const long long tiles = static_cast<long long>(p.tiles_m) * ((p.N + cols - 1) / cols);
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= c->sm_count && p.num_kb >= splits * 2) splits *= 2;
+  double here = 0.0;
+  for (int s = 1, log = 0; s <= 8 && (s == 1 || (p.num_kb >= s && tiles * s <= cluster_room(c, log))); s *= 2, ++log) {
+    const double kb = (20480.0 + 128.0 * cols) * 7.4e-6, out = 0.5 + cols / 128.0;
+    const double us = 4.5 + (tiles * s + c->sm_count - 1) / c->sm_count * (kb * ((p.num_kb + s - 1) / s) + out / s) +
+                      (s > 1 ? 1.0 + 512.0 * cols * (s - 1) / s * 3.3e-5 : 0.0);
+    if (s == 1 || us < here) {
+      here = us;
+      splits = s;
+    }
+  }
   // Or pairs of SMs on tiles of 256 x 256 (block_dot_pair.cu), by the sum of what both take in us: a start, and per round
   // of tiles its k-blocks and its output stage. Here / pairs, nvfp4: 8192^3 235 / 162, 4096^3 49 / 34, 2048^3 13.9 / 9.8,
   // 8192 x 512 x 8192 25.0 / 18.4, 1000^3 6.9 / 7.0, 1536 x 1536 x 4096 9.2 / 11.9, 4096 x 128 x 9216 10.4 / 16.4.
   const long long pair_tiles = ((m + 255ll) / 256) * ((n + 255ll) / 256);
-  const double here = 4.5 + (tiles + c->sm_count - 1) / c->sm_count * (0.25 * p.num_kb / splits + 1.5) + (splits > 1 ? 2.0 : 0.0);
   const double pairs = 5.5 + (pair_tiles + c->sm_count / 2 - 1) / (c->sm_count / 2) * (0.33 * p.num_kb + 0.7);
   if (m > 64 && n > 64 && pairs < here) {
     if (p.swapped) std::swap(a, b);
