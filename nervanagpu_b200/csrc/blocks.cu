@@ -464,34 +464,35 @@ __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(Block
   }
 }
 
-// (codes are read block by block: the four warps of a CTA find each other's neighbours in the L1 cache)
+// (units of 16 numbers: with whole blocks of 32 per thread a minibatch of 9216 x 128 had too few warps, 3.0 us. Codes are
+// read unit by unit: the warps of a CTA find each other's neighbours in the L1 cache.)
 template <typename T, int kFmt, bool kVec>
-__global__ void __launch_bounds__(kStridedThreads) dequantize_strided_kernel(BlockView q, PlainView<T> a, int early, int blocks) {
+__global__ void __launch_bounds__(kStridedThreads) dequantize_strided_kernel(BlockView q, PlainView<T> a, int early, int units) {
   NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
-  using S = StridedTile<kFmt>;
   using P = Pair<T>;
+  constexpr int kWords = F::k4 ? 2 : 4;            // of 16 codes
   const int o0 = blockIdx.x * kStridedRows;
   const int r[2] = {o0 + strided_row<kVec>(0), o0 + strided_row<kVec>(1)};
-  for (int b = blockIdx.y * 4 + (threadIdx.x >> 5); b < blocks; b += gridDim.y * 4) {
-    const int n = q.inner - b * F::kBlock;
-    uint32_t w[2][S::kBytes / 4];
+  for (int b = blockIdx.y * 4 + (threadIdx.x >> 5); b < units; b += gridDim.y * 4) {
+    const int n = q.inner - b * 16;
+    uint32_t w[2][kWords];
     float scale[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
-      for (int i = 0; i < S::kBytes / 8; ++i) {
+      for (int i = 0; i < kWords / 2; ++i) {
         uint2 c = make_uint2(0u, 0u);
-        if (r[j] < q.outer) c = *reinterpret_cast<const uint2*>(q.codes + F::code_at(q, r[j], static_cast<long long>(b) * S::kBytes + 8 * i));
+        if (r[j] < q.outer) c = *reinterpret_cast<const uint2*>(q.codes + F::code_at(q, r[j], b * (4ll * kWords) + 8 * i));
         w[j][2 * i] = c.x;
         w[j][2 * i + 1] = c.y;
       }
-      scale[j] = block_scale_value<kFmt>(r[j] < q.outer ? q.scales[F::scale_at(q, r[j], b)] : 0u, q.t);
+      scale[j] = block_scale_value<kFmt>(r[j] < q.outer ? q.scales[F::scale_at(q, r[j], b / (F::kBlock / 16))] : 0u, q.t);
     }
-    T* p = a.p + static_cast<long long>(b) * F::kBlock * a.sl;
+    T* p = a.p + b * 16ll * a.sl;
     T *p0 = p + r[0] * a.so, *p1 = p + r[1] * a.so;
 #pragma unroll
-    for (int h = 0; h < F::kBlock / 8; ++h) {
+    for (int h = 0; h < 2; ++h) {
       T v[2][8];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -564,16 +565,16 @@ int launch(const DeviceCtx* c, void (*kernel)(P...), dim3 grid, dim3 block, cuda
   return NG_OK;
 }
 // Lanes per row: its groups of 16 numbers, rounded up to 8 (four blocks of 32, whose scales leave together), over
-// CTAs of 256 threads with as few idle lanes as a power of two allows; the other threads take other rows.
-RowGrid row_grid(const DeviceCtx* c, const BlockView& q) {
+// CTAs of so many threads with as few idle lanes as a power of two allows; the other threads take other rows.
+RowGrid row_grid(const DeviceCtx* c, const BlockView& q, int threads) {
   const int groups = static_cast<int>((q.inner + 127ll) / 128 * 8);
-  int tx = 256;
+  int tx = threads;
   while (tx > 8 && (groups + tx / 2 - 1) / (tx / 2) * (tx / 2) < (groups + tx - 1) / tx * tx) tx /= 2;
-  const int ty = 256 / tx;
+  const int ty = threads / tx;
   RowGrid r;
   r.block = dim3(tx, ty);
   const long long gx = (groups + tx - 1) / tx, rows = (static_cast<long long>(q.outer) + ty - 1) / ty;
-  const long long room = std::max(1ll, 16ll * c->sm_count / gx);
+  const long long room = std::max(1ll, 4096ll / threads * c->sm_count / gx);
   r.grid = dim3(static_cast<unsigned>(gx), static_cast<unsigned>(std::min(std::min(rows, room), 65535ll)));
   return r;
 }
@@ -601,7 +602,7 @@ int quantize_one(DeviceCtx* c, const BlockView& q, PlainView<const T> a, cudaStr
   const int blocks = (q.inner + BlockFormat<kFmt>::kBlock - 1) / BlockFormat<kFmt>::kBlock;
   int rc;
   if (a.sl == 1) {
-    const RowGrid g = row_grid(c, q);
+    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128);
     a.wide = aligned_rows(a, 32);
     if (aligned_rows(a, 16)) rc = launch(c, quantize_rows_kernel<T, kFmt, true>, g.grid, g.block, stream, q, a);
     else rc = launch(c, quantize_rows_kernel<T, kFmt, false>, g.grid, g.block, stream, q, a);
@@ -615,17 +616,17 @@ int quantize_one(DeviceCtx* c, const BlockView& q, PlainView<const T> a, cudaStr
 
 template <typename T, int kFmt>
 int dequantize_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_t stream) {
-  const int blocks = (q.inner + BlockFormat<kFmt>::kBlock - 1) / BlockFormat<kFmt>::kBlock;
+  const int units = (q.inner + 15) / 16;
   int rc;
   if (a.sl == 1) {
-    const RowGrid g = row_grid(c, q);
+    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128);
     a.wide = aligned_rows(a, 32);
     if (aligned_rows(a, 16)) rc = launch(c, dequantize_rows_kernel<T, kFmt, true>, g.grid, g.block, stream, q, a);
     else rc = launch(c, dequantize_rows_kernel<T, kFmt, false>, g.grid, g.block, stream, q, a);
   } else {
-    const dim3 grid((q.outer + kStridedRows - 1) / kStridedRows, std::min((blocks + 3) / 4, 65535));
-    if (aligned_pairs(q, a)) rc = launch(c, dequantize_strided_kernel<T, kFmt, true>, grid, dim3(kStridedThreads), stream, q, a, blocks);
-    else rc = launch(c, dequantize_strided_kernel<T, kFmt, false>, grid, dim3(kStridedThreads), stream, q, a, blocks);
+    const dim3 grid((q.outer + kStridedRows - 1) / kStridedRows, std::min((units + 3) / 4, 65535));
+    if (aligned_pairs(q, a)) rc = launch(c, dequantize_strided_kernel<T, kFmt, true>, grid, dim3(kStridedThreads), stream, q, a, units);
+    else rc = launch(c, dequantize_strided_kernel<T, kFmt, false>, grid, dim3(kStridedThreads), stream, q, a, units);
   }
   return rc;
 }
@@ -635,7 +636,7 @@ int relu_mask_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_t
   const int blocks = (q.inner + 31) / 32;
   int rc;
   if (a.sl == 1) {
-    const RowGrid g = row_grid(c, q);
+    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128);
     a.wide = aligned_rows(a, 32);
     if (aligned_rows(a, 16)) rc = launch(c, relu_mask_rows_kernel<T, true>, g.grid, g.block, stream, q, a);
     else rc = launch(c, relu_mask_rows_kernel<T, false>, g.grid, g.block, stream, q, a);
