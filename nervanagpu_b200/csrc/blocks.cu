@@ -33,13 +33,13 @@ __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_
   grid_dependency_wait();            \
   if (early) grid_launch_dependents()
 
-// ---- rows form: 16 numbers per lane ------------------------------------------------------------------
+// ---- rows form: 16 numbers per lane, or 32 ------------------------------------------------------------------
 constexpr int kLane = 16;
 
-// 16 neighbours as they lie in memory
-template <typename T>
+// kCount neighbours as they lie in memory
+template <typename T, int kCount = kLane>
 struct Raw {
-  static constexpr int kVecs = kLane * sizeof(T) / 16;
+  static constexpr int kVecs = kCount * sizeof(T) / 16;
   uint4 v[kVecs];
   __device__ __forceinline__ T* at() { return reinterpret_cast<T*>(v); }
   __device__ __forceinline__ const T* at() const { return reinterpret_cast<const T*>(v); }
@@ -47,45 +47,46 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
   }
-  // The first n of 16 numbers at a 16-byte aligned address. wide: the rows are 32-byte aligned, and whole sectors
+  // The first n of them at a 16-byte aligned address. wide: the rows are 32-byte aligned, and whole sectors
   // are moved at a time (by halves, the two accesses of a warp each touched every sector).
   __device__ __forceinline__ void load(const T* p, int n, bool wide) {
-    if (n >= kLane && wide) {
+    if (n >= kCount && wide) {
 #pragma unroll
       for (int i = 0; i < kVecs; i += 2)
         asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w), "=r"(v[i + 1].x), "=r"(v[i + 1].y),
                        "=r"(v[i + 1].z), "=r"(v[i + 1].w)
                      : "l"(reinterpret_cast<const uint4*>(p) + i));
-    } else if (n >= kLane) {
+    } else if (n >= kCount) {
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) at()[i] = i < n ? p[i] : T(0.0f);
+      for (int i = 0; i < kCount; ++i) at()[i] = i < n ? p[i] : T(0.0f);
     }
   }
   __device__ __forceinline__ void store(T* p, int n, bool wide) const {
-    if (n >= kLane && wide) {
+    if (n >= kCount && wide) {
 #pragma unroll
       for (int i = 0; i < kVecs; i += 2)
         asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint4*>(p) + i),
                      "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w), "r"(v[i + 1].x), "r"(v[i + 1].y), "r"(v[i + 1].z),
                      "r"(v[i + 1].w)
                      : "memory");
-    } else if (n >= kLane) {
+    } else if (n >= kCount) {
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < kLane; ++i)
+      for (int i = 0; i < kCount; ++i)
         if (i < n) p[i] = at()[i];
     }
   }
 };
 
 // the h-th 8 of them in fp32
-__device__ __forceinline__ void to_f32x8(const Raw<__half>& r, int h, float (&x)[8]) {
+template <int kCount>
+__device__ __forceinline__ void to_f32x8(const Raw<__half, kCount>& r, int h, float (&x)[8]) {
   const uint32_t w[4] = {r.v[h].x, r.v[h].y, r.v[h].z, r.v[h].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -94,7 +95,8 @@ __device__ __forceinline__ void to_f32x8(const Raw<__half>& r, int h, float (&x)
     x[2 * i + 1] = f.y;
   }
 }
-__device__ __forceinline__ void to_f32x8(const Raw<float>& r, int h, float (&x)[8]) {
+template <int kCount>
+__device__ __forceinline__ void to_f32x8(const Raw<float, kCount>& r, int h, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint4 w = r.v[2 * h + i];
@@ -103,35 +105,38 @@ __device__ __forceinline__ void to_f32x8(const Raw<float>& r, int h, float (&x)[
   }
 }
 
-// Largest magnitude, as the bits of an fp32 number (above those of infinity for a NaN).
-__device__ __forceinline__ uint32_t top_bits(const Raw<__half>& r) {
-  uint32_t top = 0u;
+// Largest magnitude of numbers 8 h0 .. 8 h1 - 1, as the bits of an fp32 number (above those of infinity for a NaN).
+template <int kCount>
+__device__ __forceinline__ uint32_t top_bits(const Raw<__half, kCount>& r, int h0, int h1) {
+  __half2 top = __half2half2(__ushort_as_half(0));
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t w[4] = {r.v[i].x, r.v[i].y, r.v[i].z, r.v[i].w};
+  for (int h = h0; h < h1; ++h) {
+    const uint32_t w[4] = {r.v[h].x, r.v[h].y, r.v[h].z, r.v[h].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
+    for (int j = 0; j < 4; ++j) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&w[j])));
   }
-  const uint16_t bits = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
-  return magnitude_bits(__half2float(__ushort_as_half(bits)));
+  return magnitude_bits(__half2float(__hmax_nan(__low2half(top), __high2half(top))));
 }
-__device__ __forceinline__ uint32_t top_bits(const Raw<float>& r) {
+template <int kCount>
+__device__ __forceinline__ uint32_t top_bits(const Raw<float, kCount>& r, int h0, int h1) {
   uint32_t top = 0u;
 #pragma unroll
-  for (int i = 0; i < kLane; ++i) top = max(top, magnitude_bits(r.at()[i]));
+  for (int i = 2 * h0; i < 2 * h1; ++i)
+    top = max(max(top, r.v[i].x & 0x7fffffffu), max(r.v[i].y & 0x7fffffffu, max(r.v[i].z & 0x7fffffffu, r.v[i].w & 0x7fffffffu)));
   return top;
 }
 
-// Rows at addresses that are no multiples of 16 bytes: the warp moves its 512 numbers (a run of 16 << log_tx of each
-// of its rows, at least 128) in order, one number per lane and access, through shared memory. (A lane that moved its
+// Rows at addresses that are no multiples of 16 bytes: the warp moves its 32 kCount numbers (a run of kCount <<
+// log_tx of each of its rows, at least 128) in order, one number per lane and access, through shared memory. (A lane that moved its
 // own 16 one by one touched 32 sectors per access: 139968 x 125 fp16 read back from 8 bits took 51 us.)
-template <typename T, bool kStore>
+template <typename T, bool kStore, int kCount>
 __device__ __forceinline__ void warp_move(T* base, long long so, long long o_first, int outer, int l_first, int inner, int log_tx, T* stage) {
   const int lane = threadIdx.x + threadIdx.y * blockDim.x & 31;
+  const int per_row = log_tx + (kCount == 32 ? 5 : 4) - 7;      // logarithm: pieces of 128 in a row
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long o = o_first + (i >> (log_tx - 3));
-    const int l = l_first + (i & ((1 << (log_tx - 3)) - 1)) * 128 + lane;
+  for (int i = 0; i < kCount / 4; ++i) {
+    const long long o = o_first + (i >> per_row);
+    const int l = l_first + (i & ((1 << per_row) - 1)) * 128 + lane;
     T* p = base + o * so + l;
     T* s = stage + i * 128 + lane;
     const int n = o < outer ? inner - l : 0;
@@ -145,53 +150,67 @@ __device__ __forceinline__ void warp_move(T* base, long long so, long long o_fir
     }
   }
 }
-template <typename T>
+template <typename T, int kCount>
 __device__ __forceinline__ void warp_load(const T* base, long long so, long long o_first, int outer, int l_first, int inner, int log_tx,
-                                          T* stage, Raw<T>& r) {
+                                          T* stage, Raw<T, kCount>& r) {
   const int lane = threadIdx.x + threadIdx.y * blockDim.x & 31;
-  warp_move<T, false>(const_cast<T*>(base), so, o_first, outer, l_first, inner, log_tx, stage);
+  warp_move<T, false, kCount>(const_cast<T*>(base), so, o_first, outer, l_first, inner, log_tx, stage);
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < Raw<T>::kVecs; ++i) r.v[i] = reinterpret_cast<const uint4*>(stage + lane * kLane)[i];
+  for (int i = 0; i < Raw<T, kCount>::kVecs; ++i) r.v[i] = reinterpret_cast<const uint4*>(stage + lane * kCount)[i];
   __syncwarp();
 }
-template <typename T>
+template <typename T, int kCount>
 __device__ __forceinline__ void warp_store(T* base, long long so, long long o_first, int outer, int l_first, int inner, int log_tx,
-                                           T* stage, const Raw<T>& r) {
+                                           T* stage, const Raw<T, kCount>& r) {
   const int lane = threadIdx.x + threadIdx.y * blockDim.x & 31;
 #pragma unroll
-  for (int i = 0; i < Raw<T>::kVecs; ++i) reinterpret_cast<uint4*>(stage + lane * kLane)[i] = r.v[i];
+  for (int i = 0; i < Raw<T, kCount>::kVecs; ++i) reinterpret_cast<uint4*>(stage + lane * kCount)[i] = r.v[i];
   __syncwarp();
-  warp_move<T, true>(base, so, o_first, outer, l_first, inner, log_tx, stage);
+  warp_move<T, true, kCount>(base, so, o_first, outer, l_first, inner, log_tx, stage);
   __syncwarp();
 }
 
 // One step of a rows kernel: this thread's row, and the warp's first row and first group (warp_load).
-#define NG_ROWS_PROLOGUE(T)                                                                             \
-  __shared__ __align__(16) T stage_all[kVec ? 1 : 256 * kLane];                                         \
+// (Rows that are moved through shared memory have CTAs of 128 threads.)
+#define NG_ROWS_PROLOGUE(T, count)                                                                      \
+  __shared__ __align__(16) T stage_all[kVec ? 1 : 128 * count];                                         \
   const int tid = threadIdx.x + threadIdx.y * blockDim.x;                                               \
-  T* stage = kVec ? stage_all : stage_all + (tid & ~31) * kLane;                                        \
+  T* stage = kVec ? stage_all : stage_all + (tid & ~31) * count;                                        \
   const int log_tx = min(31 - __clz(blockDim.x), 5);      /* lanes of one warp in a row */              \
-  const int g = blockIdx.x * blockDim.x + threadIdx.x, n = q.inner - g * kLane;                         \
-  const int l_warp = (g - (tid & 31 & (static_cast<int>(blockDim.x) - 1))) * kLane;                     \
+  const int g = blockIdx.x * blockDim.x + threadIdx.x, n = q.inner - g * count;                         \
+  const int l_warp = (g - (tid & 31 & (static_cast<int>(blockDim.x) - 1))) * count;                     \
   const int y_warp = (tid & ~31) / static_cast<int>(blockDim.x);                                        \
   const long long step = static_cast<long long>(gridDim.y) * blockDim.y
+
+// Numbers per lane in a quantisation: 32 from fp16 to 4 bits, where what a block and a row cost besides, some 50
+// instructions, counted more than the numbers themselves with 16 (4096 x 9216 nvfp4 18.1 -> 16.1 us); with the wider
+// codes or numbers they take too many registers (1001 x 4097 fp32 8.3 -> 9.4, 139968 x 125 mxfp8 15.0 -> 16.3).
+template <typename T, int kFmt>
+__host__ __device__ constexpr int quantize_lane() {
+  return BlockFormat<kFmt>::k4 && sizeof(T) == 2 ? 32 : 16;
+}
 
 template <typename T, int kFmt, bool kVec>
 __global__ void __launch_bounds__(256, !kVec && sizeof(T) == 4 ? 6 : 4) quantize_rows_kernel(BlockView q, PlainView<const T> a, int early) {
   NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
-  NG_ROWS_PROLOGUE(T);
-  constexpr int kUnroll = kVec ? 2 : 1;       // rows whose loads are in flight together
+  constexpr int kPer = quantize_lane<T, kFmt>();
+  NG_ROWS_PROLOGUE(T, kPer);
+  constexpr int kUnroll = kVec ? 2 : 1;                             // rows whose loads are in flight together
+  constexpr int kBlocks = kPer > F::kBlock ? kPer / F::kBlock : 1;  // of a lane
+  constexpr int kDup = kPer < F::kBlock ? 2 : 1;                    // lanes that share one
+  constexpr int kSharers = 4 / kBlocks;                             // lanes whose scales make a word, the sharing ones once
+  constexpr int kEights = kPer / 8 / kBlocks;
   // (whole warps stay to the end of the loop: lanes exchange magnitudes and scales)
   for (long long o0 = static_cast<long long>(blockIdx.y) * blockDim.y; o0 < q.outer; o0 += kUnroll * step) {
-    Raw<T> raw[kUnroll];
+    Raw<T, kPer> raw[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const long long o = o0 + u * step + threadIdx.y;
       if (kVec) {
         raw[u].clear();
-        if (o < q.outer && n > 0) raw[u].load(a.p + o * a.so + static_cast<long long>(g) * kLane, n, a.wide);
+        if (o < q.outer && n > 0) raw[u].load(a.p + o * a.so + static_cast<long long>(g) * kPer, n, a.wide);
       } else {
         warp_load(a.p, a.so, o0 + u * step + y_warp, q.outer, l_warp, q.inner, log_tx, stage, raw[u]);
       }
@@ -200,38 +219,48 @@ __global__ void __launch_bounds__(256, !kVec && sizeof(T) == 4 ? 6 : 4) quantize
     for (int u = 0; u < kUnroll; ++u) {
       const long long o = o0 + u * step + threadIdx.y;
       const bool live = o < q.outer && n > 0;
-      uint32_t top = top_bits(raw[u]);
-      if (!F::kNv) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      const BlockScale s = block_scale<kFmt, sizeof(T) == 2>(top, q.t);
-      uint2 c[2];
-      // (by up to 2^30 is two fp16 factors; a block of zeros needs none)
-      if (!F::k4 && sizeof(T) == 2 && !s.nan && (s.by <= 1073741824.0f || top == 0u)) {
-        __half2 by0, by1;
-        block_scale_f16(s.by, by0, by1);
+      uint2 c[kPer / 8];
+      uint32_t word = 0u;           // this lane's scales
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          c[h].x = block_encode4_f16(raw[u].v[h].x, raw[u].v[h].y, by0, by1);
-          c[h].y = block_encode4_f16(raw[u].v[h].z, raw[u].v[h].w, by0, by1);
+      for (int b = 0; b < kBlocks; ++b) {
+        uint32_t top = top_bits(raw[u], b * kEights, (b + 1) * kEights);
+        if (kDup == 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        const BlockScale s = block_scale<kFmt, sizeof(T) == 2>(top, q.t);
+        if (live && b * F::kBlock < n) word |= s.byte << (8 * b);
+        bool done = false;
+        if constexpr (!F::k4 && sizeof(T) == 2) {
+          // (by up to 2^30 is two fp16 factors; a block of zeros needs none)
+          if (!s.nan && (s.by <= 1073741824.0f || top == 0u)) {
+            done = true;
+            __half2 by0, by1;
+            block_scale_f16(s.by, by0, by1);
+#pragma unroll
+            for (int h = 0; h < kEights; ++h) {
+              c[h].x = block_encode4_f16(raw[u].v[h].x, raw[u].v[h].y, by0, by1);
+              c[h].y = block_encode4_f16(raw[u].v[h].z, raw[u].v[h].w, by0, by1);
+            }
+          }
         }
-      } else {
+        if (!done) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x[8];
-          to_f32x8(raw[u], h, x);
-          c[h] = block_encode8<kFmt, sizeof(T) == 2>(x, s);
+          for (int h = b * kEights; h < (b + 1) * kEights; ++h) {
+            float x[8];
+            to_f32x8(raw[u], h, x);
+            c[h] = block_encode8<kFmt, sizeof(T) == 2>(x, s);
+          }
         }
       }
-      // the scales of four blocks leave together: four lanes, or eight that hold each twice
-      constexpr int kShare = F::kNv ? 1 : 2;
-      uint32_t word = live ? s.byte << (8 * (g / kShare % 4)) : 0u;
-      word |= __shfl_xor_sync(0xffffffffu, word, kShare);
-      word |= __shfl_xor_sync(0xffffffffu, word, 2 * kShare);
+      // the scales of four blocks leave together
+      word <<= 8 * kBlocks * (g / kDup % kSharers);
+#pragma unroll
+      for (int d = 1; d < kSharers; d *= 2) word |= __shfl_xor_sync(0xffffffffu, word, d * kDup);
       if (live) {
-        uint8_t* dst = q.codes + F::code_at(q, static_cast<int>(o), static_cast<long long>(g) * (2 * F::kBytes8));
-        if (F::k4) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0].x, c[1].x);
-        else *reinterpret_cast<uint4*>(dst) = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
-        if (g % (4 * kShare) == 0)
-          *reinterpret_cast<uint32_t*>(q.scales + F::scale_at(q, static_cast<int>(o), g / kShare)) = word;
+        uint8_t* dst = q.codes + F::code_at(q, static_cast<int>(o), g * (kPer / 8ll * F::kBytes8));
+        if (!F::k4) *reinterpret_cast<uint4*>(dst) = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
+        else if (kPer == 32) *reinterpret_cast<uint4*>(dst) = make_uint4(c[0].x, c[1].x, c[kPer / 8 - 2].x, c[kPer / 8 - 1].x);
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(c[0].x, c[1].x);
+        if (g % (kSharers * kDup) == 0)
+          *reinterpret_cast<uint32_t*>(q.scales + F::scale_at(q, static_cast<int>(o), g / kDup * kBlocks)) = word;
       }
     }
   }
@@ -241,7 +270,7 @@ template <typename T, int kFmt, bool kVec>
 __global__ void __launch_bounds__(256) dequantize_rows_kernel(BlockView q, PlainView<T> a, int early) {
   NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
-  NG_ROWS_PROLOGUE(T);
+  NG_ROWS_PROLOGUE(T, kLane);
   constexpr int kShare = F::kNv ? 1 : 2;
   constexpr int kUnroll = kVec ? 2 : 1;
   for (long long o0 = static_cast<long long>(blockIdx.y) * blockDim.y; o0 < q.outer; o0 += kUnroll * step) {
@@ -564,12 +593,12 @@ int launch(const DeviceCtx* c, void (*kernel)(P...), dim3 grid, dim3 block, cuda
   NG_CHECK_LAUNCH();
   return NG_OK;
 }
-// Lanes per row: its groups of 16 numbers, rounded up to 8 (four blocks of 32, whose scales leave together), over
+// Lanes per row: its groups of `count` numbers, rounded up to 128 of these (four blocks, whose scales leave together), over
 // CTAs of so many threads with as few idle lanes as a power of two allows; the other threads take other rows.
-RowGrid row_grid(const DeviceCtx* c, const BlockView& q, int threads) {
-  const int groups = static_cast<int>((q.inner + 127ll) / 128 * 8);
+RowGrid row_grid(const DeviceCtx* c, const BlockView& q, int threads, int count) {
+  const int groups = static_cast<int>((q.inner + 127ll) / 128 * (128 / count));
   int tx = threads;
-  while (tx > 8 && (groups + tx / 2 - 1) / (tx / 2) * (tx / 2) < (groups + tx - 1) / tx * tx) tx /= 2;
+  while (tx > 128 / count && (groups + tx / 2 - 1) / (tx / 2) * (tx / 2) < (groups + tx - 1) / tx * tx) tx /= 2;
   const int ty = threads / tx;
   RowGrid r;
   r.block = dim3(tx, ty);
@@ -602,7 +631,7 @@ int quantize_one(DeviceCtx* c, const BlockView& q, PlainView<const T> a, cudaStr
   const int blocks = (q.inner + BlockFormat<kFmt>::kBlock - 1) / BlockFormat<kFmt>::kBlock;
   int rc;
   if (a.sl == 1) {
-    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128);
+    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128, quantize_lane<T, kFmt>());
     a.wide = aligned_rows(a, 32);
     if (aligned_rows(a, 16)) rc = launch(c, quantize_rows_kernel<T, kFmt, true>, g.grid, g.block, stream, q, a);
     else rc = launch(c, quantize_rows_kernel<T, kFmt, false>, g.grid, g.block, stream, q, a);
@@ -619,7 +648,7 @@ int dequantize_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_
   const int units = (q.inner + 15) / 16;
   int rc;
   if (a.sl == 1) {
-    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128);
+    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128, kLane);
     a.wide = aligned_rows(a, 32);
     if (aligned_rows(a, 16)) rc = launch(c, dequantize_rows_kernel<T, kFmt, true>, g.grid, g.block, stream, q, a);
     else rc = launch(c, dequantize_rows_kernel<T, kFmt, false>, g.grid, g.block, stream, q, a);
@@ -636,7 +665,7 @@ int relu_mask_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_t
   const int blocks = (q.inner + 31) / 32;
   int rc;
   if (a.sl == 1) {
-    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128);
+    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128, kLane);
     a.wide = aligned_rows(a, 32);
     if (aligned_rows(a, 16)) rc = launch(c, relu_mask_rows_kernel<T, true>, g.grid, g.block, stream, q, a);
     else rc = launch(c, relu_mask_rows_kernel<T, false>, g.grid, g.block, stream, q, a);

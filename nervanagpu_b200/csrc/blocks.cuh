@@ -189,8 +189,10 @@ __device__ __forceinline__ uint32_t block_encode4_f16(uint32_t x0, uint32_t x1, 
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const __half2 v = *reinterpret_cast<const __half2*>(&x[i]);
-    const __half2 m = __hmax2(__habs2(__hmul2(__hmul2(v, by0), by1)), __half2half2(__ushort_as_half(0x1800)));   // 2^-9
-    const uint32_t y = (*reinterpret_cast<const uint32_t*>(&m) | (x[i] & 0x80008000u)) & __hne2_mask(v, __half2half2(__ushort_as_half(0)));
+    // (the least is 2^-9 for a number that is not zero: 2^15 times any such is no less)
+    const __half2 least = __hmin2(__habs2(__hmul2(v, __half2half2(__ushort_as_half(0x7800)))), __half2half2(__ushort_as_half(0x1800)));
+    const __half2 m = __hmax2(__habs2(__hmul2(__hmul2(v, by0), by1)), least);
+    const uint32_t y = *reinterpret_cast<const uint32_t*>(&m) | (x[i] & 0x80008000u);
     uint16_t c;
     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(y));
     r[i] = c;
