@@ -203,6 +203,19 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
       uint32_t word = j < p.N ? *reinterpret_cast<const uint32_t*>(scales) : 0u;
       for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
         const int s = it % T::kStages, x = it % kMixRaw;
+        // A, when TMA cannot: 16 rows per warp, two numbers per lane and row, on their way while this waits
+        constexpr int kRows = 128 / kMixConv;
+        __half2 from_a[kRows];
+        const int a_row = (warp - 2 - kMixEpi) * kRows;
+        if (!p.a_tma) {
+          const int k0 = kb * 64 + lane;
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) {
+            const __half* row = p.A + static_cast<long long>(m0 + a_row + i) * p.lda + k0;
+            const bool row_ok = m0 + a_row + i < p.M;
+            from_a[i] = __halves2half2(row_ok && k0 < p.K ? row[0] : __half(0.0f), row_ok && k0 + 32 < p.K ? row[32] : __half(0.0f));
+          }
+        }
         ok = mbar_wait(rawf_bar(x), (it / kMixRaw) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns) &&
              (it < T::kStages || mbar_wait(empty_bar(s), (it / T::kStages - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns));
         if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
@@ -246,18 +259,13 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
         if (lane == 0) mbar_arrive(rawe_bar(x));
         if ((kb & 1) && kb + 1 < p.num_kb && j < p.N) word = *reinterpret_cast<const uint32_t*>(scales + (kb + 1) * 2ll);
         if (!p.a_tma) {
-          // 16 rows of A per warp, two numbers per lane and row
-          const int cw = warp - 2 - kMixEpi, k0 = kb * 64 + lane;
-          uint8_t* a = ring_gen + s * T::kSlot;
+          uint8_t* a = ring_gen + s * T::kSlot + a_row * 128 + ((lane * 2) & 15);
+          const int at = (lane * 2) & 112;
 #pragma unroll
-          for (int i = 0; i < 128 / kMixConv; ++i) {
-            const int ar = cw * (128 / kMixConv) + i;
-            const __half* src = p.A + static_cast<long long>(m0 + ar) * p.lda + k0;
-            const bool row_ok = m0 + ar < p.M;
-            const __half lo = row_ok && k0 < p.K ? src[0] : __half(0.0f), hi = row_ok && k0 + 32 < p.K ? src[32] : __half(0.0f);
-            const int at = lane * 2, sw = (ar & 7) << 4;
-            *reinterpret_cast<__half*>(a + ar * 128 + ((at & 112) ^ sw) + (at & 15)) = lo;
-            *reinterpret_cast<__half*>(a + ar * 128 + (((at + 64) & 112) ^ sw) + (at & 15)) = hi;
+          for (int i = 0; i < kRows; ++i) {
+            const int sw = (i & 7) << 4;         // (a_row is a multiple of 8)
+            *reinterpret_cast<__half*>(a + i * 128 + (at ^ sw)) = __low2half(from_a[i]);
+            *reinterpret_cast<__half*>(a + i * 128 + ((at + 64) ^ sw)) = __high2half(from_a[i]);
           }
         }
         fence_async_smem();

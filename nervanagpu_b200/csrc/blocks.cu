@@ -404,11 +404,11 @@ struct Pair<float> {
 // Largest magnitudes of both rows, as the bits of fp32 numbers.
 template <int kN>
 __device__ __forceinline__ void top_of_pairs(const uint32_t (&raw)[kN], uint32_t (&top)[2]) {
-  uint32_t t = 0u;
+  __half2 t = __half2half2(__ushort_as_half(0));
 #pragma unroll
-  for (int i = 0; i < kN; ++i) t = __vmaxu2(t, raw[i] & 0x7fff7fffu);
-  top[0] = magnitude_bits(Pair<__half>::get(t, 0));
-  top[1] = magnitude_bits(Pair<__half>::get(t, 1));
+  for (int i = 0; i < kN; ++i) t = __hmax2_nan(t, __habs2(*reinterpret_cast<const __half2*>(&raw[i])));
+  top[0] = magnitude_bits(__low2float(t));
+  top[1] = magnitude_bits(__high2float(t));
 }
 template <int kN>
 __device__ __forceinline__ void top_of_pairs(const uint2 (&raw)[kN], uint32_t (&top)[2]) {
@@ -443,11 +443,16 @@ __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(Block
     const T* p = a.p + static_cast<long long>(b) * F::kBlock * a.sl;
     const int r0 = o0 + strided_row<kVec>(0), r1 = o0 + strided_row<kVec>(1);
     if (kVec) {
-      const bool live = r0 < q.outer;
+      const T* p0 = p + r0;
+      if (r0 < q.outer && n >= F::kBlock) {
 #pragma unroll
-      for (int i = 0; i < F::kBlock; ++i) {
-        raw[i] = P::of(T(0.0f), T(0.0f));
-        if (live && i < n) raw[i] = *reinterpret_cast<const typename P::Vec*>(p + r0 + i * a.sl);
+        for (int i = 0; i < F::kBlock; ++i) raw[i] = *reinterpret_cast<const typename P::Vec*>(p0 + i * a.sl);
+      } else {
+#pragma unroll
+        for (int i = 0; i < F::kBlock; ++i) {
+          raw[i] = P::of(T(0.0f), T(0.0f));
+          if (r0 < q.outer && i < n) raw[i] = *reinterpret_cast<const typename P::Vec*>(p0 + i * a.sl);
+        }
       }
     } else {
       const T *p0 = p + r0 * a.so, *p1 = p + r1 * a.so;
