@@ -232,7 +232,7 @@ int ng_pool_bprop_argmax(const ng_pool_desc* desc, int dtype_bytes, const void* 
  * scale. Formats:
  *   NG_BLOCK_MXFP4  4-bit numbers (E2M1, up to 6), blocks of 32, scale a power of two (E8M0)
  *   NG_BLOCK_NVFP4  4-bit numbers, blocks of 16, scale an E4M3 number times `scale`, one power of two for
- *                   the matrix (2^-64 .. 2^64)
+ *                   the matrix (2^-32 .. 2^32)
  *   NG_BLOCK_MXFP8  8-bit numbers (E4M3, up to 448), blocks of 32, scale a power of two; a number that is not
  *                   zero never becomes zero
  * A power-of-two scale is the smallest that brings the block's largest magnitude within the format; an

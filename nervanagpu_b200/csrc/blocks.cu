@@ -717,8 +717,8 @@ int check_shape(const ng_block_desc* d) {
   if (d->rows > 0x7fff0000 || d->cols > 0x7fff0000) return fail(NG_ERR_TOO_LARGE, "a matrix in blocks has at most 2^31 - 65536 rows and columns");
   if (d->format == NG_BLOCK_NVFP4) {
     int ex = 0;
-    if (!(d->scale > 0.0f) || !std::isfinite(d->scale) || std::frexp(d->scale, &ex) != 0.5f || ex < -63 || ex > 65)
-      return fail(NG_ERR_INVALID_ARG, "the scale of an nvfp4 matrix is a power of two from 2^-64 to 2^64");
+    if (!(d->scale > 0.0f) || !std::isfinite(d->scale) || std::frexp(d->scale, &ex) != 0.5f || ex < -31 || ex > 33)
+      return fail(NG_ERR_INVALID_ARG, "the scale of an nvfp4 matrix is a power of two from 2^-32 to 2^32");
   } else if (d->scale != 1.0f) {
     return fail(NG_ERR_INVALID_ARG, "only nvfp4 matrices have a scale");
   }

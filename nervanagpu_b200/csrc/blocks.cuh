@@ -62,7 +62,7 @@ struct BlockFormat {
   }
   static __device__ __forceinline__ long long scale_at(const BlockView& v, int o, int b) {
     if (!k4) return o * v.spitch + b;
-    return (o >> 7) * v.spitch + (b >> 2) * kScaleTile + (o & 31) * 16 + ((o >> 5) & 3) * 4 + (b & 3);
+    return (o >> 7) * v.spitch + (b >> 2) * static_cast<long long>(kScaleTile) + (o & 31) * 16 + ((o >> 5) & 3) * 4 + (b & 3);
   }
 };
 

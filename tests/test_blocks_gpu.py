@@ -107,7 +107,7 @@ def test_nvfp4_scales_saturate_and_never_vanish(ng):
     x[0, :16] = np.linspace(0, 6 * 448 * 3.0, 16)       # scale limited to 448: numbers to 6 * 448
     x[1, :16] = np.linspace(0, 6 * 2.0 ** -12, 16)      # scale kept at 2^-9
     x[2, 16:] = 1.0
-    for t in (1.0, 2.0 ** -64, 2.0 ** 64, 2.0 ** -8):
+    for t in (1.0, 2.0 ** -32, 2.0 ** 32, 2.0 ** -8):
         got = round_trip(ng, x, "nvfp4", 1, t)
         assert np.array_equal(got.astype(np.float64), rm.block_values(x, "nvfp4", 1, t)), t
 
