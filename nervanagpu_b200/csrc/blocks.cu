@@ -127,12 +127,25 @@ __device__ __forceinline__ uint32_t top_bits(const Raw<float, kCount>& r, int h0
 }
 
 // Rows at addresses that are no multiples of 16 bytes: the warp moves its 32 kCount numbers (a run of kCount <<
-// log_tx of each of its rows, at least 128) in order, one number per lane and access, through shared memory. (A lane that moved its
+// log_tx of each of its rows) in order, one number per lane and access, through shared memory. (A lane that moved its
 // own 16 one by one touched 32 sectors per access: 139968 x 125 fp16 read back from 8 bits took 51 us.)
 template <typename T, bool kStore, int kCount>
 __device__ __forceinline__ void warp_move(T* base, long long so, long long o_first, int outer, int l_first, int inner, int log_tx, T* stage) {
   const int lane = threadIdx.x + threadIdx.y * blockDim.x & 31;
   const int per_row = log_tx + (kCount == 32 ? 5 : 4) - 7;      // logarithm: pieces of 128 in a row
+  if (per_row < 0) {
+    // short rows, several in 128 numbers
+    const int run = 128 >> -per_row;
+#pragma unroll 4
+    for (int i = 0; i < kCount; ++i) {
+      const int e = i * 32 + lane, l = l_first + (e & (run - 1));
+      const long long o = o_first + (e >> (7 + per_row));
+      const bool live = o < outer && l < inner;
+      if (!kStore) stage[e] = live ? base[o * so + l] : T(0.0f);
+      else if (live) base[o * so + l] = stage[e];
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < kCount / 4; ++i) {
     const long long o = o_first + (i >> per_row);
@@ -191,10 +204,13 @@ __host__ __device__ constexpr int quantize_lane() {
   return BlockFormat<kFmt>::k4 && sizeof(T) == 2 ? 32 : 16;
 }
 
-template <typename T, int kFmt, bool kVec>
-__global__ void __launch_bounds__(256, !kVec && sizeof(T) == 4 ? 6 : 4) quantize_rows_kernel(BlockView q, PlainView<const T> a, int early) {
+// kForm: 0 rows at odd addresses; 1 aligned rows; 2 aligned rows of less than 128 numbers, with fewer lanes than share a word
+// of scales (the test for that costs the others 0.8 of 10.3 us, 139968 x 128 mxfp8).
+template <typename T, int kFmt, int kForm>
+__global__ void __launch_bounds__(256, kForm == 0 && sizeof(T) == 4 ? 6 : 4) quantize_rows_kernel(BlockView q, PlainView<const T> a, int early) {
   NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
+  constexpr bool kVec = kForm != 0;
   constexpr int kPer = quantize_lane<T, kFmt>();
   NG_ROWS_PROLOGUE(T, kPer);
   constexpr int kUnroll = kVec ? 2 : 1;                             // rows whose loads are in flight together
@@ -253,7 +269,10 @@ __global__ void __launch_bounds__(256, !kVec && sizeof(T) == 4 ? 6 : 4) quantize
       // the scales of four blocks leave together
       word <<= 8 * kBlocks * (g / kDup % kSharers);
 #pragma unroll
-      for (int d = 1; d < kSharers; d *= 2) word |= __shfl_xor_sync(0xffffffffu, word, d * kDup);
+      for (int d = 1; d < kSharers; d *= 2) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, word, d * kDup);
+        if (kForm == 1 || d * kDup < static_cast<int>(blockDim.x)) word |= other;
+      }
       if (live) {
         uint8_t* dst = q.codes + F::code_at(q, static_cast<int>(o), g * (kPer / 8ll * F::kBytes8));
         if (!F::k4) *reinterpret_cast<uint4*>(dst) = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
@@ -352,6 +371,16 @@ __global__ void __launch_bounds__(256) relu_mask_rows_kernel(BlockView q, PlainV
       // zeros, one number per lane and access, in the order of warp_move
       const int l_warp = (g - (lane & (static_cast<int>(blockDim.x) - 1))) * kLane;
       const long long o_warp = o0 + (tid & ~31) / static_cast<int>(blockDim.x);
+      if (log_tx < 3) {
+#pragma unroll 4
+        for (int i = 0; i < kLane; ++i) {
+          const int e = i * 32 + lane, l = l_warp + (e & ((16 << log_tx) - 1));
+          const long long row = o_warp + (e >> (4 + log_tx));
+          const uint32_t mask = __shfl_sync(0xffffffffu, off, i * 2 + (lane >> 4));
+          if ((mask >> (lane & 15) & 1u) && row < q.outer && l < q.inner) a.p[row * a.so + l] = T(0.0f);
+        }
+        continue;
+      }
 #pragma unroll 1
       for (int i = 0; i < 4; ++i) {
         const long long row = o_warp + (i >> (log_tx - 3));
@@ -598,12 +627,19 @@ int launch(const DeviceCtx* c, void (*kernel)(P...), dim3 grid, dim3 block, cuda
   NG_CHECK_LAUNCH();
   return NG_OK;
 }
-// Lanes per row: its groups of `count` numbers, rounded up to 128 of these (four blocks, whose scales leave together), over
-// CTAs of so many threads with as few idle lanes as a power of two allows; the other threads take other rows.
-RowGrid row_grid(const DeviceCtx* c, const BlockView& q, int threads, int count) {
-  const int groups = static_cast<int>((q.inner + 127ll) / 128 * (128 / count));
-  int tx = threads;
-  while (tx > 128 / count && (groups + tx / 2 - 1) / (tx / 2) * (tx / 2) < (groups + tx - 1) / tx * tx) tx /= 2;
+// Lanes per row: its groups of `count` numbers, over CTAs of so many threads with as few idle lanes as a power of two allows;
+// the other threads take other rows. The scales of four blocks leave together, so a row has no fewer lanes than 128 numbers
+// take, unless all of it fits into fewer (a shared block's two at least).
+RowGrid row_grid(const DeviceCtx* c, const BlockView& q, int threads, int count, int least) {
+  const int few = 128 / count;
+  int groups = static_cast<int>((q.inner + count - 1ll) / count), tx = threads;
+  if (groups < few) {
+    for (tx = least; tx < groups; tx *= 2) {}
+    groups = tx;
+  } else {
+    groups = (groups + few - 1) / few * few;
+    while (tx > few && (groups + tx / 2 - 1) / (tx / 2) * (tx / 2) < (groups + tx - 1) / tx * tx) tx /= 2;
+  }
   const int ty = threads / tx;
   RowGrid r;
   r.block = dim3(tx, ty);
@@ -636,10 +672,11 @@ int quantize_one(DeviceCtx* c, const BlockView& q, PlainView<const T> a, cudaStr
   const int blocks = (q.inner + BlockFormat<kFmt>::kBlock - 1) / BlockFormat<kFmt>::kBlock;
   int rc;
   if (a.sl == 1) {
-    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128, quantize_lane<T, kFmt>());
+    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128, quantize_lane<T, kFmt>(), quantize_lane<T, kFmt>() < BlockFormat<kFmt>::kBlock ? 2 : 1);
     a.wide = aligned_rows(a, 32);
-    if (aligned_rows(a, 16)) rc = launch(c, quantize_rows_kernel<T, kFmt, true>, g.grid, g.block, stream, q, a);
-    else rc = launch(c, quantize_rows_kernel<T, kFmt, false>, g.grid, g.block, stream, q, a);
+    if (!aligned_rows(a, 16)) rc = launch(c, quantize_rows_kernel<T, kFmt, 0>, g.grid, g.block, stream, q, a);
+    else if (g.block.x * quantize_lane<T, kFmt>() >= 128) rc = launch(c, quantize_rows_kernel<T, kFmt, 1>, g.grid, g.block, stream, q, a);
+    else rc = launch(c, quantize_rows_kernel<T, kFmt, 2>, g.grid, g.block, stream, q, a);
   } else {
     const dim3 grid((q.outer + kStridedRows - 1) / kStridedRows, std::min((blocks + 3) / 4, 65535));
     if (aligned_pairs(q, a)) rc = launch(c, quantize_strided_kernel<T, kFmt, true>, grid, dim3(kStridedThreads), stream, q, a, blocks);
@@ -653,7 +690,7 @@ int dequantize_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_
   const int units = (q.inner + 15) / 16;
   int rc;
   if (a.sl == 1) {
-    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128, kLane);
+    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128, kLane, 1);
     a.wide = aligned_rows(a, 32);
     if (aligned_rows(a, 16)) rc = launch(c, dequantize_rows_kernel<T, kFmt, true>, g.grid, g.block, stream, q, a);
     else rc = launch(c, dequantize_rows_kernel<T, kFmt, false>, g.grid, g.block, stream, q, a);
@@ -670,7 +707,7 @@ int relu_mask_one(DeviceCtx* c, const BlockView& q, PlainView<T> a, cudaStream_t
   const int blocks = (q.inner + 31) / 32;
   int rc;
   if (a.sl == 1) {
-    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128, kLane);
+    const RowGrid g = row_grid(c, q, aligned_rows(a, 16) ? 256 : 128, kLane, 1);
     a.wide = aligned_rows(a, 32);
     if (aligned_rows(a, 16)) rc = launch(c, relu_mask_rows_kernel<T, true>, g.grid, g.block, stream, q, a);
     else rc = launch(c, relu_mask_rows_kernel<T, false>, g.grid, g.block, stream, q, a);
