@@ -260,7 +260,8 @@ int ng_block_bytes(const ng_block_desc* desc, size_t* codes_bytes, size_t* scale
  * the n_outs (1 to 4) matrices in blocks, all of A's shape. */
 int ng_block_quantize(const void* A, int dtype_bytes, long long row_stride, long long col_stride,
                       const ng_block_desc* outs, int n_outs, void* stream);
-/* The values that the codes stand for; where dtype_bytes is 2, rounded to fp16 and limited to +-65504. */
+/* The values that the codes stand for; rounded to fp16 where dtype_bytes is 2, and limited to the type's
+ * largest number. */
 int ng_block_dequantize(const ng_block_desc* q, void* out, int dtype_bytes, long long row_stride, long long col_stride,
                         void* stream);
 /* E = q > 0 ? E : 0 in place, q in mxfp8: the mask of a ReLU whose output was put into q. */

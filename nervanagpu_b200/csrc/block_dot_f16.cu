@@ -246,7 +246,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
             for (int h = 0; h < 2; ++h) {
               float f[8];
               block_decode8<NG_BLOCK_MXFP8>(h ? make_uint2(w[i].z, w[i].w) : make_uint2(w[i].x, w[i].y), scale[i / 2], f);
-              block_limit_f16<NG_BLOCK_MXFP8>(scale[i / 2], f);
+              block_limit<NG_BLOCK_MXFP8, __half>(scale[i / 2], f);
               __half2* o = reinterpret_cast<__half2*>(&v[h]);
 #pragma unroll
               for (int y = 0; y < 4; ++y) o[y] = __floats2half2_rn(f[2 * y], f[2 * y + 1]);

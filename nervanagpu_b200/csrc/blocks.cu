@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(BlockView q, Plain
         for (int h = 0; h < 2; ++h) {
           float v[8];
           block_decode8<kFmt>(h == 0 ? make_uint2(codes[u].x, codes[u].y) : make_uint2(codes[u].z, codes[u].w), scale, v);
-          if (sizeof(T) == 2) block_limit_f16<kFmt>(scale, v);
+          block_limit<kFmt, T>(scale, v);
 #pragma unroll
           for (int i = 0; i < 8; ++i) from_f32(v[i], r.at()[8 * h + i]);
         }
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kStridedThreads) dequantize_strided_kernel(Blo
       for (int j = 0; j < 2; ++j) {
         float f[8];
         block_decode8<kFmt>(F::k4 ? make_uint2(w[j][h], 0u) : make_uint2(w[j][2 * h], w[j][2 * h + 1]), scale[j], f);
-        if (sizeof(T) == 2) block_limit_f16<kFmt>(scale[j], f);
+        block_limit<kFmt, T>(scale[j], f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) from_f32(f[i], v[j][i]);
       }

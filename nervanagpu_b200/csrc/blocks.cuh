@@ -12,7 +12,8 @@
 //   code = RN(x / scale), ties to even, limited to the largest number
 //   mxfp8: a number that is not zero gets a code that is not zero, so that x > 0 can be told from the code.
 //
-// Read as fp16, values are limited to +-65504: a number next to fp16's largest may have been rounded to one beyond it.
+// Values are read limited to the largest number of the type that they are read as: a number next to it may have been
+// rounded to one beyond it.
 //
 // A block with an infinity or a NaN has the scale NaN (0xff, or 0x7f in E4M3): all of it reads back as NaN. A
 // product sums over the block, so its result is lost either way. mxfp8 codes keep the signs in such blocks too.
@@ -260,13 +261,14 @@ __device__ __forceinline__ uint4 block_decode8_f16(uint2 codes, __half2 scale) {
   return r;
 }
 
-// The same for an fp16 result: limited to its largest number (a NaN stays one).
-template <int kFmt>
-__device__ __forceinline__ void block_limit_f16(float scale, float (&v)[8]) {
-  if (scale * (BlockFormat<kFmt>::k4 ? 6.0f : 448.0f) > 65504.0f) {
+// The same, limited to the largest number of the result's type (a NaN stays one).
+template <int kFmt, typename T>
+__device__ __forceinline__ void block_limit(float scale, float (&v)[8]) {
+  constexpr float kLargest = sizeof(T) == 2 ? 65504.0f : 3.402823466e+38f;
+  if (scale * (BlockFormat<kFmt>::k4 ? 6.0f : 448.0f) > kLargest) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (fabsf(v[i]) > 65504.0f) v[i] = copysignf(65504.0f, v[i]);
+      if (fabsf(v[i]) > kLargest) v[i] = copysignf(kLargest, v[i]);
   }
 }
 

@@ -795,7 +795,7 @@ class NervanaGPU(object):
         return outs[0] if len(outs) == 1 else outs
 
     def dequantize(self, Q, out):
-        """out = the values that Q's codes stand for (fp16: rounded, and limited to +-65504)."""
+        """out = the values that Q's codes stand for (fp16: rounded), limited to the largest of out's type."""
         if _native.block_plain(0, self, Q, out):
             return out
         self._plain_matrix(out, Q)
