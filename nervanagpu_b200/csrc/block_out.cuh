@@ -11,7 +11,7 @@ struct OutParams {
   void* C;
   long long ldc;
   int out_f32;
-  int store;              // 1: C's rows are such as TMA can address; 0: one number per lane and access
+  int store;              // 1: TMA can address C's rows, whole; 0: one number per lane and access
   EpiArgs ea;
 };
 

@@ -787,7 +787,10 @@ int plain_map(CUtensorMap* map, const void* base, long long rows, long long cols
 OutParams make_out(void* C, int m, int n, int ldc, int out_f32, const EpiArgs& ea) {
   OutParams out = {};
   out.M = m; out.N = n; out.C = C; out.ldc = ldc; out.out_f32 = out_f32; out.ea = ea;
-  out.store = (reinterpret_cast<uintptr_t>(C) & 15u) == 0 && ldc % (out_f32 ? 4 : 8) == 0;
+  // (a box that leaves the matrix is cut at whole 16 bytes: rows that end inside one, in a wider matrix, would have their
+  // neighbours overwritten)
+  const int per16 = out_f32 ? 4 : 8;
+  out.store = (reinterpret_cast<uintptr_t>(C) & 15u) == 0 && ldc % per16 == 0 && n % per16 == 0;
   return out;
 }
 

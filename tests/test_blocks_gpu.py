@@ -284,6 +284,23 @@ def test_product_output_stage(ng, m, n, k, mixed):
     assert np.array_equal(C.get(), got)
 
 
+@pytest.mark.parametrize("m,n,k", [(300, 7, 40), (2049, 2301, 300), (2500, 2310, 96), (130, 13, 256)])
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_rows_that_end_inside_16_bytes_of_a_wider_matrix(ng, m, n, k, mixed, dtype):
+    """Aligned rows with a ragged end: what lies behind them stays."""
+    W, X = np.ones((m, k), np.float16), np.ones((k, n), np.float16)
+    A = ng.array(W) if mixed else filled(ng, W, "mxfp4", 1)
+    B = filled(ng, X, "mxfp8" if mixed else "mxfp4", 0)
+    ld = -(-(n + 1) // 8) * 8
+    wide = ng.array(np.full((m + 1, ld), 3.0), dtype=dtype)
+    want = np.full((m + 1, ld), 3.0)
+    for beta in (0.0, 1.0):
+        ng.block_dot(A, B, wide[:m, :n], beta=beta)
+        want[:m, :n] = k * (1 + beta)
+        assert np.array_equal(wide.get(), want.astype(dtype)), beta
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (2, 3, 31), (128, 64, 32), (33, 17, 125), (130, 257, 300), (1001, 515, 125),
                                    (64, 256, 2048), (300, 200, 64), (16, 1000, 128), (257, 9, 4100),
                                    (2048, 1301, 70), (2496, 2304, 96), (2400, 2311, 33), (19000, 65, 40)])
