@@ -301,6 +301,26 @@ def test_rows_that_end_inside_16_bytes_of_a_wider_matrix(ng, m, n, k, mixed, dty
         assert np.array_equal(wide.get(), want.astype(dtype)), beta
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 40, 7), (300, 300, 45), (130, 700, 1003), (2100, 2061, 301)])
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4", "nvfp4"])
+def test_what_lies_around_an_input_is_not_read(ng, m, n, k, fmt):
+    """Inputs that are views of wider matrices, aligned or not, between NaN. In nvfp4 a block of ones has the scale
+    1/6, to the nearest e4m3 number 0.171875, and 1 is read back as 6 * 0.171875 = 1.03125; its square is a multiple of
+    2^-10 and sums of up to 2^13 of them are exact in 32 bits."""
+    one = 1.03125 if fmt == "nvfp4" else 1.0
+    for first, more in ((0, -k % 8), (8, -k % 8), (1, 2)):
+        def within(r, c):
+            wide = np.full((r + 2, first + c + more), np.nan, np.float16)
+            wide[1:r + 1, first:first + c] = 1
+            return ng.array(wide)[1:r + 1, first:first + c]
+        W, X = within(m, k), within(n, k)
+        A = W if fmt == "mxfp8" else ng.quantize(W, ng.block_empty((m, k), fmt))
+        B = ng.quantize(X, ng.block_empty((n, k), fmt)).T
+        C = ng.empty((m, n), dtype=np.float32)
+        ng.block_dot(A, B, C)
+        assert np.array_equal(C.get(), np.full((m, n), k * one * one)), (first, more)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (2, 3, 31), (128, 64, 32), (33, 17, 125), (130, 257, 300), (1001, 515, 125),
                                    (64, 256, 2048), (300, 200, 64), (16, 1000, 128), (257, 9, 4100),
                                    (2048, 1301, 70), (2496, 2304, 96), (2400, 2311, 33), (19000, 65, 40)])
