@@ -301,6 +301,60 @@ def test_rows_that_end_inside_16_bytes_of_a_wider_matrix(ng, m, n, k, mixed, dty
         assert np.array_equal(wide.get(), want.astype(dtype)), beta
 
 
+def long_matrix(ng, rows, cols, rng):
+    """More than 2^32 numbers: zeros but for whole numbers up to 4 in the last two rows (read back as they are in every
+    format whose blocks hold them: each block of 16 has a 4, and a 1 or 2 else)."""
+    A = ng.empty((rows, cols), dtype=np.float16)
+    A.fill(0)
+    last = rng.choice([1.0, 2.0], (2, cols)).astype(np.float16)
+    last[:, ::16] = 4
+    A[rows - 2:].set(last)
+    return A, last
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("axis", [0, 1])
+def test_matrices_of_more_numbers_than_32_bits_count(ng, fmt, axis):
+    rows, cols = 70002, 65008
+    A, last = long_matrix(ng, rows, cols, np.random.default_rng(3))
+    Q = ng.quantize(A, ng.block_empty((rows, cols), fmt, axis=axis))
+    A.fill(9)
+    ng.dequantize(Q, A)
+    assert np.array_equal(A[rows - 2:].get(), last)
+    assert not A[rows - 200:rows - 2].get().any()
+    if fmt == "mxfp8" and axis == 1:
+        A.fill(9)
+        ng.relu_mask(Q, A)
+        assert np.array_equal(A[rows - 2:].get(), np.where(last > 0, 9.0, 0.0))
+        assert not A[rows - 200:rows - 2].get().any()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_products_of_long_matrices(ng, fmt):
+    """The long matrix as the left side, and as the output. Sums of up to 65008 products of up to 4, whole numbers below
+    2^24, are exact in 32 bits."""
+    rows, cols = 70002, 65008
+    A, last = long_matrix(ng, rows, cols, np.random.default_rng(4))
+    X = np.ones((8, cols), np.float16)
+    B = ng.quantize(ng.array(X), ng.block_empty((8, cols), fmt)).T
+    left = A if fmt == "mxfp8" else ng.quantize(A, ng.block_empty((rows, cols), fmt))
+    C = ng.empty((rows, 8), dtype=np.float32)
+    ng.block_dot(left, B, C)
+    got = C.get()
+    assert not got[:-2].any()
+    assert np.array_equal(got[-2:], np.tile(last.sum(axis=1, dtype=np.float64)[:, None], (1, 8)))
+
+    w = np.zeros((rows, 32), np.float16)
+    w[-2:] = 1
+    x = np.ones((cols, 32), np.float16)
+    x[-1] = 2
+    W = ng.array(w) if fmt == "mxfp8" else filled(ng, w, fmt, 1)
+    A.fill(9)
+    ng.block_dot(W, filled(ng, x, fmt, 1).T, A)
+    assert not A[rows - 200:rows - 2].get().any()
+    assert np.array_equal(A[rows - 2:].get(), np.tile(32 * x[:, 0], (2, 1)))
+
+
 @pytest.mark.parametrize("m,n,k", [(5, 40, 7), (300, 300, 45), (130, 700, 1003), (2100, 2061, 301)])
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4", "nvfp4"])
 def test_what_lies_around_an_input_is_not_read(ng, m, n, k, fmt):
