@@ -222,7 +222,9 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
   if (warp >= 2) {
     const bool done = mbar_wait(acc_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
     __syncwarp();
-    if (done && !*abort_flag) {
+    if (!done) {
+      wait_for_strays();
+    } else if (!*abort_flag) {
       tc_fence_after();
       const int group = warp & 3, half = (warp - 2) >> 2;
       float* row = reinterpret_cast<float*>(ring_gen) + (group * 32 + lane) * T::kPitch;
@@ -266,7 +268,10 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
     tmem_dealloc(tmem, T::kCols);
   }
   if (splits > 1) {
-    mbar_wait(part_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
+    if (!mbar_wait(part_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns)) {
+      int none = 0;          // given up: the parts come all the same, those of a CTA that gave up too, and later than here maybe
+      mbar_wait(part_bar, 0, &none, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
+    }
     __syncwarp();
     cluster_arrive();        // (with everybody's: all parts have arrived, nobody's tile is read any more)
     __syncthreads();         // the abort flag is final
@@ -367,7 +372,7 @@ int launch_dot(DeviceCtx* c, DotParams& p, int splits, cudaStream_t stream) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = tuning().dependent_launch != 0 ? 2 : 1;
   static std::atomic<unsigned long long> ready{0};      // devices on which this instance may use its shared memory
   if (!(ready.load(std::memory_order_relaxed) >> c->device & 1u)) {
     NG_CUDA(cudaFuncSetAttribute(block_dot_kernel<kN, kNv>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));

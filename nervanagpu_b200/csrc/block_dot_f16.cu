@@ -129,12 +129,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
           tma_load_5d(ring + s * T::kSlot, &mapA, full_bar(s), kb * 64, m0, 0, 0, 0);
         }
       }
-      if (!ok) {
-        // Given up: the loads in flight must land before the CTA may end. Their barriers may never complete, the
-        // other arrivals missing, so this waits for time instead, which no copy inside the device takes.
-        const uint64_t t0 = global_timer_ns();
-        while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
-      }
+      if (!ok) wait_for_strays();
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -163,10 +158,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
         }
         if (ok) tc_commit(accf_bar(acc));
       }
-      if (!ok) {   // what was issued must end before tensor memory is given back (a fresh use of a barrier is not at hand)
-        const uint64_t t0 = global_timer_ns();
-        while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
-      }
+      if (!ok) wait_for_strays();
     }
     __syncwarp();
   } else if (warp < 2 + kMixEpi) {
@@ -177,7 +169,10 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++local) {
       const int acc = local & 1;
       const bool ok = mbar_wait(accf_bar(acc), (local / 2) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
-      if (__any_sync(0xffffffffu, !ok)) break;
+      if (__any_sync(0xffffffffu, !ok)) {
+        wait_for_strays();
+        break;
+      }
       tc_fence_after();
       const int m0 = t / p.tiles_n * 128 + group * 32, n0 = t % p.tiles_n * kN + half * T::kEpiCols;
       const uint32_t taddr = tmem + (static_cast<uint32_t>(group * 32) << 16) + acc * kN + half * T::kEpiCols;

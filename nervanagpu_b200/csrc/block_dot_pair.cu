@@ -156,7 +156,10 @@ block_dot_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_consta
     int local = 0;
     for (int t = first_tile; t < p.tiles; t += step, ++local) {
       const bool ok = mbar_wait(accf_bar, local & 1, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
-      if (__any_sync(0xffffffffu, !ok)) break;
+      if (__any_sync(0xffffffffu, !ok)) {
+        gave_up = true;
+        break;
+      }
       tc_fence_after();
       const int m0 = t / p.tiles_n * 256 + rank * 128 + group * 32, n0 = t % p.tiles_n * 256 + half * 128;
       const uint32_t taddr = tmem + (static_cast<uint32_t>(group * 32) << 16) + half * 128;
@@ -166,12 +169,7 @@ block_dot_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_consta
     }
     if (lane == 0) tma_store_wait_all();
   }
-  // Given up: copies and MMAs in flight end by themselves in microseconds, but the barriers that would tell may never
-  // complete without the other arrivals. So this waits for time.
-  if (gave_up) {
-    const uint64_t t0 = global_timer_ns();
-    while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
-  }
+  if (gave_up) wait_for_strays();
   __syncwarp();
   __syncthreads();
   cluster_sync_all();                // nobody arrives here any more

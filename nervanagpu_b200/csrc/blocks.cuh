@@ -67,6 +67,13 @@ struct BlockFormat {
   }
 };
 
+// For a kernel that gives up: copies and MMAs in flight must end before the CTA may, and do so in microseconds, but the
+// barriers that would tell may never complete, other arrivals missing. So this waits for time.
+__device__ __forceinline__ void wait_for_strays() {
+  const uint64_t t0 = global_timer_ns();
+  while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
+}
+
 // fp32 -> E4M3 / E2M1, two at a time, the first in the low half; to nearest, ties to even, limited to the largest
 __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
   uint16_t r;

@@ -52,6 +52,8 @@ class Layer(object):
             self.fprop_out = shared[0].share(self.dimO)
             shared.reverse()
         self.act_stats = self.lib.empty((self.dimO2[0], 1), dtype=np.float32)
+        if self.checkpoint:
+            self.record = self.lib.block_empty(self.dimI2, "mxfp8")
 
     def init_deltas(self, shared=None):
         if shared is None:
@@ -93,8 +95,6 @@ class Layer(object):
         every activation in fp16, nervanagpu/layers.py:64-70.)"""
         outs = list(operands)
         if self.checkpoint:
-            if self.record is None:
-                self.record = self.lib.block_empty(self.dimI2, "mxfp8")
             outs.append(self.record)
         if outs:
             self.lib.quantize(fprop_in.reshape(self.dimI2), *outs)
@@ -236,18 +236,23 @@ class FullLayer(Layer):
         self.dimF = self.dimF2 = (nOut, nIn)
         self.sizeI, self.sizeO, self.sizeF = nIn * N, nOut * N, nIn * nOut
 
-    def quantize_weights(self):
-        if self.weight_blocks is None:
+    def init_activations(self, shared=None):
+        super(FullLayer, self).init_activations(shared)
+        if self.products:
             ws, xs = self.scales if self.products == "nvfp4" else (1.0, 1.0)
             self.weight_blocks = self.lib.block_empty(self.dimF, self.products, axis=1, scale=ws)
             self.input_blocks = self.lib.block_empty(self.dimI, self.products, axis=0, scale=xs)
-        self.lib.quantize(self.weights, self.weight_blocks)
+        self.weights_fixed = False
+
+    def init_weights(self, *args, **kwargs):
+        super(FullLayer, self).init_weights(*args, **kwargs)
+        self.weights_fixed = False
 
     def fix_weights(self):
         """Quantise the weights now and no more until the next descent: for inference. A program that writes `weights`
         itself calls this again."""
         if self.products:
-            self.quantize_weights()
+            self.lib.quantize(self.weights, self.weight_blocks)
             self.weights_fixed = True
 
     def grad_descent(self):
@@ -262,7 +267,7 @@ class FullLayer(Layer):
         fprop_in = super(FullLayer, self).fprop(fprop_in)
         if self.products:
             if not self.weights_fixed:
-                self.quantize_weights()
+                self.lib.quantize(self.weights, self.weight_blocks)
             self.record_input(fprop_in, self.input_blocks)
             self.lib.block_dot(self.weight_blocks, self.input_blocks, self.fprop_out, relu=True)
         else:
@@ -346,14 +351,17 @@ class ConvLayer(Layer):
             self.lib.bprop_conv(self, self.weights, bprop_in, self.bprop_out)
         inputs = self.fprop_in
         if self.checkpoint:
-            if self.restored is None:
-                self.init_restored()
             inputs = self.restored
             self.lib.dequantize(self.record, inputs.reshape(self.dimI2))
         self.lib.update_conv(self, inputs, bprop_in, self.updat_out)
         self.grad_descent()
         self.mask_below()
         return self.bprop_out
+
+    def init_activations(self, shared=None):
+        super(ConvLayer, self).init_activations(shared)
+        if self.checkpoint and self.restored is None:
+            self.init_restored()
 
     def init_restored(self, shared=None):
         self.restored = self.lib.empty(self.dimI, dtype=self.dtype) if shared is None else shared.share(self.dimI)

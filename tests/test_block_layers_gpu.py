@@ -162,6 +162,30 @@ def test_fixed_weights_follow_a_descent_and_recorded_steps_repeat():
         assert_close(layer.updat_out.get(), em @ xr.T, product_tol(em @ xr.T, np.abs(em) @ xr.T, 32))
 
 
+def test_new_weights_are_quantised_and_a_first_step_can_be_recorded():
+    """All that a fully-connected layer's step needs is there before it: no allocation, which a recording refuses. (A
+    convolution's workspace grows when it first runs: that is refused in a recording, with records or without.) Weights of
+    ones and inputs of powers of two: exact in every format."""
+    ng = NervanaGPU(stochastic_round=False)
+    ng.stream = ng.new_stream()
+    full = FullLayer(ng, np.float16, 32, 96, 64, products="mxfp4", checkpoint=True)
+    full.init_activations()
+    full.init_deltas()
+    full.init_weights(zeros=True)
+    full.fix_weights()
+    full.init_weights(zeros=True)
+    full.weights.fill(1)
+    X, E = ng.empty((96, 32)), ng.empty((64, 32))
+    X.fill(2), E.fill(1)
+
+    def step():
+        full.fprop(X)
+        full.bprop(E)
+
+    ng.capture(step).launch()
+    assert (full.fprop_out.get() == 192).all() and (full.updat_out.get() == 64).all()
+
+
 def test_networks_run_through_the_driver_with_records_and_blocks():
     ng = NervanaGPU(stochastic_round=False)
     res = cb.run_network(ng, "Alexnet", loops=1, out=lambda line: None, checkpoint=True, products="nvfp4")
