@@ -92,25 +92,6 @@ __device__ __forceinline__ void bulk_push(uint32_t dst_cluster, uint32_t src, ui
 // only says that nobody reads this CTA's tile any more. As a release each took half a microsecond.)
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// One output, in fp16 or fp32 (the arithmetic of epi_store8).
-__device__ __forceinline__ void epi_store1(const EpiArgs& e, float acc, void* out, int out_f32, unsigned long long lin) {
-  float c = epi_scale(e, acc);
-  if (out_f32) {
-    float* p = static_cast<float*>(out);
-    if (e.beta != 0.0f) c = fmaf(e.beta, *p, c);
-    *p = c;
-    return;
-  }
-  __half* p = static_cast<__half*>(out);
-  if (e.beta != 0.0f) c = fmaf(e.beta, __half2float(*p), c);
-  if (e.sr_bits) {
-    uint32_t rnd[8];
-    sr_bits8(e, lin >> 3, rnd);
-    *p = f2h_sr(c, rnd[lin & 7ull], e.sr_bits);
-  } else {
-    *p = f2h_rn(c);
-  }
-}
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t n;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
@@ -335,19 +316,57 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
     const int run_step = p.swapped ? 1 : T::kPitch, step = p.swapped ? T::kPitch : 1;
     const long long row0 = p.swapped ? n0 : m0 + r0, col0 = p.swapped ? m0 + r0 : n0;
     const int width = p.swapped ? p.M : p.N;
-    const bool plain = p.ea.beta == 0.0f && p.ea.sr_bits == 0 && !p.out_f32;
-    for (int u = warp; u < runs; u += kDotThreads / 32) {
-      const long long row = row0 + u;
-      uint8_t* out = static_cast<uint8_t*>(p.C) + (row * p.ldc + col0) * (p.out_f32 ? 4 : 2);
-      const float* src = own + u * run_step;
+    auto rows_of = [&](auto* base) {
+      using E = std::remove_pointer_t<decltype(base)>;
+      constexpr int kWarps = kDotThreads / 32;
+      if (sizeof(E) == 2 && p.ea.sr_bits) {
+        // eight neighbours at a time, which share their random bits
+        const int eights = (len + 7) / 8;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < runs * eights; i += kDotThreads) {
+          const int u = i / eights, c = i % eights * 8;
+          const float* src = own + u * run_step + c * step;
+          float v[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = j * 32 + lane;
-        if (i >= len) break;
-        if (plain) reinterpret_cast<__half*>(out)[i] = f2h_rn(epi_scale(p.ea, src[i * step]));
-        else epi_store1(p.ea, src[i * step], out + i * (p.out_f32 ? 4 : 2), p.out_f32, static_cast<unsigned long long>(row) * width + col0 + i);
+          for (int j = 0; j < 8; ++j) v[j] = c + j < len ? src[j * step] : 0.0f;
+          E* row = base + (row0 + u) * p.ldc;
+          epi_store8_call<false>(p.ea, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], row, row, static_cast<int>(col0) + c,
+                                 static_cast<unsigned long long>(row0 + u) * width + col0 + c, min(8, len - c), false);
+        }
+        return;
       }
-    }
+      // (what C held in four rows is on its way together: one by one, 128 rows of a tile took 10 us)
+#pragma unroll 1
+      for (int u0 = warp; u0 < runs && p.ea.beta != 0.0f; u0 += 4 * kWarps) {
+        OldBits<E> old[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int u = u0 + r * kWarps, i = j * 32 + lane;
+            old[r][j] = u < runs && i < len ? reinterpret_cast<const OldBits<E>*>(base)[(row0 + u) * p.ldc + col0 + i] : OldBits<E>(0);
+          }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int u = u0 + r * kWarps;
+          if (u >= runs) break;
+          E* out = base + (row0 + u) * p.ldc + col0 + lane;
+          const float* src = own + u * run_step + lane * step;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j * 32 + lane < len) epi_store_nearest(p.ea, src[j * 32 * step], to_f32(old[r][j]), out + j * 32);
+        }
+      }
+      for (int u = warp; u < runs && p.ea.beta == 0.0f; u += kWarps) {
+        E* out = base + (row0 + u) * p.ldc + col0 + lane;
+        const float* src = own + u * run_step + lane * step;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j * 32 + lane < len) epi_put(epi_scale(p.ea, src[j * 32 * step]), out + j * 32);
+      }
+    };
+    if (p.out_f32) rows_of(static_cast<float*>(p.C));
+    else rows_of(static_cast<__half*>(p.C));
   }
 #undef NG_BY_PARTS
   __syncwarp();

@@ -55,8 +55,7 @@ struct MixParams {
   unsigned long long wait_limit_ns;
 };
 
-// kLean: fp16 outputs rounded to nearest with nothing added; the other instance does all.
-template <int kN, bool kLean>
+template <int kN, int kForm>
 __global__ void __launch_bounds__(kMixThreads, 1)
 block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapX,
                      const __grid_constant__ CUtensorMap mapC, const __grid_constant__ MixParams p) {
@@ -165,21 +164,24 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     const int group = warp & 3, half = (warp - 2) >> 2;
     const uint32_t stage = staging + (warp - 2) * 4096u;
     uint8_t* stage_gen = ring_gen + (stage - ring);
+    auto row_of = [&](int t) { return t / p.tiles_n * 128 + group * 32; };
+    auto col_of = [&](int t) { return t % p.tiles_n * kN + half * T::kEpiCols; };
     int local = 0;
     for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++local) {
       const int acc = local & 1;
+      const int m0 = row_of(t), n0 = col_of(t);
+      if (local == 0) out_ahead<kForm, T::kEpiCols>(p.out, m0, n0);
       const bool ok = mbar_wait(accf_bar(acc), (local / 2) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
       if (__any_sync(0xffffffffu, !ok)) {
         wait_for_strays();
         break;
       }
       tc_fence_after();
-      const int m0 = t / p.tiles_n * 128 + group * 32, n0 = t % p.tiles_n * kN + half * T::kEpiCols;
+      if (t + static_cast<int>(gridDim.x) < p.tiles) out_ahead<kForm, T::kEpiCols>(p.out, row_of(t + gridDim.x), col_of(t + gridDim.x));
       const uint32_t taddr = tmem + (static_cast<uint32_t>(group * 32) << 16) + acc * kN + half * T::kEpiCols;
       auto release = [&] { if (lane == 0) mbar_arrive(acce_bar(acc)); };
       if (half * T::kEpiCols >= kN) release();
-      else if constexpr (kLean) out_lean<T::kEpiCols>(p.out, &mapC, taddr, stage, stage_gen, m0, n0, release);
-      else out_any<T::kEpiCols>(p.out, &mapC, taddr, stage, stage_gen, m0, n0, release);
+      else out_tile<kForm, T::kEpiCols>(p.out, &mapC, taddr, stage, stage_gen, m0, n0, release);
     }
     if (lane == 0) tma_store_wait_all();
     __syncwarp();
@@ -208,7 +210,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
           for (int i = 0; i < kRows; ++i) {
             const __half* row = p.A + static_cast<long long>(m0 + a_row + i) * p.lda + k0;
             const bool row_ok = m0 + a_row + i < p.M;
-            from_a[i] = __halves2half2(row_ok && k0 < p.K ? row[0] : __half(0.0f), row_ok && k0 + 32 < p.K ? row[32] : __half(0.0f));
+            from_a[i] = __halves2half2(row_ok && k0 < p.K ? row[0] : zero_of<__half>(), row_ok && k0 + 32 < p.K ? row[32] : zero_of<__half>());
           }
         }
         ok = mbar_wait(rawf_bar(x), (it / kMixRaw) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns) &&
@@ -276,7 +278,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
   }
 }
 
-template <int kN, bool kLean>
+template <int kN, int kForm>
 int launch_mix(DeviceCtx* c, MixParams& p, cudaStream_t stream) {
   using T = MixTile<kN>;
   p.tiles_n = (p.N + kN - 1) / kN;
@@ -302,10 +304,10 @@ int launch_mix(DeviceCtx* c, MixParams& p, cudaStream_t stream) {
   cfg.numAttrs = tuning().dependent_launch != 0 ? 1 : 0;
   static std::atomic<unsigned long long> ready{0};
   if (!(ready.load(std::memory_order_relaxed) >> c->device & 1u)) {
-    NG_CUDA(cudaFuncSetAttribute(block_dot_f16_kernel<kN, kLean>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
+    NG_CUDA(cudaFuncSetAttribute(block_dot_f16_kernel<kN, kForm>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
     ready.fetch_or(1ull << c->device, std::memory_order_relaxed);
   }
-  NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_f16_kernel<kN, kLean>, mapA, mapX, mapC, p));
+  NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_f16_kernel<kN, kForm>, mapA, mapX, mapC, p));
   NG_CHECK_LAUNCH();
   return NG_OK;
 }
@@ -344,7 +346,6 @@ int run_block_dot_f16(DeviceCtx* c, const void* A, int lda, const ng_block_desc&
   p.x = x;
   p.out = make_out(C, m, x.outer, ldc, out_f32, ea);
   p.status = c->status; p.wait_limit_ns = c->wait_limit_ns;
-  const bool lean = out_is_lean(p.out);
   // Columns of a tile: what takes the SMs least time, a tile of n columns counted as n + 64 (its rows of A, its start
   // and its end). 1001 x 4097 x 125: one round of 136 tiles of 256 columns, or four of 520 tiles of 64.
   const long long row_tiles = (m + 127ll) / 128;
@@ -364,8 +365,13 @@ int run_block_dot_f16(DeviceCtx* c, const void* A, int lda, const ng_block_desc&
   const long long rounds = best / (cols + 64);
   int rc;
   if (p.num_kb > 2 && rounds * p.num_kb > 16 && from_scratch(c, A, lda, d, x, C, m, ldc, out_f32, ea, stream, rc)) return rc;
-#define NG_MIX(kn) (lean ? launch_mix<kn, true>(c, p, stream) : launch_mix<kn, false>(c, p, stream))
-  return cols == 256 ? NG_MIX(256) : cols == 128 ? NG_MIX(128) : NG_MIX(64);
+#define NG_MIX(form) \
+  (cols == 256 ? launch_mix<256, form>(c, p, stream) : cols == 128 ? launch_mix<128, form>(c, p, stream) : launch_mix<64, form>(c, p, stream))
+  switch (out_form(p.out)) {
+    case kOutLean: return NG_MIX(kOutLean);
+    case kOutF16: return NG_MIX(kOutF16);
+    default: return NG_MIX(kOutF32);
+  }
 #undef NG_MIX
 }
 

@@ -56,7 +56,7 @@ __device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
-template <bool kNv, bool kLean>
+template <bool kNv, int kForm>
 __global__ void __launch_bounds__(kPairThreads, 1)
 block_dot_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ PairParams p) {
   using T = PairTile<kNv>;
@@ -153,19 +153,22 @@ block_dot_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_consta
     const uint32_t stage = staging + (warp - 2) * 4096u;
     uint8_t* stage_gen = ring_gen + (stage - ring);
     const uint32_t done_bar = map_to_cta(acce_bar, 0);
+    auto row_of = [&](int t) { return t / p.tiles_n * 256 + rank * 128 + group * 32; };
+    auto col_of = [&](int t) { return t % p.tiles_n * 256 + half * 128; };
     int local = 0;
     for (int t = first_tile; t < p.tiles; t += step, ++local) {
+      const int m0 = row_of(t), n0 = col_of(t);
+      if (local == 0) out_ahead<kForm, 128>(p.out, m0, n0);
       const bool ok = mbar_wait(accf_bar, local & 1, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
       if (__any_sync(0xffffffffu, !ok)) {
         gave_up = true;
         break;
       }
       tc_fence_after();
-      const int m0 = t / p.tiles_n * 256 + rank * 128 + group * 32, n0 = t % p.tiles_n * 256 + half * 128;
+      if (t + step < p.tiles) out_ahead<kForm, 128>(p.out, row_of(t + step), col_of(t + step));
       const uint32_t taddr = tmem + (static_cast<uint32_t>(group * 32) << 16) + half * 128;
       auto release = [&] { if (lane == 0) mbar_arrive_relaxed(done_bar); };
-      if constexpr (kLean) out_lean<128>(p.out, &maps.out, taddr, stage, stage_gen, m0, n0, release);
-      else out_any<128>(p.out, &maps.out, taddr, stage, stage_gen, m0, n0, release);
+      out_tile<kForm, 128>(p.out, &maps.out, taddr, stage, stage_gen, m0, n0, release);
     }
     if (lane == 0) tma_store_wait_all();
   }
@@ -188,7 +191,7 @@ int rows_map(CUtensorMap* map, const void* base, long long bytes, int box_rows) 
   return make_tensor_map(map, base, dims, strides, box, 2, true);
 }
 
-template <bool kNv, bool kLean>
+template <bool kNv, int kForm>
 int launch_pair(DeviceCtx* c, const BlockView& a, const BlockView& b, const PairParams& p, cudaStream_t stream) {
   using T = PairTile<kNv>;
   PairMaps maps = {};
@@ -215,10 +218,10 @@ int launch_pair(DeviceCtx* c, const BlockView& a, const BlockView& b, const Pair
   cfg.numAttrs = tuning().dependent_launch != 0 ? 2 : 1;
   static std::atomic<unsigned long long> ready{0};
   if (!(ready.load(std::memory_order_relaxed) >> c->device & 1u)) {
-    NG_CUDA(cudaFuncSetAttribute(block_dot_pair_kernel<kNv, kLean>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
+    NG_CUDA(cudaFuncSetAttribute(block_dot_pair_kernel<kNv, kForm>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
     ready.fetch_or(1ull << c->device, std::memory_order_relaxed);
   }
-  NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_pair_kernel<kNv, kLean>, maps, p));
+  NG_CUDA(cudaLaunchKernelEx(&cfg, block_dot_pair_kernel<kNv, kForm>, maps, p));
   NG_CHECK_LAUNCH();
   return NG_OK;
 }
@@ -234,8 +237,13 @@ int run_block_dot_pair(DeviceCtx* c, const BlockView& a, const BlockView& b, boo
   p.tiles = static_cast<int>(tiles);
   p.out = out;
   p.status = c->status; p.wait_limit_ns = c->wait_limit_ns;
-  if (out_is_lean(out)) return nv ? launch_pair<true, true>(c, a, b, p, stream) : launch_pair<false, true>(c, a, b, p, stream);
-  return nv ? launch_pair<true, false>(c, a, b, p, stream) : launch_pair<false, false>(c, a, b, p, stream);
+#define NG_PAIR(form) (nv ? launch_pair<true, form>(c, a, b, p, stream) : launch_pair<false, form>(c, a, b, p, stream))
+  switch (out_form(out)) {
+    case kOutLean: return NG_PAIR(kOutLean);
+    case kOutF16: return NG_PAIR(kOutF16);
+    default: return NG_PAIR(kOutF32);
+  }
+#undef NG_PAIR
 }
 
 }  // namespace ngb

@@ -1,6 +1,8 @@
 // Output stage of the persistent products on matrices in blocks: a warp takes 32 rows x kCols columns of an
 // accumulator from tensor memory through a staged box of [32 rows][128 bytes] (128-byte swizzle) to C.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "epilogue.cuh"
 
@@ -14,6 +16,22 @@ struct OutParams {
   int store;              // 1: TMA can address C's rows, whole; 0: one number per lane and access
   EpiArgs ea;
 };
+
+// One output, rounded to nearest, with what C held given.
+// (Loaded as bits, converted when used: a load with its conversion under one condition becomes a branch, and waits for the one
+// before.)
+template <typename E>
+using OldBits = std::conditional_t<sizeof(E) == 2, unsigned short, float>;
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(unsigned short x) { return __half2float(__ushort_as_half(x)); }
+__device__ __forceinline__ void epi_put(float c, float* out) { *out = c; }
+__device__ __forceinline__ void epi_put(float c, __half* out) { *out = f2h_rn(c); }
+template <typename E>
+__device__ __forceinline__ void epi_store_nearest(const EpiArgs& e, float acc, float old, E* out) {
+  float c = epi_scale(e, acc);
+  if (e.beta != 0.0f) c = fmaf(e.beta, old, c);
+  epi_put(c, out);
+}
 
 // fp16, rounded to nearest, nothing added: all columns to registers first, then `release` gives the accumulator back.
 template <int kCols, typename F>
@@ -63,27 +81,41 @@ __device__ __forceinline__ void out_lean(const OutParams& p, const CUtensorMap* 
       __syncwarp();
       __half* out = static_cast<__half*>(p.C) + m0 * p.ldc + n0 + c + lane;
       const int rows = min(32, p.M - m0), cols = p.N - n0 - c - lane;
-#pragma unroll 8
-      for (int i = 0; i < rows; ++i, out += p.ldc) {
-        const uint8_t* src = stage_gen + i * 128 + ((lane * 2) & 15);
-        if (cols > 0) out[0] = *reinterpret_cast<const __half*>(src + (((lane >> 3) ^ (i & 7)) << 4));
-        if (cols > 32) out[32] = *reinterpret_cast<const __half*>(src + (((4 + (lane >> 3)) ^ (i & 7)) << 4));
+#pragma unroll 1
+      for (int i0 = 0; i0 < rows; i0 += 16) {
+        __half x[16], y[16];   // (all of them first: no load passes a store)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint8_t* src = stage_gen + (i0 + i) * 128 + ((lane * 2) & 15);
+          x[i] = *reinterpret_cast<const __half*>(src + (((lane >> 3) ^ (i & 7)) << 4));
+          y[i] = *reinterpret_cast<const __half*>(src + (((4 + (lane >> 3)) ^ (i & 7)) << 4));
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i, out += p.ldc) {
+          if (i0 + i < rows && cols > 0) out[0] = x[i];
+          if (i0 + i < rows && cols > 32) out[32] = y[i];
+        }
       }
       __syncwarp();
     }
   }
 }
 
-// Everything else: fp32, C added, stochastic rounding.
-template <int kCols, typename F>
-__device__ __forceinline__ void out_any(const OutParams& p, const CUtensorMap* mapC, uint32_t taddr, uint32_t stage, uint8_t* stage_gen,
-                                        int m0, int n0, F release) {
+// Everything else: fp32, C added, stochastic rounding. 32 columns at a time go through the staged box in fp32, so that
+// neighbouring lanes read and write neighbours of C, and what C held in all 32 rows is on its way together. (With a row per lane
+// each access touched 32 sectors, and the loads of one chunk waited for the stores of the last: with C added, 5664 x 546 x 1698
+// 28.5 -> 15.5 us and 4096 x 9216 x 128 160 -> 48, against 8.4 and 20 without.) First, rows of C at any address: a number per lane.
+template <int kCols, typename E, typename F>
+__device__ __forceinline__ void out_odd(const OutParams& p, uint32_t taddr, uint8_t* stage_gen, int m0, int n0, F release) {
   const int lane = threadIdx.x & 31;
-  const long long row = m0 + lane;
-  const bool f32 = p.out_f32;
-  const int esz = f32 ? 4 : 2;
 #pragma unroll 1
   for (int c = 0; c < kCols; c += 32) {
+    const int rows = min(32, p.M - m0), col = n0 + c + lane;
+    E* out = static_cast<E*>(p.C) + m0 * p.ldc + col;
+    OldBits<E> old[32];
+    const int held = p.ea.beta != 0.0f && col < p.N ? rows : 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) old[i] = i < held ? reinterpret_cast<const OldBits<E>*>(out)[i * p.ldc] : OldBits<E>(0);
     uint32_t r[32];
     tc_ld_32x32(taddr + c, r);
     tc_wait_ld();
@@ -93,56 +125,125 @@ __device__ __forceinline__ void out_any(const OutParams& p, const CUtensorMap* m
       release();
     }
     if (m0 >= p.M || n0 + c >= p.N) continue;
-    // into this lane's row of the staged box: 32 columns are 64 bytes of fp16 (half a row) or 128 of fp32
-    const int at = f32 ? 0 : (c & 32) * 2;
-    if (at == 0) {             // (the box before must have left)
+#pragma unroll
+    for (int g = 0; g < 8; ++g)
+      *reinterpret_cast<uint4*>(stage_gen + lane * 128 + ((g ^ (lane & 7)) << 4)) = make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
+    __syncwarp();
+    auto at = [&](int i) {
+      return *reinterpret_cast<const float*>(stage_gen + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4);
+    };
+    if (sizeof(E) == 2 && p.ea.sr_bits) {
+      // eight neighbours at a time, which share their random bits
+      const int first = n0 + c + (lane & 3) * 8;
+#pragma unroll 1
+      for (int i = lane >> 2; i < rows && first < p.N; i += 8) {
+        const uint8_t* src = stage_gen + i * 128;
+        const float4 x = *reinterpret_cast<const float4*>(src + (((lane & 3) * 2 ^ (i & 7)) << 4));
+        const float4 y = *reinterpret_cast<const float4*>(src + (((lane & 3) * 2 + 1 ^ (i & 7)) << 4));
+        E* row = static_cast<E*>(p.C) + (m0 + i) * p.ldc;
+        epi_store8_call<false>(p.ea, x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, row, row, first,
+                               static_cast<unsigned long long>(m0 + i) * p.N + first, min(8, p.N - first), false);
+      }
+    } else if (col < p.N) {
+      float x[32];             // (all of them first: no load passes a store)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = at(i);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < rows) epi_store_nearest(p.ea, x[i], to_f32(old[i]), out + i * p.ldc);
+    }
+    __syncwarp();
+  }
+}
+
+// The same in rows of whole aligned vectors: one per lane, 4 (fp16) or 8 (fp32) lanes on a row. What is fp32 leaves by TMA, from
+// the box as it is (4096 x 9216 x 128 57.8 -> 45 us).
+template <int kCols, typename E, typename F>
+__device__ __forceinline__ void out_even(const OutParams& p, const CUtensorMap* mapC, uint32_t taddr, uint32_t stage, uint8_t* stage_gen,
+                                         int m0, int n0, F release) {
+  constexpr int kPer = 16 / sizeof(E), kLanes = 32 / kPer, kStep = 32 / kLanes;      // numbers of a lane, lanes and rows of an access
+  const int lane = threadIdx.x & 31, row0 = lane / kLanes, col0 = lane % kLanes * kPer;
+#pragma unroll 1
+  for (int c = 0; c < kCols; c += 32) {
+    const int col = n0 + c + col0;
+    const int rows = col < p.N ? p.M - m0 - row0 : 0;      // of this lane, one in kStep
+    E* out = static_cast<E*>(p.C) + (m0 + row0) * p.ldc + col;
+    uint4 old[kLanes];
+#pragma unroll
+    for (int t = 0; t < kLanes; ++t)
+      old[t] = p.ea.beta != 0.0f && kStep * t < rows ? *reinterpret_cast<const uint4*>(out + kStep * t * p.ldc) : make_uint4(0u, 0u, 0u, 0u);
+    uint32_t r[32];
+    tc_ld_32x32(taddr + c, r);
+    tc_wait_ld();
+    if (c + 32 >= kCols) {     // the accumulator has been read
+      tc_fence_before();
+      __syncwarp();
+      release();
+    }
+    if (m0 >= p.M || n0 + c >= p.N) continue;
+    if (kPer == 4) {           // (the box before must have left)
       if (lane == 0) tma_store_wait_read<0>();
       __syncwarp();
     }
-    uint8_t* dst = stage_gen + lane * 128;
-    const uint32_t sw = (lane & 7) << 4;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float v[8];
+    for (int g = 0; g < 8; ++g)
+      *reinterpret_cast<uint4*>(stage_gen + lane * 128 + ((g ^ (lane & 7)) << 4)) = make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[8 * g + i]);
-      uint4 lo, hi;
-      const int col = n0 + c + 8 * g;
-      const int nvalid = row < p.M ? max(0, min(8, p.N - col)) : 0;
-      const unsigned long long lin = static_cast<unsigned long long>(row) * p.N + col;
-      const void* oldp = nvalid > 0 ? static_cast<const uint8_t*>(p.C) + (row * p.ldc + col) * esz : nullptr;
-      if (f32) epi_pack8<true>(p.ea, v, oldp, lin, lo, hi, max(nvalid, 1));
-      else epi_pack8<false>(p.ea, v, oldp, lin, lo, hi, max(nvalid, 1));
-      if (f32) {
-        *reinterpret_cast<uint4*>(dst + ((32 * g) ^ sw)) = lo;
-        *reinterpret_cast<uint4*>(dst + ((32 * g + 16) ^ sw)) = hi;
+    for (int t = 0; t < kLanes; ++t) {
+      if (kStep * t >= rows) continue;
+      const int row = row0 + kStep * t;
+      auto piece = [&](int h) { return reinterpret_cast<float4*>(stage_gen + row * 128 + (((col0 / 4 + h) ^ (row & 7)) << 4)); };
+      if constexpr (kPer == 8) {
+        const float4 x = *piece(0), y = *piece(1);
+        float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        uint4 w, same;
+        epi_pack8<false>(p.ea, v, &old[t], static_cast<unsigned long long>(m0 + row) * p.N + col, w, same);
+        *reinterpret_cast<uint4*>(out + kStep * t * p.ldc) = w;
       } else {
-        *reinterpret_cast<uint4*>(dst + ((at + 16 * g) ^ sw)) = lo;
+        float4 x = *piece(0);
+        float* v = &x.x;
+        const uint32_t o[4] = {old[t].x, old[t].y, old[t].z, old[t].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = epi_scale(p.ea, v[i]);
+          if (p.ea.beta != 0.0f) v[i] = fmaf(p.ea.beta, __uint_as_float(o[i]), v[i]);
+        }
+        *piece(0) = x;
       }
     }
-    if (!f32 && at == 0 && n0 + c + 32 < p.N) continue;    // the other half of the box comes next
-    const int col0 = n0 + (f32 ? c : c & ~63);
-    if (p.store) {
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_5d(mapC, stage, col0, m0, 0, 0, 0);
-        tma_store_commit();
-      }
-    } else {
-      __syncwarp();
-      const int rows = min(32, p.M - m0), cols = min(128 / esz, p.N - col0);
-      for (int i = 0; i < rows; ++i) {
-        uint8_t* out = static_cast<uint8_t*>(p.C) + ((m0 + i) * p.ldc + col0) * esz;
-        for (int j = lane; j < cols; j += 32) {
-          const uint8_t* src = stage_gen + i * 128 + (((j * esz) & 112) ^ ((i & 7) << 4)) + ((j * esz) & 15);
-          if (f32) reinterpret_cast<float*>(out)[j] = *reinterpret_cast<const float*>(src);
-          else reinterpret_cast<__half*>(out)[j] = *reinterpret_cast<const __half*>(src);
-        }
-      }
-      __syncwarp();
+    if (kPer == 4) fence_async_smem();
+    __syncwarp();
+    if (kPer == 4 && lane == 0) {
+      tma_store_5d(mapC, stage, n0 + c, m0, 0, 0, 0);
+      tma_store_commit();
     }
   }
+}
+
+// Which of these a kernel has: the lean form, and the others in fp16 or fp32. (One kernel with all of them was larger than the
+// instruction cache: 1001 x 4097 x 125 in fp32 15.6 -> 19.8 us.)
+enum OutForm { kOutLean, kOutF16, kOutF32 };
+inline OutForm out_form(const OutParams& out) {
+  return out.out_f32 ? kOutF32 : out.ea.beta == 0.0f && out.ea.sr_bits == 0 ? kOutLean : kOutF16;
+}
+template <int kForm, int kCols, typename F>
+__device__ __forceinline__ void out_tile(const OutParams& p, const CUtensorMap* mapC, uint32_t taddr, uint32_t stage, uint8_t* stage_gen,
+                                         int m0, int n0, F release) {
+  using E = std::conditional_t<kForm == kOutF32, float, __half>;
+  if constexpr (kForm == kOutLean) out_lean<kCols>(p, mapC, taddr, stage, stage_gen, m0, n0, release);
+  else if (p.store) out_even<kCols, E>(p, mapC, taddr, stage, stage_gen, m0, n0, release);
+  else out_odd<kCols, E>(p, taddr, stage_gen, m0, n0, release);
+}
+
+// What an fp32 C holds in 32 rows x kCols columns to the L2 cache, a tile before it is needed: 4096 x 9216 x 128 with C added
+// 90 -> 76 us (fp16, of half as many bytes, was slower with it, 48 -> 52).
+template <int kForm, int kCols>
+__device__ __forceinline__ void out_ahead(const OutParams& p, int m0, int n0) {
+  const int row = m0 + (threadIdx.x & 31);
+  if (kForm != kOutF32 || p.ea.beta == 0.0f || row >= p.M || n0 >= p.N) return;
+  const float* at = static_cast<const float*>(p.C) + row * p.ldc + n0;
+  for (int c = 0; c < min(kCols, p.N - n0); c += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + c));
 }
 
 }  // namespace ngb

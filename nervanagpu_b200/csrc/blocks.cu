@@ -61,8 +61,17 @@ struct Raw {
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
+      // (the end of a row: whole vectors as far as they go)
+      constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-      for (int i = 0; i < kCount; ++i) at()[i] = i < n ? p[i] : T(0.0f);
+      for (int i = 0; i < kVecs; ++i) {
+        if ((i + 1) * kPer <= n) {
+          v[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+#pragma unroll
+          for (int j = i * kPer; j < (i + 1) * kPer; ++j) at()[j] = j < n ? p[j] : zero_of<T>();
+        }
+      }
     }
   }
   __device__ __forceinline__ void store(T* p, int n, bool wide) const {
@@ -77,9 +86,17 @@ struct Raw {
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
     } else {
+      constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-      for (int i = 0; i < kCount; ++i)
-        if (i < n) p[i] = at()[i];
+      for (int i = 0; i < kVecs; ++i) {
+        if ((i + 1) * kPer <= n) {
+          reinterpret_cast<uint4*>(p)[i] = v[i];
+        } else {
+#pragma unroll
+          for (int j = i * kPer; j < (i + 1) * kPer; ++j)
+            if (j < n) p[j] = at()[j];
+        }
+      }
     }
   }
 };
@@ -141,7 +158,7 @@ __device__ __forceinline__ void warp_move(T* base, long long so, long long o_fir
       const int e = i * 32 + lane, l = l_first + (e & (run - 1));
       const long long o = o_first + (e >> (7 + per_row));
       const bool live = o < outer && l < inner;
-      if (!kStore) stage[e] = live ? base[o * so + l] : T(0.0f);
+      if (!kStore) stage[e] = live ? base[o * so + l] : zero_of<T>();
       else if (live) base[o * so + l] = stage[e];
     }
     return;
@@ -159,7 +176,7 @@ __device__ __forceinline__ void warp_move(T* base, long long so, long long o_fir
         if (j * 32 < n) p[j * 32] = s[j * 32];
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j * 32] = j * 32 < n ? p[j * 32] : T(0.0f);
+      for (int j = 0; j < 4; ++j) s[j * 32] = j * 32 < n ? p[j * 32] : zero_of<T>();
     }
   }
 }
@@ -365,7 +382,7 @@ __global__ void __launch_bounds__(256) relu_mask_rows_kernel(BlockView q, PlainV
       r.load(p, n, a.wide);
 #pragma unroll
       for (int i = 0; i < kLane; ++i)
-        if (off >> i & 1u) r.at()[i] = T(0.0f);
+        if (off >> i & 1u) r.at()[i] = zero_of<T>();
       r.store(p, n, a.wide);
     } else {
       // zeros, one number per lane and access, in the order of warp_move
@@ -377,7 +394,7 @@ __global__ void __launch_bounds__(256) relu_mask_rows_kernel(BlockView q, PlainV
           const int e = i * 32 + lane, l = l_warp + (e & ((16 << log_tx) - 1));
           const long long row = o_warp + (e >> (4 + log_tx));
           const uint32_t mask = __shfl_sync(0xffffffffu, off, i * 2 + (lane >> 4));
-          if ((mask >> (lane & 15) & 1u) && row < q.outer && l < q.inner) a.p[row * a.so + l] = T(0.0f);
+          if ((mask >> (lane & 15) & 1u) && row < q.outer && l < q.inner) a.p[row * a.so + l] = zero_of<T>();
         }
         continue;
       }
@@ -389,7 +406,7 @@ __global__ void __launch_bounds__(256) relu_mask_rows_kernel(BlockView q, PlainV
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t mask = __shfl_sync(0xffffffffu, off, i * 8 + j * 2 + (lane >> 4));
-          if ((mask >> (lane & 15) & 1u) && row < q.outer && l + j * 32 < q.inner) p[j * 32] = T(0.0f);
+          if ((mask >> (lane & 15) & 1u) && row < q.outer && l + j * 32 < q.inner) p[j * 32] = zero_of<T>();
         }
       }
     }
@@ -399,8 +416,8 @@ __global__ void __launch_bounds__(256) relu_mask_rows_kernel(BlockView q, PlainV
 // ---- strided form --------------------------------------------------------------------------------------
 // A CTA takes 64 outer rows x 4 blocks: half a tile of 4-bit scales, and 32 to 128 neighbouring bytes of codes per outer
 // row, so that a quantisation leaves in whole sectors through shared memory. A warp has one block, a lane two outer
-// rows: kVec (the outer axis is the contiguous one, in aligned pairs): neighbours, in one access; else 32
-// apart, one by one. (Four rows per lane were faster for large matrices by 5 % and took 6.7 us instead of 2.9 for a
+// rows: neighbours, in one access, where the outer axis is the contiguous one in aligned pairs (a quantisation
+// from fp16: at any address; words put together for the way back were slower than numbers, 16.8 to 13.9 us); else 32 apart, one by one. (Four rows per lane were faster for large matrices by 5 % and took 6.7 us instead of 2.9 for a
 // minibatch of 9216 x 128, with too few warps to hide their latency.)
 constexpr int kStridedThreads = 128;
 constexpr int kStridedRows = 64;
@@ -448,14 +465,16 @@ __device__ __forceinline__ void top_of_pairs(const uint2 (&raw)[kN], uint32_t (&
     top[1] = max(top[1], raw[i].y & 0x7fffffffu);
   }
 }
+// How the outer rows lie in memory: anyhow; as neighbours in aligned pairs; as neighbours (fp16) at any address.
+enum StridedForm { kStridedAny, kStridedPairs, kStridedShifted };
 // row of the tile that is this lane's j-th
-template <bool kVec>
+template <bool kNeighbours>
 __device__ __forceinline__ int strided_row(int j) {
   const int lane = threadIdx.x & 31;
-  return kVec ? 2 * lane + j : lane + 32 * j;
+  return kNeighbours ? 2 * lane + j : lane + 32 * j;
 }
 
-template <typename T, int kFmt, bool kVec>
+template <typename T, int kFmt, int kForm>
 __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(BlockView q, PlainView<const T> a, int early, int blocks) {
   NG_DEPENDENT_PROLOGUE(early);
   using F = BlockFormat<kFmt>;
@@ -470,8 +489,35 @@ __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(Block
     const int n = q.inner - b * F::kBlock;          // numbers of the block that exist
     typename P::Vec raw[F::kBlock];
     const T* p = a.p + static_cast<long long>(b) * F::kBlock * a.sl;
-    const int r0 = o0 + strided_row<kVec>(0), r1 = o0 + strided_row<kVec>(1);
-    if (kVec) {
+    const int r0 = o0 + strided_row<kForm != kStridedAny>(0), r1 = o0 + strided_row<kForm != kStridedAny>(1);
+    if constexpr (kForm == kStridedShifted) {
+      // Numbers 2 lane and 2 lane + 1 of each run, from aligned words: where a run starts in the middle of one, a lane
+      // loads the word behind that, and its first number is the second of the lane below. The first number of such a run,
+      // and the last of one that ends in the middle of a word, are loaded by a lane per run. (4097 x 125 from 2.7 to 2.3
+      // us, 6168 x 3385 from 15.5 to 11.8. Two loads into one register, for either case, would wait for each other: 4.1.)
+      const int lane = threadIdx.x & 31, last = q.outer - 1 - o0;
+      const T* run = p + o0;
+      // which runs start in the middle of a word: the even ones, the odd ones
+      const int odd[2] = {static_cast<int>(reinterpret_cast<uintptr_t>(run) >> 1) & 1,
+                          static_cast<int>(reinterpret_cast<uintptr_t>(run + a.sl) >> 1) & 1};
+      const bool whole[2] = {2 * lane + odd[0] < last, 2 * lane + odd[1] < last};
+      uint32_t ends = 0u;         // first and last number of run `lane`
+      if (lane < min(n, F::kBlock)) {
+        const unsigned short* at = reinterpret_cast<const unsigned short*>(run + lane * a.sl);
+        ends = at[0] | static_cast<uint32_t>(at[min(last, kStridedRows - 1)]) << 16;
+      }
+      const T* at = run + 2 * lane;
+#pragma unroll
+      for (int i = 0; i < F::kBlock; ++i, at += a.sl)
+        raw[i] = i < n && whole[i & 1] ? *reinterpret_cast<const uint32_t*>(at + odd[i & 1]) : 0u;
+#pragma unroll
+      for (int i = 0; i < F::kBlock; ++i) {
+        const uint32_t e = __shfl_sync(0xffffffffu, ends, i);
+        if (2 * lane + odd[i & 1] == last) raw[i] = e >> 16;
+        const uint32_t below = __shfl_up_sync(0xffffffffu, raw[i], 1);
+        if (odd[i & 1]) raw[i] = __byte_perm(lane == 0 ? e << 16 : below, raw[i], 0x5432);
+      }
+    } else if (kForm == kStridedPairs) {
       const T* p0 = p + r0;
       if (r0 < q.outer && n >= F::kBlock) {
 #pragma unroll
@@ -479,7 +525,7 @@ __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(Block
       } else {
 #pragma unroll
         for (int i = 0; i < F::kBlock; ++i) {
-          raw[i] = P::of(T(0.0f), T(0.0f));
+          raw[i] = P::of(zero_of<T>(), zero_of<T>());
           if (r0 < q.outer && i < n) raw[i] = *reinterpret_cast<const typename P::Vec*>(p0 + i * a.sl);
         }
       }
@@ -487,13 +533,13 @@ __global__ void __launch_bounds__(kStridedThreads) quantize_strided_kernel(Block
       const T *p0 = p + r0 * a.so, *p1 = p + r1 * a.so;
 #pragma unroll
       for (int i = 0; i < F::kBlock; ++i)
-        raw[i] = P::of(r0 < q.outer && i < n ? p0[i * a.sl] : T(0.0f), r1 < q.outer && i < n ? p1[i * a.sl] : T(0.0f));
+        raw[i] = P::of(r0 < q.outer && i < n ? p0[i * a.sl] : zero_of<T>(), r1 < q.outer && i < n ? p1[i * a.sl] : zero_of<T>());
     }
     uint32_t top[2];
     top_of_pairs(raw, top);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int row = strided_row<kVec>(j);
+      const int row = strided_row<kForm != kStridedAny>(j);
       const BlockScale s = block_scale<kFmt, sizeof(T) == 2>(top[j], q.t);
       uint8_t* dst = codes + row * S::kPitch + which * S::kBytes;
 #pragma unroll
@@ -593,7 +639,7 @@ __global__ void __launch_bounds__(256) relu_mask_strided_kernel(BlockView q, Pla
     const int n = q.inner - b * 32;
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      if (i < n && not_positive(w[i / 4] >> (8 * (i & 3)) & 0xffu)) p[i * a.sl] = T(0.0f);
+      if (i < n && not_positive(w[i / 4] >> (8 * (i & 3)) & 0xffu)) p[i * a.sl] = zero_of<T>();
   }
 }
 
@@ -667,6 +713,10 @@ bool aligned_pairs(const BlockView& q, const PlainView<T>& a) {
   return a.so == 1 && q.outer % 2 == 0 && a.sl % 2 == 0 && (reinterpret_cast<uintptr_t>(a.p) & (2 * sizeof(T) - 1)) == 0;
 }
 
+// neighbours to be quantised from any address (fp32 numbers, one per lane, fill an access as it is)
+template <typename T>
+constexpr int kNeighbours = sizeof(T) == 2 ? kStridedShifted : kStridedAny;
+
 template <typename T, int kFmt>
 int quantize_one(DeviceCtx* c, const BlockView& q, PlainView<const T> a, cudaStream_t stream) {
   const int blocks = (q.inner + BlockFormat<kFmt>::kBlock - 1) / BlockFormat<kFmt>::kBlock;
@@ -679,8 +729,9 @@ int quantize_one(DeviceCtx* c, const BlockView& q, PlainView<const T> a, cudaStr
     else rc = launch(c, quantize_rows_kernel<T, kFmt, 2>, g.grid, g.block, stream, q, a);
   } else {
     const dim3 grid((q.outer + kStridedRows - 1) / kStridedRows, std::min((blocks + 3) / 4, 65535));
-    if (aligned_pairs(q, a)) rc = launch(c, quantize_strided_kernel<T, kFmt, true>, grid, dim3(kStridedThreads), stream, q, a, blocks);
-    else rc = launch(c, quantize_strided_kernel<T, kFmt, false>, grid, dim3(kStridedThreads), stream, q, a, blocks);
+    if (aligned_pairs(q, a)) rc = launch(c, quantize_strided_kernel<T, kFmt, kStridedPairs>, grid, dim3(kStridedThreads), stream, q, a, blocks);
+    else if (sizeof(T) == 2 && a.so == 1) rc = launch(c, quantize_strided_kernel<T, kFmt, kNeighbours<T>>, grid, dim3(kStridedThreads), stream, q, a, blocks);
+    else rc = launch(c, quantize_strided_kernel<T, kFmt, kStridedAny>, grid, dim3(kStridedThreads), stream, q, a, blocks);
   }
   return rc;
 }

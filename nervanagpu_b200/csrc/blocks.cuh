@@ -67,6 +67,15 @@ struct BlockFormat {
   }
 };
 
+// Zero as bits. (A conversion of 0.0f is an instruction of its own that the compiler does not move: `p ? load : zero` became
+// a branch, and the loads beside it waited for one another.)
+template <typename T>
+__device__ __forceinline__ T zero_of();
+template <>
+__device__ __forceinline__ float zero_of<float>() { return 0.0f; }
+template <>
+__device__ __forceinline__ __half zero_of<__half>() { return __ushort_as_half(0); }
+
 // For a kernel that gives up: copies and MMAs in flight must end before the CTA may, and do so in microseconds, but the
 // barriers that would tell may never complete, other arrivals missing. So this waits for time.
 __device__ __forceinline__ void wait_for_strays() {

@@ -20,7 +20,6 @@ int plain_map(CUtensorMap* map, const void* base, long long rows, long long cols
 // Output stage of a product: its parameters, the boxes it stores, and whether its lean form will do.
 OutParams make_out(void* C, int m, int n, int ldc, int out_f32, const EpiArgs& ea);
 int out_map(CUtensorMap* map, const OutParams& out);
-inline bool out_is_lean(const OutParams& out) { return !out.out_f32 && out.ea.beta == 0.0f && out.ea.sr_bits == 0; }
 // The product of block_dot_pair.cu: two 4-bit matrices of more than 64 outer rows each.
 int run_block_dot_pair(DeviceCtx* c, const BlockView& a, const BlockView& b, bool nv, const OutParams& out, cudaStream_t stream);
 // The product of block_dot_f16.cu, from checked operands.
