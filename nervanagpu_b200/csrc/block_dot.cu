@@ -7,10 +7,7 @@
 // per 512 bytes takes these to tensor memory.
 //
 // A CTA computes a tile of 128 rows x kN columns (kN from 16 to 128). Few tiles are split along the sum over the
-// CTAs of a thread-block cluster. Each of them then gets a share of the tile's rows from all the others by bulk copies
-// between their shared memories and adds them up in the order of the partitions: one launch, no scratch memory, the
-// same bits every time. (Fetched by loads from the others' shared memory instead, the partial tiles of 4096 x 128 x
-// 9216 took 3.8 us of 12.2.)
+// CTAs of a thread-block cluster (block_share.cuh).
 //
 //   warp 0     producer (the first loads leave before tensor memory is allocated)
 //   warp 1     tensor memory, scale copies and MMAs, by one thread
@@ -21,6 +18,7 @@
 #include <type_traits>
 
 #include "block_mma.cuh"
+#include "block_share.cuh"
 #include "blocks.h"
 
 namespace ngb {
@@ -40,9 +38,8 @@ struct DotTile {
   static constexpr uint32_t kCodesB = kN * 128u;
   static constexpr uint32_t kScales = kScaleTiles * kScaleTile;      // of 128 rows
   static constexpr uint32_t kStageBytes = (kCodesA + kCodesB + 2 * kScales + 1023u) & ~1023u;
-  // partial tiles in shared memory: rows of kN + 4 floats, so that lanes in successive rows meet different banks
-  static constexpr int kPitch = kN + 4;
-  static constexpr uint32_t kParts = 128u * kPitch * 4u;
+  static constexpr int kPitch = kSharePitch<kN>;
+  static constexpr uint32_t kParts = kShareTile<kN>;
   static constexpr int kRoom = static_cast<int>((kDotSmemLimit - 1024u - kDotCtrl - kParts) / kStageBytes);
   static constexpr int kStages = kRoom < kDotStages ? kRoom : kDotStages;
   // tensor memory: the accumulator, then two buffers of scales, A's before B's
@@ -56,7 +53,6 @@ struct DotTile {
 };
 
 struct DotParams {
-  int M, N;                  // rows of the two operands
   int num_kb;
   int tiles_m;
   const uint8_t *ca, *cb;    // codes
@@ -64,11 +60,8 @@ struct DotParams {
   long long pitch_a, pitch_b;    // bytes of a row of tiles of codes
   int tile_a;                // bytes of a tile of A's codes
   long long spitch;          // bytes of a row of scale tiles (the same for both: one format, one length)
-  void* C;
-  long long ldc;
-  int out_f32, vec_ok;
+  ShareOut out;
   int swapped;               // the tile's rows are C's columns
-  EpiArgs ea;
   int* status;
   unsigned long long wait_limit_ns;
 };
@@ -82,22 +75,6 @@ __device__ __forceinline__ void tc_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-// bytes of this CTA's shared memory to another's (or its own), counted on a barrier there
-__device__ __forceinline__ void bulk_push(uint32_t dst_cluster, uint32_t src, uint32_t bytes, uint32_t bar_cluster) {
-  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst_cluster),
-               "r"(src), "r"(bytes), "r"(bar_cluster)
-               : "memory");
-}
-// (relaxed: neither arrival publishes memory. The barriers that the first tells of are fenced when they are made, the second
-// only says that nobody reads this CTA's tile any more. As a release each took half a microsecond.)
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t n;
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
-  return n;
-}
-
 template <int kN, bool kNv>
 __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_constant__ DotParams p) {
   using T = DotTile<kN, kNv>;
@@ -117,9 +94,7 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
   const int m0 = (tile % p.tiles_m) * 128, n0 = (tile / p.tiles_m) * kN;
   const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * rank / splits);
   const int count = static_cast<int>(static_cast<long long>(p.num_kb) * (rank + 1) / splits) - kb0;
-  // this CTA's share of the tile
-  const int rows = 128 / splits, r0 = rank * rows;
-  const uint32_t share_bytes = static_cast<uint32_t>(rows) * T::kPitch * 4u;
+  const uint32_t share_bytes = T::kParts / splits;
 
   // k-block i of this partition into slot i % kStages
   const int rt = m0 / 128, ct = n0 / 128;
@@ -236,139 +211,15 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
     fence_async_smem();      // (the parts leave by bulk copies)
   }
   __syncthreads();
-  if (splits > 1) {
-    cluster_wait();          // (with everybody's arrival long ago: the barriers that the parts count on exist)
-    if (warp == 0 && lane > 0 && lane < splits) {
-      const int to = (rank + lane) % splits;
-      bulk_push(map_to_cta(parts + rank * share_bytes, to), ring + to * share_bytes, share_bytes, map_to_cta(part_bar, to));
-    }
-    __syncwarp();
-  }
+  if (splits > 1) share_push(ring, parts, share_bytes, rank, splits, part_bar);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, T::kCols);
   }
-  if (splits > 1) {
-    if (!mbar_wait(part_bar, 0, abort_flag, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns)) {
-      int none = 0;          // given up: the parts come all the same, those of a CTA that gave up too, and later than here maybe
-      mbar_wait(part_bar, 0, &none, p.status, NG_DEV_TIMEOUT_EPILOGUE, p.wait_limit_ns);
-    }
-    __syncwarp();
-    cluster_arrive();        // (with everybody's: all parts have arrived, nobody's tile is read any more)
-    __syncthreads();         // the abort flag is final
-  }
-
-  // The sum over the partitions, in their order, and the output stage. (When a partition gave up, the others' shares
-  // hold what was there: the status word tells.)
-  const bool whole = !p.swapped && p.vec_ok;        // rows of whole aligned vectors of C
-  const int live = max(0, min(rows, p.M - m0 - r0));
-  const float* own = reinterpret_cast<const float*>(ring_gen) + r0 * T::kPitch;
-  const float* others = reinterpret_cast<const float*>(ring_gen + (parts - ring));
-  auto part = [&](int s) { return s == rank ? own : others + s * rows * T::kPitch; };
-  auto sum4 = [&](auto n, int off) {
-    constexpr int kParts = decltype(n)::value;
-    float4 x[kParts];
-#pragma unroll
-    for (int s = 0; s < kParts; ++s) x[s] = *reinterpret_cast<const float4*>(part(s) + off);
-#pragma unroll
-    for (int s = 1; s < kParts; ++s) {
-      x[0].x += x[s].x; x[0].y += x[s].y; x[0].z += x[s].z; x[0].w += x[s].w;
-    }
-    return x[0];
-  };
-  auto store_whole = [&](auto n) {
-    for (int i = threadIdx.x; i < live * (kN / 8); i += kDotThreads) {
-      const int r = i / (kN / 8), c = (i % (kN / 8)) * 8;
-      const int col = n0 + c;
-      const long long row = m0 + r0 + r;
-      if (col >= p.N) continue;
-      const float4 x = sum4(n, r * T::kPitch + c), y = sum4(n, r * T::kPitch + c + 4);
-      float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-      const unsigned long long lin = static_cast<unsigned long long>(row) * p.N + col;
-      const int nvalid = min(8, p.N - col);
-      uint8_t* crow = static_cast<uint8_t*>(p.C) + row * p.ldc * (p.out_f32 ? 4 : 2);
-      if (p.out_f32) epi_store8<true>(p.ea, v, crow, crow, col, lin, nvalid, true);
-      else epi_store8<false>(p.ea, v, crow, crow, col, lin, nvalid, true);
-    }
-  };
-  auto sum_in_place = [&](auto n) {
-    for (int i = threadIdx.x; i < live * (kN / 4); i += kDotThreads) {
-      const int off = i / (kN / 4) * T::kPitch + i % (kN / 4) * 4;
-      *reinterpret_cast<float4*>(const_cast<float*>(own) + off) = sum4(n, off);
-    }
-    __syncthreads();
-  };
-#define NG_BY_PARTS(call, from)                                                 \
-  switch (splits) {                                                             \
-    case 1: if (from <= 1) call(std::integral_constant<int, 1>()); break;       \
-    case 2: call(std::integral_constant<int, 2>()); break;                      \
-    case 4: call(std::integral_constant<int, 4>()); break;                      \
-    default: call(std::integral_constant<int, 8>()); break;                     \
-  }
-  if (*abort_flag) {
-  } else if (whole) {
-    NG_BY_PARTS(store_whole, 1)
-  } else {
-    // C's rows are at any address, or run down the tile: one output per lane and access, neighbours in lanes
-    NG_BY_PARTS(sum_in_place, 2)
-    const int cols = min(kN, p.N - n0);
-    const int runs = p.swapped ? cols : live, len = p.swapped ? live : cols;       // rows of C that have some, and how many
-    const int run_step = p.swapped ? 1 : T::kPitch, step = p.swapped ? T::kPitch : 1;
-    const long long row0 = p.swapped ? n0 : m0 + r0, col0 = p.swapped ? m0 + r0 : n0;
-    const int width = p.swapped ? p.M : p.N;
-    auto rows_of = [&](auto* base) {
-      using E = std::remove_pointer_t<decltype(base)>;
-      constexpr int kWarps = kDotThreads / 32;
-      if (sizeof(E) == 2 && p.ea.sr_bits) {
-        // eight neighbours at a time, which share their random bits
-        const int eights = (len + 7) / 8;
-#pragma unroll 1
-        for (int i = threadIdx.x; i < runs * eights; i += kDotThreads) {
-          const int u = i / eights, c = i % eights * 8;
-          const float* src = own + u * run_step + c * step;
-          float v[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = c + j < len ? src[j * step] : 0.0f;
-          E* row = base + (row0 + u) * p.ldc;
-          epi_store8_call<false>(p.ea, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], row, row, static_cast<int>(col0) + c,
-                                 static_cast<unsigned long long>(row0 + u) * width + col0 + c, min(8, len - c), false);
-        }
-        return;
-      }
-      // (what C held in four rows is on its way together: one by one, 128 rows of a tile took 10 us)
-#pragma unroll 1
-      for (int u0 = warp; u0 < runs && p.ea.beta != 0.0f; u0 += 4 * kWarps) {
-        OldBits<E> old[4][4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int u = u0 + r * kWarps, i = j * 32 + lane;
-            old[r][j] = u < runs && i < len ? reinterpret_cast<const OldBits<E>*>(base)[(row0 + u) * p.ldc + col0 + i] : OldBits<E>(0);
-          }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int u = u0 + r * kWarps;
-          if (u >= runs) break;
-          E* out = base + (row0 + u) * p.ldc + col0 + lane;
-          const float* src = own + u * run_step + lane * step;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j * 32 + lane < len) epi_store_nearest(p.ea, src[j * 32 * step], to_f32(old[r][j]), out + j * 32);
-        }
-      }
-      for (int u = warp; u < runs && p.ea.beta == 0.0f; u += kWarps) {
-        E* out = base + (row0 + u) * p.ldc + col0 + lane;
-        const float* src = own + u * run_step + lane * step;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j * 32 + lane < len) epi_put(epi_scale(p.ea, src[j * 32 * step]), out + j * 32);
-      }
-    };
-    if (p.out_f32) rows_of(static_cast<float*>(p.C));
-    else rows_of(static_cast<__half*>(p.C));
-  }
-#undef NG_BY_PARTS
+  if (splits > 1) share_wait(part_bar, abort_flag, p.status, p.wait_limit_ns);
+  if (!*abort_flag)
+    share_store<kN, kDotThreads>(p.out, p.swapped, reinterpret_cast<float*>(ring_gen), reinterpret_cast<const float*>(ring_gen + (parts - ring)),
+                                 splits, rank, m0, n0);
   __syncwarp();
   if (splits > 1) cluster_wait();
 }
@@ -376,7 +227,7 @@ __global__ void __launch_bounds__(kDotThreads, 1) block_dot_kernel(const __grid_
 template <int kN, bool kNv>
 int launch_dot(DeviceCtx* c, DotParams& p, int splits, cudaStream_t stream) {
   using T = DotTile<kN, kNv>;
-  const long long tiles = static_cast<long long>(p.tiles_m) * ((p.N + kN - 1ll) / kN);
+  const long long tiles = static_cast<long long>(p.tiles_m) * ((p.out.N + kN - 1ll) / kN);
   if (tiles * splits > 0x7fffffffll) return fail(NG_ERR_TOO_LARGE, "too many tiles");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
@@ -401,6 +252,18 @@ int launch_dot(DeviceCtx* c, DotParams& p, int splits, cudaStream_t stream) {
   NG_CHECK_LAUNCH();
   return NG_OK;
 }
+
+int pad_columns(int n) { return n <= 64 ? block_tile_rows(n) : (n + 127) / 128 * 128; }
+
+int check_output(const void* C, int ldc, int n, int sr_bits, int out_f32) {
+  if (!C) return fail(NG_ERR_INVALID_ARG, "null operand");
+  if (ldc < n) return fail(NG_ERR_INVALID_ARG, "leading dimension too small");
+  if (sr_bits < 0 || sr_bits > 10) return fail(NG_ERR_INVALID_ARG, "stochastic rounding keeps 1..10 mantissa bits");
+  if (sr_bits && out_f32) return fail(NG_ERR_UNSUPPORTED, "stochastic rounding is to fp16");
+  return NG_OK;
+}
+
+}  // namespace
 
 // CTAs that run at the same time in clusters of 2^log: larger ones leave SMs of their GPCs over (132 in clusters of 4, 120
 // in clusters of 8; 2048 x 128 x 2048 as 128 CTAs in clusters of 8 took two rounds, 12.0 us).
@@ -429,18 +292,6 @@ int cluster_room(const DeviceCtx* c, int log) {
   return n;
 }
 
-int pad_columns(int n) { return n <= 64 ? block_tile_rows(n) : (n + 127) / 128 * 128; }
-
-int check_output(const void* C, int ldc, int n, int sr_bits, int out_f32) {
-  if (!C) return fail(NG_ERR_INVALID_ARG, "null operand");
-  if (ldc < n) return fail(NG_ERR_INVALID_ARG, "leading dimension too small");
-  if (sr_bits < 0 || sr_bits > 10) return fail(NG_ERR_INVALID_ARG, "stochastic rounding keeps 1..10 mantissa bits");
-  if (sr_bits && out_f32) return fail(NG_ERR_UNSUPPORTED, "stochastic rounding is to fp16");
-  return NG_OK;
-}
-
-}  // namespace
-
 }  // namespace ngb
 
 using namespace ngb;
@@ -467,17 +318,18 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
 
   const bool nv = A->format == NG_BLOCK_NVFP4;
   DotParams p = {};
-  p.ea.alpha = nv ? alpha * a.t * b.t : alpha;     // (powers of two)
-  p.ea.beta = beta; p.ea.relu = relu; p.ea.sr_bits = sr_bits;
-  p.ea.seed_lo = static_cast<uint32_t>(seed); p.ea.seed_hi = static_cast<uint32_t>(seed >> 32); p.ea.rng_offset = rng_offset;
-  p.C = C; p.ldc = ldc; p.out_f32 = out_f32;
-  p.vec_ok = (reinterpret_cast<uintptr_t>(C) & 15u) == 0 && ldc % (out_f32 ? 4 : 8) == 0;
+  EpiArgs& ea = p.out.ea;
+  ea.alpha = nv ? alpha * a.t * b.t : alpha;     // (powers of two)
+  ea.beta = beta; ea.relu = relu; ea.sr_bits = sr_bits;
+  ea.seed_lo = static_cast<uint32_t>(seed); ea.seed_hi = static_cast<uint32_t>(seed >> 32); ea.rng_offset = rng_offset;
+  p.out.C = C; p.out.ldc = ldc; p.out.out_f32 = out_f32;
+  p.out.vec_ok = (reinterpret_cast<uintptr_t>(C) & 15u) == 0 && ldc % (out_f32 ? 4 : 8) == 0;
   // The operand with more rows goes to the tile's 128 rows where that leaves less of the tiles empty.
   const long long as_is = (m + 127ll) / 128 * 128 * pad_columns(n), turned = (n + 127ll) / 128 * 128 * pad_columns(m);
   p.swapped = turned < as_is;
   if (p.swapped) std::swap(a, b);
-  p.M = a.outer; p.N = b.outer;
-  p.tiles_m = (p.M + 127) / 128;
+  p.out.M = a.outer; p.out.N = b.outer;
+  p.tiles_m = (p.out.M + 127) / 128;
   p.num_kb = (a.inner + 255) / 256;
   p.ca = a.codes; p.cb = b.codes; p.pitch_a = a.pitch; p.pitch_b = b.pitch; p.tile_a = a.tile;
   p.sa = a.scales; p.sb = b.scales; p.spitch = a.spitch;
@@ -485,8 +337,8 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   // Columns of a tile: B's rows padded, as its scales lie; a column of more has its tile in the middle of a scale tile, which
   // tensor memory cannot address. Partitions of the sum, by what they take in us: per round of tiles, the k-blocks at 135
   // bytes/ns and the output stage; when split, the exchange, at 30 bytes/ns of what each CTA gets.
-  const int cols = p.N > 64 ? 128 : pad_columns(p.N);
-  const long long tiles = static_cast<long long>(p.tiles_m) * ((p.N + cols - 1) / cols);
+  const int cols = p.out.N > 64 ? 128 : pad_columns(p.out.N);
+  const long long tiles = static_cast<long long>(p.tiles_m) * ((p.out.N + cols - 1) / cols);
   int splits = 1;
   double here = 0.0;
   for (int s = 1, log = 0; s <= 8 && (s == 1 || (p.num_kb >= s && tiles * s <= cluster_room(c, log))); s *= 2, ++log) {
@@ -505,7 +357,7 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   const double pairs = 5.5 + (pair_tiles + c->sm_count / 2 - 1) / (c->sm_count / 2) * (0.33 * p.num_kb + 0.7);
   if (m > 64 && n > 64 && pairs < here) {
     if (p.swapped) std::swap(a, b);
-    return run_block_dot_pair(c, a, b, nv, make_out(C, m, n, ldc, out_f32, p.ea), static_cast<cudaStream_t>(stream));
+    return run_block_dot_pair(c, a, b, nv, make_out(C, m, n, ldc, out_f32, ea), static_cast<cudaStream_t>(stream));
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define NG_DOT(kn) (nv ? launch_dot<kn, true>(c, p, splits, s) : launch_dot<kn, false>(c, p, splits, s))

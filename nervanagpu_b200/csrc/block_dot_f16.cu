@@ -8,7 +8,8 @@
 // their power of two (exact) and store them where the 128-byte swizzle wants them; no fp16 copy of the record is ever
 // in memory. A's tiles come by TMA, or, from rows that TMA cannot address, through the same warps. A CTA
 // computes tiles of 128 x kN, one after the other, with two accumulators, so that the output stage of one tile runs
-// beside the products of the next: with few images the time is that of writing C.
+// beside the products of the next: with few images the time is that of writing C. Few tiles with a long sum are split
+// along it instead (kMixSplit), a tile over the CTAs of a cluster (block_share.cuh).
 //
 //   warp 0       TMA producer
 //   warp 1       tensor memory, MMAs
@@ -17,6 +18,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "block_share.cuh"
 #include "blocks.h"
 
 namespace ngb {
@@ -31,14 +33,18 @@ constexpr int kMixRaw = 3;                                // slots of codes
 constexpr uint32_t kMixCtrl = 256;
 constexpr uint32_t kMixSmemLimit = 232448;
 
-template <int kN>
+constexpr int kMixSplit = 3;                              // besides the OutForms
+
+template <int kN, bool kSplit>
 struct MixTile {
   static constexpr uint32_t kB = kN * 128u;
   static constexpr uint32_t kSlot = kMixA + kB;
   static constexpr uint32_t kRaw = kN * 64u;              // a k-block of codes
-  static constexpr int kRoom = static_cast<int>((kMixSmemLimit - 1024u - kMixCtrl - kMixStage - kMixRaw * kRaw) / kSlot);
+  static constexpr uint32_t kOut = kSplit ? kShareTile<kN> : kMixStage;      // output staging, or the others' parts
+  static constexpr int kRoom = static_cast<int>((kMixSmemLimit - 1024u - kMixCtrl - kOut - kMixRaw * kRaw) / kSlot);
   static constexpr int kStages = kRoom < 6 ? kRoom : 6;
-  static constexpr uint32_t kSmem = kStages * kSlot + kMixRaw * kRaw + kMixStage + kMixCtrl + 1024u;
+  static constexpr uint32_t kSmem = kStages * kSlot + kMixRaw * kRaw + kOut + kMixCtrl + 1024u;
+  static_assert(!kSplit || kOut <= kStages * kSlot, "the ring is smaller than the tile");
   static constexpr uint32_t kCols = 2 * kN;               // of tensor memory: two accumulators
   static constexpr int kEpiCols = kN > 64 ? kN / 2 : 64;  // columns of an output-stage warp (64: one of the two has them all)
 };
@@ -51,6 +57,7 @@ struct MixParams {
   int tiles_n, tiles, num_kb;
   BlockView x;
   OutParams out;
+  ShareOut share;
   int* status;
   unsigned long long wait_limit_ns;
 };
@@ -59,21 +66,29 @@ template <int kN, int kForm>
 __global__ void __launch_bounds__(kMixThreads, 1)
 block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapX,
                      const __grid_constant__ CUtensorMap mapC, const __grid_constant__ MixParams p) {
-  using T = MixTile<kN>;
+  constexpr bool kSplit = kForm == kMixSplit;
+  using T = MixTile<kN, kSplit>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* ring_gen = smem_raw + (ring - smem_u32(smem_raw));
   const uint32_t raw = ring + T::kStages * T::kSlot, staging = raw + kMixRaw * T::kRaw;
-  const uint32_t ctrl = staging + kMixStage;
+  const uint32_t ctrl = staging + T::kOut;
   auto full_bar = [&](int s) { return ctrl + 8u * s; };
   auto empty_bar = [&](int s) { return ctrl + 8u * (6 + s); };
   auto accf_bar = [&](int a) { return ctrl + 8u * (12 + a); };
   auto acce_bar = [&](int a) { return ctrl + 8u * (14 + a); };
   auto rawf_bar = [&](int s) { return ctrl + 8u * (16 + s); };
   auto rawe_bar = [&](int s) { return ctrl + 8u * (19 + s); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_gen + (ctrl - ring) + 8 * 22);
+  const uint32_t part_bar = ctrl + 8u * 22;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_gen + (ctrl - ring) + 8 * 23);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // this CTA's tiles and its part of their sums
+  const int splits = kSplit ? static_cast<int>(cluster_size()) : 1, rank = kSplit ? static_cast<int>(cluster_cta_rank()) : 0;
+  const int first_tile = kSplit ? blockIdx.x / splits : blockIdx.x, step = kSplit ? p.tiles : gridDim.x;
+  const int kb0 = kSplit ? static_cast<int>(static_cast<long long>(p.num_kb) * rank / splits) : 0;
+  const int kb1 = kSplit ? static_cast<int>(static_cast<long long>(p.num_kb) * (rank + 1) / splits) : p.num_kb;
+  const uint32_t share_bytes = T::kOut / splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < T::kStages; ++s) {
@@ -88,11 +103,13 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
       mbar_init(rawf_bar(s), 1);
       mbar_init(rawe_bar(s), kMixConv);
     }
+    mbar_init(part_bar, 1);
     *abort_flag = 0;
     mbar_fence_init();
+    if (kSplit) mbar_expect_tx(part_bar, (splits - 1) * share_bytes);
     if (p.a_tma) tma_prefetch_desc(&mapA);
     tma_prefetch_desc(&mapX);
-    if (p.out.store) tma_prefetch_desc(&mapC);
+    if (!kSplit && p.out.store) tma_prefetch_desc(&mapC);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), T::kCols);
@@ -101,6 +118,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (kSplit) cluster_arrive();      // (this CTA's barriers exist)
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
 
@@ -109,9 +127,9 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     if (elect_one()) {
       int it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+      for (int t = first_tile; t < p.tiles && ok; t += step) {
         const int m0 = t / p.tiles_n * 128, n0 = t % p.tiles_n * kN;
-        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % T::kStages, x = it % kMixRaw;
           if (it >= kMixRaw && !mbar_wait(rawe_bar(x), (it / kMixRaw - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_PRODUCER, p.wait_limit_ns)) {
             ok = false;
@@ -137,14 +155,14 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
       const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(kN >> 3) << 17) | ((128u >> 4) << 24);
       int it = 0, local = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x, ++local) {
+      for (int t = first_tile; t < p.tiles && ok; t += step, ++local) {
         const int acc = local & 1;
         if (local >= 2 && !mbar_wait(acce_bar(acc), (local / 2 - 1) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_ACC, p.wait_limit_ns)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % T::kStages;
           if (!mbar_wait(full_bar(s), (it / T::kStages) & 1, abort_flag, p.status, NG_DEV_TIMEOUT_MMA, p.wait_limit_ns)) {
             ok = false;
@@ -152,7 +170,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
           }
           tc_fence_after();
           const uint32_t a = ring + s * T::kSlot;
-          tc_mma_f16_run<false, 4>(tmem + acc * kN, lo | (a >> 4), hi, lo | ((a + kMixA) >> 4), hi, idesc, kb != 0, 2u, 2u);
+          tc_mma_f16_run<false, 4>(tmem + acc * kN, lo | (a >> 4), hi, lo | ((a + kMixA) >> 4), hi, idesc, kb != kb0, 2u, 2u);
           tc_commit(empty_bar(s));
         }
         if (ok) tc_commit(accf_bar(acc));
@@ -167,7 +185,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     auto row_of = [&](int t) { return t / p.tiles_n * 128 + group * 32; };
     auto col_of = [&](int t) { return t % p.tiles_n * kN + half * T::kEpiCols; };
     int local = 0;
-    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++local) {
+    for (int t = first_tile; t < p.tiles; t += step, ++local) {
       const int acc = local & 1;
       const int m0 = row_of(t), n0 = col_of(t);
       if (local == 0) out_ahead<kForm, T::kEpiCols>(p.out, m0, n0);
@@ -177,10 +195,24 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
         break;
       }
       tc_fence_after();
-      if (t + static_cast<int>(gridDim.x) < p.tiles) out_ahead<kForm, T::kEpiCols>(p.out, row_of(t + gridDim.x), col_of(t + gridDim.x));
+      if (t + step < p.tiles) out_ahead<kForm, T::kEpiCols>(p.out, row_of(t + step), col_of(t + step));
       const uint32_t taddr = tmem + (static_cast<uint32_t>(group * 32) << 16) + acc * kN + half * T::kEpiCols;
       auto release = [&] { if (lane == 0) mbar_arrive(acce_bar(acc)); };
-      if (half * T::kEpiCols >= kN) release();
+      if constexpr (kSplit) {
+        // the partial tile, where the ring was
+        float* row = reinterpret_cast<float*>(ring_gen) + (group * 32 + lane) * kSharePitch<kN>;
+#pragma unroll 1
+        for (int c = half * (kN / 2); c < (half + 1) * (kN / 2); c += 32) {
+          uint32_t r[32];
+          tc_ld_32x32(tmem + (static_cast<uint32_t>(group * 32) << 16) + c, r);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            reinterpret_cast<uint4*>(row + c)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        }
+        tc_fence_before();
+        fence_async_smem();      // (the parts leave by bulk copies)
+      } else if (half * T::kEpiCols >= kN) release();
       else out_tile<kForm, T::kEpiCols>(p.out, &mapC, taddr, stage, stage_gen, m0, n0, release);
     }
     if (lane == 0) tma_store_wait_all();
@@ -193,12 +225,12 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     const int r = tid / kPer, part = tid % kPer;
     int it = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+    for (int t = first_tile; t < p.tiles && ok; t += step) {
       const int m0 = t / p.tiles_n * 128, j = t % p.tiles_n * kN + r;
       // the scales of 128 codes are a word
       const uint8_t* scales = p.x.scales + static_cast<long long>(j) * p.x.spitch;
-      uint32_t word = j < p.N ? *reinterpret_cast<const uint32_t*>(scales) : 0u;
-      for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+      uint32_t word = j < p.N ? *reinterpret_cast<const uint32_t*>(scales + kb0 / 2 * 4ll) : 0u;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % T::kStages, x = it % kMixRaw;
         // A, when TMA cannot: 16 rows per warp, two numbers per lane and row, on their way while this waits
         constexpr int kRows = 128 / kMixConv;
@@ -254,7 +286,7 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(rawe_bar(x));
-        if ((kb & 1) && kb + 1 < p.num_kb && j < p.N) word = *reinterpret_cast<const uint32_t*>(scales + (kb + 1) * 2ll);
+        if ((kb & 1) && kb + 1 < kb1 && j < p.N) word = *reinterpret_cast<const uint32_t*>(scales + (kb + 1) * 2ll);
         if (!p.a_tma) {
           uint8_t* a = ring_gen + s * T::kSlot + a_row * 128 + ((lane * 2) & 15);
           const int at = (lane * 2) & 112;
@@ -272,15 +304,25 @@ block_dot_f16_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     }
   }
   __syncthreads();
+  if (kSplit) share_push(ring, staging, share_bytes, rank, splits, part_bar);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, T::kCols);
   }
+  if constexpr (kSplit) {
+    share_wait(part_bar, abort_flag, p.status, p.wait_limit_ns);
+    if (!*abort_flag)
+      share_store<kN, kMixThreads>(p.share, false, reinterpret_cast<float*>(ring_gen), reinterpret_cast<const float*>(ring_gen + (staging - ring)),
+                                   splits, rank, first_tile / p.tiles_n * 128, first_tile % p.tiles_n * kN);
+    __syncwarp();
+    cluster_wait();
+  }
 }
 
 template <int kN, int kForm>
-int launch_mix(DeviceCtx* c, MixParams& p, cudaStream_t stream) {
-  using T = MixTile<kN>;
+int launch_mix(DeviceCtx* c, MixParams& p, int splits, cudaStream_t stream) {
+  constexpr bool kSplit = kForm == kMixSplit;
+  using T = MixTile<kN, kSplit>;
   p.tiles_n = (p.N + kN - 1) / kN;
   const long long tiles = static_cast<long long>(p.tiles_n) * ((p.M + 127ll) / 128);
   if (tiles > 0x3fffffffll) return fail(NG_ERR_TOO_LARGE, "too many tiles");
@@ -290,18 +332,22 @@ int launch_mix(DeviceCtx* c, MixParams& p, cudaStream_t stream) {
   if (p.a_tma) rc = plain_map(&mapA, p.A, p.M, p.K, p.lda, 64, 128, 2);
   // (codes as 16-bit units; zeros beyond the last row)
   if (rc == NG_OK) rc = plain_map(&mapX, p.x.codes, p.N, p.x.pitch / 2, p.x.pitch / 2, 32, kN, 2);
-  if (rc == NG_OK && p.out.store) rc = out_map(&mapC, p.out);
+  if (rc == NG_OK && !kSplit && p.out.store) rc = out_map(&mapC, p.out);
   if (rc != NG_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, c->sm_count)));
+  cfg.gridDim = dim3(static_cast<unsigned>(kSplit ? tiles * splits : std::min<long long>(tiles, c->sm_count)));
   cfg.blockDim = dim3(kMixThreads);
   cfg.dynamicSmemBytes = T::kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = tuning().dependent_launch != 0 ? 1 : 0;
+  cfg.numAttrs = tuning().dependent_launch != 0 ? 2 : 1;
   static std::atomic<unsigned long long> ready{0};
   if (!(ready.load(std::memory_order_relaxed) >> c->device & 1u)) {
     NG_CUDA(cudaFuncSetAttribute(block_dot_f16_kernel<kN, kForm>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
@@ -358,15 +404,39 @@ int run_block_dot_f16(DeviceCtx* c, const void* A, int lda, const ng_block_desc&
       cols = n;
     }
   }
-  // Converting on the way costs a k-block of a 256-column tile 0.66 us where its products take 0.27, so longer sums are
-  // better off with an fp16 copy, which costs a launch and its traffic but leaves the product alone: here / from
-  // scratch, us: 1024 x 1024 x 1024 9.4 / 14.6, 4096 x 4096 x 256 18.2 / 17.1, x 512 28.9 / 24.6, x 1024 50.7 / 35.5,
-  // 512 x 512 x 8192 55 / 17, 1000 x 4096 x 2000 27.0 / 24.0. Two k-blocks are always within the time of writing C.
+  // Whole sums, sums in parts, or a copy, by what each takes in us. whole / parts / copy, measured: 512 x 512 x 1024 10.0 / 6.7 /
+  // 11.9, 300 x 300 x 4000 31 / 8.9 / 14.3, x 4001 65 / 13.2 / 16.9, 5844 x 64 x 773 15.9 / 11.7 / 13.8, 512 x 512 x 8192 62 / 20.5 /
+  // 16.4, 128 x 128 x 256 5.0 / 5.0 / 7.0; without room for parts 1001 x 4097 x 1000 17.5 / - / 21.9, 4096 x 4096 x 250 27 / - / 18.
+  // A k-block of a tile, whose conversion takes longer than its products (with A's odd rows more), the
+  // tiles one after the other, each with its output.
+  const double odd = p.a_tma ? 0.0 : 0.45;
+  auto kblock = [&](int n) { return 0.32 + n * 0.0013 + odd; };
   const long long rounds = best / (cols + 64);
+  const double whole = 4.0 + rounds * (p.num_kb * kblock(cols) + 0.8 + cols * 0.0047);
+  // Or the sum in parts, with their exchange at 30 bytes/ns of what each CTA gets.
+  double here = whole;
+  int splits = 1, split_cols = 0;
+  for (int n = 64; n <= 128; n *= 2)
+    for (int log = 1; log <= 3; ++log) {
+      const int s = 1 << log;
+      if (p.num_kb < s || row_tiles * ((p.N + n - 1ll) / n) * s > cluster_room(c, log)) break;
+      const double us = 3.6 + (p.num_kb + s - 1) / s * kblock(n) + 1.0 + 512.0 * n * (s - 1) / s * 3.3e-5 + 1.0 / s;
+      if (us < here) {
+        here = us;
+        splits = s;
+        split_cols = n;
+      }
+    }
+  // Or an fp16 copy of the record, and of A's odd rows, which cost launches and traffic but leave the product alone.
+  const double copy = 11.0 + 2.0 * m * p.N * p.K * 1e-9 + (3.0 * p.N * p.K + (p.a_tma ? 0.0 : 4.0 * m * p.K)) * 2e-7;
   int rc;
-  if (p.num_kb > 2 && rounds * p.num_kb > 16 && from_scratch(c, A, lda, d, x, C, m, ldc, out_f32, ea, stream, rc)) return rc;
+  if (copy < here && from_scratch(c, A, lda, d, x, C, m, ldc, out_f32, ea, stream, rc)) return rc;
+  if (splits > 1) {
+    p.share = {m, p.N, C, ldc, out_f32, (reinterpret_cast<uintptr_t>(C) & 15u) == 0 && ldc % (out_f32 ? 4 : 8) == 0, ea};
+    return split_cols == 128 ? launch_mix<128, kMixSplit>(c, p, splits, stream) : launch_mix<64, kMixSplit>(c, p, splits, stream);
+  }
 #define NG_MIX(form) \
-  (cols == 256 ? launch_mix<256, form>(c, p, stream) : cols == 128 ? launch_mix<128, form>(c, p, stream) : launch_mix<64, form>(c, p, stream))
+  (cols == 256 ? launch_mix<256, form>(c, p, 1, stream) : cols == 128 ? launch_mix<128, form>(c, p, 1, stream) : launch_mix<64, form>(c, p, 1, stream))
   switch (out_form(p.out)) {
     case kOutLean: return NG_MIX(kOutLean);
     case kOutF16: return NG_MIX(kOutF16);

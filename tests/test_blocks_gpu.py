@@ -401,6 +401,39 @@ def test_block_dot_f16(ng, m, n, k, shift):
     assert abs(f(W) - float(F.get()[i, j])) <= product_tol(ref, mag, k, f32=True)[i, j] + 1e-12 * mag[i, j]
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 3, 700), (70, 90, 1000), (130, 65, 2049), (129, 200, 1537), (300, 300, 1500), (513, 20, 650)])
+@pytest.mark.parametrize("aligned", [False, True])
+def test_long_sums_of_few_outputs(ng, m, n, k, aligned):
+    """Sums that are split over several SMs: every output form, views, and the same bits every time."""
+    rng = np.random.default_rng(m + n + k)
+    E = (rng.standard_normal((m, k)) * 0.1).astype(np.float16)
+    X = np.maximum(rng.standard_normal((n, k)), 0).astype(np.float16)
+    lda = k + -k % 8 if aligned else k + 1 + k % 2
+    wide = np.full((m, lda), np.nan, np.float16)
+    wide[:, :k] = E
+    A, B = ng.array(wide)[:, :k], ng.quantize(ng.array(X), ng.block_empty((n, k), "mxfp8")).T
+    x = rm.block_values(X, "mxfp8")
+    e = E.astype(np.float64)
+    dot, mag = e @ x.T, np.abs(e) @ np.abs(x).T
+    ldc = n + -n % 8 if aligned else n + 3
+    for dtype in (np.float16, np.float32):
+        old = rng.standard_normal((m, n)).astype(np.float16)
+        first = None
+        for _ in range(3):
+            C = ng.array(np.full((m + 1, ldc), 7.0), dtype=dtype)
+            C[:m, :n] = ng.array(old, dtype=dtype)
+            ng.block_dot(A, B, C[:m, :n], alpha=2.0, beta=-1.0, relu=True)
+            got = C.get()
+            first = got if first is None else first
+            assert np.array_equal(first, got)
+        ref = np.maximum(2 * dot, 0) - old
+        assert_close(got[:m, :n], ref, product_tol(ref, 2 * mag + np.abs(old), k + 2, f32=dtype is np.float32), str(dtype))
+        assert (got[m] == 7).all() and (got[:, n:] == 7).all()
+    C = ng.empty((m, n))
+    ng.block_dot(A, B, C, stochastic_round=10)
+    assert_close(C.get(), dot, product_tol(dot, mag, k, steps=2.0))
+
+
 def test_extreme_records_in_the_mixed_product(ng):
     """The largest and smallest fp16 numbers, and numbers that a record keeps only by their sign."""
     X = np.zeros((8, 64), np.float16)
