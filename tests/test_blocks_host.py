@@ -128,6 +128,15 @@ def test_transposed_views_share_memory():
     assert "nvfp4" in str(q) and q.size == 1024
 
 
+def test_a_transposed_view_is_made_once_and_holds_no_cycle():
+    import weakref
+    q = block(Host(), (16, 64), "mxfp8", 1, 1.0)
+    t, gone = q.T, weakref.ref(q)
+    assert q.T is t
+    del q
+    assert gone() is None and t.shape == (64, 16)       # (freed at once, not by the collector)
+
+
 def test_block_descriptor_matches_header():
     assert [f[0] for f in _lib.BlockDesc._fields_] == "format axis rows cols device scale codes scales".split()
     assert ctypes.sizeof(_lib.BlockDesc) == 40
