@@ -33,6 +33,15 @@ __device__ __forceinline__ void epi_store_nearest(const EpiArgs& e, float acc, f
   epi_put(c, out);
 }
 
+__device__ __forceinline__ void tc_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 // fp16, rounded to nearest, nothing added: all columns to registers first, then `release` gives the accumulator back.
 template <int kCols, typename F>
 __device__ __forceinline__ void out_lean(const OutParams& p, const CUtensorMap* mapC, uint32_t taddr, uint32_t stage, uint8_t* stage_gen,
@@ -41,12 +50,12 @@ __device__ __forceinline__ void out_lean(const OutParams& p, const CUtensorMap* 
   const bool as_is = p.ea.alpha == 1.0f && !p.ea.relu;
   uint32_t w[kCols / 2];
 #pragma unroll
-  for (int c = 0; c < kCols; c += 32) {
-    uint32_t r[32];
-    tc_ld_32x32(taddr + c, r);
+  for (int c = 0; c < kCols; c += 16) {      // (by 32 columns the registers did not suffice in tiles of 256)
+    uint32_t r[16];
+    tc_ld_32x16(taddr + c, r);
     tc_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       float a = __uint_as_float(r[2 * i]), b = __uint_as_float(r[2 * i + 1]);
       if (!as_is) {
         a = epi_scale(p.ea, a);
