@@ -522,6 +522,31 @@ def test_other_streams_and_recorded_sequences():
         second.launch()
 
 
+def test_a_long_sum_recorded_without_room_and_with_it():
+    """600 x 500 x 8200 would take a copy in scratch memory: a recording on a new stream, which cannot grow it, and one after
+    a run that did; two recordings in turn."""
+    ng = NervanaGPU(stochastic_round=False)
+    rng = np.random.default_rng(5)
+    m, n, k = 600, 500, 8200
+    E = (rng.standard_normal((m, k)) * 0.1).astype(np.float16)
+    X = np.maximum(rng.standard_normal((n, k)), 0).astype(np.float16)
+    A, Q = ng.array(E), ng.quantize(ng.array(X), ng.block_empty((n, k), "mxfp8"))
+    ng.synchronize()
+    x, e = rm.block_values(X, "mxfp8"), E.astype(np.float64)
+    ref, mag = e @ x.T, np.abs(e) @ x.T
+    ng.stream = ng.new_stream()
+    C, D = ng.zeros((m, n), dtype=np.float32), ng.zeros((m, n), dtype=np.float32)
+    first = ng.capture(lambda: ng.block_dot(A, Q.T, C))
+    first.launch()
+    assert_close(C.get(), ref, product_tol(ref, mag, k, f32=True))
+    ng.block_dot(A, Q.T, C)
+    second = ng.capture(lambda: ng.block_dot(A, Q.T, D))
+    for run in (second, first, second):
+        C.fill(0), D.fill(0)
+        run.launch()
+        assert_close((D if run is second else C).get(), ref, product_tol(ref, mag, k, f32=True))
+
+
 def test_launches_and_no_fallback(ng, lib):
     """Each call launches the library's kernels and none of the CUDA-core products."""
     import ctypes
