@@ -111,9 +111,9 @@ __device__ __forceinline__ void out_lean(const OutParams& p, const CUtensorMap* 
 }
 
 // Everything else: fp32, C added, stochastic rounding. 32 columns at a time go through the staged box in fp32, so that
-// neighbouring lanes read and write neighbours of C, and what C held in all 32 rows is on its way together. (With a row per lane
+// neighbouring lanes read and write neighbours of C, and what C held in 16 or 32 rows is on its way together. (With a row per lane
 // each access touched 32 sectors, and the loads of one chunk waited for the stores of the last: with C added, 5664 x 546 x 1698
-// 28.5 -> 15.5 us and 4096 x 9216 x 128 160 -> 48, against 8.4 and 20 without.) First, rows of C at any address: a number per lane.
+// 28.5 -> 15.4 us and 4096 x 9216 x 128 160 -> 45, against 8.4 and 20 without.) First, rows of C at any address: a number per lane.
 template <int kCols, typename E, typename F>
 __device__ __forceinline__ void out_odd(const OutParams& p, uint32_t taddr, uint8_t* stage_gen, int m0, int n0, F release) {
   const int lane = threadIdx.x & 31;
@@ -121,10 +121,6 @@ __device__ __forceinline__ void out_odd(const OutParams& p, uint32_t taddr, uint
   for (int c = 0; c < kCols; c += 32) {
     const int rows = min(32, p.M - m0), col = n0 + c + lane;
     E* out = static_cast<E*>(p.C) + m0 * p.ldc + col;
-    OldBits<E> old[32];
-    const int held = p.ea.beta != 0.0f && col < p.N ? rows : 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) old[i] = i < held ? reinterpret_cast<const OldBits<E>*>(out)[i * p.ldc] : OldBits<E>(0);
     uint32_t r[32];
     tc_ld_32x32(taddr + c, r);
     tc_wait_ld();
@@ -154,12 +150,21 @@ __device__ __forceinline__ void out_odd(const OutParams& p, uint32_t taddr, uint
                                static_cast<unsigned long long>(m0 + i) * p.N + first, min(8, p.N - first), false);
       }
     } else if (col < p.N) {
-      float x[32];             // (all of them first: no load passes a store)
+      // (fp32: with 32 rows at a time the registers did not suffice, 1001 x 4097 x 125 17.6 us for 13.0; fp16 with 16: 20.4 for 15.1)
+      constexpr int kRows = sizeof(E) == 4 ? 16 : 32;
+      const int held = p.ea.beta != 0.0f ? rows : 0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < rows; i0 += kRows) {
+        OldBits<E> old[kRows];
+        float x[kRows];          // (all of them first: no load passes a store)
 #pragma unroll
-      for (int i = 0; i < 32; ++i) x[i] = at(i);
+        for (int i = 0; i < kRows; ++i) old[i] = i0 + i < held ? reinterpret_cast<const OldBits<E>*>(out)[(i0 + i) * p.ldc] : OldBits<E>(0);
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < rows) epi_store_nearest(p.ea, x[i], to_f32(old[i]), out + i * p.ldc);
+        for (int i = 0; i < kRows; ++i) x[i] = at(i0 + i);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (i0 + i < rows) epi_store_nearest(p.ea, x[i], to_f32(old[i]), out + (i0 + i) * p.ldc);
+      }
     }
     __syncwarp();
   }
