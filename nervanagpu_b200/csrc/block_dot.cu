@@ -15,7 +15,6 @@
 //   all        sum over the cluster, output stage (epilogue.cuh), stores
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "block_mma.cuh"
 #include "block_share.cuh"

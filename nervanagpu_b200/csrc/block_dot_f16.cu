@@ -407,11 +407,12 @@ int run_block_dot_f16(DeviceCtx* c, const void* A, int lda, const ng_block_desc&
       cols = n;
     }
   }
-  // Whole sums, sums in parts, or a copy, by what each takes in us. whole / parts / copy, measured: 512 x 512 x 1024 10.0 / 6.7 /
-  // 11.9, 300 x 300 x 4000 31 / 8.9 / 14.3, x 4001 65 / 13.2 / 16.9, 5844 x 64 x 773 15.9 / 11.7 / 13.8, 512 x 512 x 8192 62 / 20.5 /
-  // 16.4, 128 x 128 x 256 5.0 / 5.0 / 7.0; without room for parts 1001 x 4097 x 1000 17.5 / - / 21.9, 4096 x 4096 x 250 27 / - / 18, 4096 x 9216 x 128 20.0 / - / 20.9.
-  // A k-block of a tile, whose conversion takes longer than its products (with A's odd rows more), the
-  // tiles one after the other, each with its output.
+  // Whole sums, sums in parts, or a copy, by what each takes in us. Measured, whole / parts / copy: 512 x 512 x 1024 10.0 / 6.7
+  // / 11.9, 300 x 300 x 4000 31 / 8.9 / 14.3, x 4001 65 / 13.2 / 16.9, 5844 x 64 x 773 15.9 / 11.7 / 13.8, 512 x 512 x 8192
+  // 62 / 20.5 / 16.4, 128 x 128 x 256 5.0 / 5.0 / 7.0; without room for parts, whole / copy: 1001 x 4097 x 1000 17.5 / 21.9,
+  // 4096 x 4096 x 250 27 / 18, 4096 x 9216 x 128 20.0 / 20.9.
+  // Whole: the tiles one after the other, k-blocks, whose conversion takes longer than their products (A's odd rows more
+  // still), and output.
   const double odd = p.a_tma ? 0.0 : 0.45;
   auto kblock = [&](int n) { return 0.32 + n * 0.0013 + odd; };
   const long long rounds = best / (cols + 64);
@@ -432,7 +433,8 @@ int run_block_dot_f16(DeviceCtx* c, const void* A, int lda, const ng_block_desc&
       }
     }
   // Or an fp16 copy of the record, and of A's odd rows, which cost launches and traffic but leave the product alone.
-  const double copy = 11.0 + std::max(2.0 * m * p.N * p.K * 1e-9, m * (out_f32 ? 4.0 : 2.0) * p.N * 2.6e-7) + (3.0 * p.N * p.K + (p.a_tma ? 0.0 : 4.0 * m * p.K)) * 2e-7;
+  const double copy = 11.0 + std::max(2.0 * m * p.N * p.K * 1e-9, m * (out_f32 ? 4.0 : 2.0) * p.N * 2.6e-7) +
+                      (3.0 * p.N * p.K + (p.a_tma ? 0.0 : 4.0 * m * p.K)) * 2e-7;
   int rc;
   if (copy < here && from_scratch(c, A, lda, d, x, C, m, ldc, out_f32, ea, stream, rc)) return rc;
   if (splits > 1) {

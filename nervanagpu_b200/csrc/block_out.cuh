@@ -13,19 +13,19 @@ struct OutParams {
   void* C;
   long long ldc;
   int out_f32;
-  int store;              // 1: TMA can address C's rows, whole; 0: one number per lane and access
+  int store;              // 1: C's rows are whole aligned vectors, which TMA can address; 0: any address
   EpiArgs ea;
 };
 
-// One output, rounded to nearest, with what C held given.
-// (Loaded as bits, converted when used: a load with its conversion under one condition becomes a branch, and waits for the one
-// before.)
+// What C held, loaded as bits and converted when used: a load with its conversion under one condition becomes a branch, and
+// waits for the one before.
 template <typename E>
 using OldBits = std::conditional_t<sizeof(E) == 2, unsigned short, float>;
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(unsigned short x) { return __half2float(__ushort_as_half(x)); }
 __device__ __forceinline__ void epi_put(float c, float* out) { *out = c; }
 __device__ __forceinline__ void epi_put(float c, __half* out) { *out = f2h_rn(c); }
+// One output, rounded to nearest.
 template <typename E>
 __device__ __forceinline__ void epi_store_nearest(const EpiArgs& e, float acc, float old, E* out) {
   float c = epi_scale(e, acc);
@@ -42,6 +42,7 @@ __device__ __forceinline__ void tc_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
+
 // fp16, rounded to nearest, nothing added: all columns to registers first, then `release` gives the accumulator back.
 template <int kCols, typename F>
 __device__ __forceinline__ void out_lean(const OutParams& p, const CUtensorMap* mapC, uint32_t taddr, uint32_t stage, uint8_t* stage_gen,
