@@ -237,7 +237,8 @@ int ng_pool_bprop_argmax(const ng_pool_desc* desc, int dtype_bytes, const void* 
  *                   zero never becomes zero
  * A power-of-two scale is the smallest that brings the block's largest magnitude within the format; an
  * nvfp4 scale is RN_E4M3(largest / 6 / scale), kept from 2^-9 to 448. Numbers are rounded to nearest, ties to
- * even, and limited to the largest. A block that holds an infinity or NaN reads back as NaN.
+ * even, and limited to the largest; signs are kept, those of zeros too but in nvfp4. A block that holds an infinity or
+ * NaN reads back as NaN.
  * axis: 1 = blocks run along the rows (neighbouring columns), 0 = down the columns.
  * codes, scales: device memory of ng_block_bytes() bytes each, 128-byte aligned, zeroed when it is allocated
  * (the padding of rows and tiles has to be zero; no call writes it) and laid out for one axis and format.

@@ -11,6 +11,10 @@
 //   s = RN_E4M3(max|x| / (6 t)), kept from 2^-9 (a block that is not all zero keeps a scale) to 448
 //   code = RN(x / scale), ties to even, limited to the largest number
 //   mxfp8: a number that is not zero gets a code that is not zero, so that x > 0 can be told from the code.
+//   Signs are kept, in mxfp4 and mxfp8 those of zeros and of what becomes zero too: the codes of a matrix are the same bytes
+//   whatever its type, strides and blocked axis. (nvfp4 rounds with sums that lose the sign of a zero, fp16 numbers below
+//   2^-16 of the scale theirs too, fp32 numbers not: those zeros may differ in their sign. An instruction per number that
+//   puts it back took 7 % of a quantisation, 4096 x 9216 13.6 -> 14.6 us.)
 //
 // Values are read limited to the largest number of the type that they are read as: a number next to it may have been
 // rounded to one beyond it.
@@ -190,7 +194,8 @@ __device__ __forceinline__ uint2 block_encode8(const float (&x)[8], const BlockS
     for (int i = 0; i < 8; ++i) {
       // not zero: no less than the smallest code; in a block with the scale NaN the smallest code of x's sign
       const float mag = s.nan ? 0.001953125f : fmaxf(fabsf(x[i]) * s.by, 0.001953125f);
-      y[i] = (x[i] > 0.0f || x[i] < 0.0f) ? copysignf(mag, x[i]) : 0.0f;
+      // (a zero as it is, 0 for a NaN; as the sign put on a 0 it took 7 registers more, 139968 x 128 fp16 8.0 -> 8.4 us)
+      y[i] = (x[i] > 0.0f || x[i] < 0.0f) ? copysignf(mag, x[i]) : fminf(x[i], 0.0f);
     }
     r.x = cvt_e4m3x2(y[0], y[1]) | (cvt_e4m3x2(y[2], y[3]) << 16);
     r.y = cvt_e4m3x2(y[4], y[5]) | (cvt_e4m3x2(y[6], y[7]) << 16);
