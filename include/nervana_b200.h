@@ -270,8 +270,8 @@ int ng_block_relu_mask(const ng_block_desc* q, void* E, int dtype_bytes, long lo
                        void* stream);
 /* C[m x n] = relu?(alpha * A * B) + beta * C, C row-major, fp16 or fp32 (out_f32), fp32 accumulation; rounding
  * as in ng_hgemm. A is m x k with axis 1, B is k x n with axis 0: the blocks run along the sum. Both are in the
- * same 4-bit format. (A matrix is its transpose with rows and cols exchanged and the other axis: the memory is the
- * same.) */
+ * same 4-bit format; alpha * A.scale * B.scale has to be an fp32 number (it is, for alpha from 2^-62 to 2^63).
+ * (A matrix is its transpose with rows and cols exchanged and the other axis: the memory is the same.) */
 int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ldc, int out_f32, float alpha,
                  float beta, int relu, int sr_bits, unsigned long long seed, unsigned int rng_offset, void* stream);
 /* The same with A an m x k fp16 matrix (leading dimension lda) and B in mxfp8: the weight gradient of a

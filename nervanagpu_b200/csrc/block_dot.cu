@@ -15,6 +15,7 @@
 //   all        sum over the cluster, output stage (epilogue.cuh), stores
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "block_mma.cuh"
 #include "block_share.cuh"
@@ -299,6 +300,10 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   const int m = A->rows, n = B->cols;
   rc = check_output(C, ldc, n, sr_bits, out_f32);
   if (rc != NG_OK) return rc;
+  // The output stage multiplies once, with alpha times the operands' powers of two (themselves from 2^-64 to 2^64, 1 in mxfp4).
+  const float factor = alpha * (A->scale * B->scale);
+  if (std::isfinite(alpha) && static_cast<double>(factor) != static_cast<double>(alpha) * A->scale * B->scale)
+    return fail(NG_ERR_UNSUPPORTED, "alpha times the operands' scales is beyond the range of fp32: %g * %g * %g", alpha, A->scale, B->scale);
   DeviceCtx* c = current_ctx();
   if (!c) return NG_ERR_CUDA;
   BlockView a, b;
@@ -309,7 +314,7 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   const bool nv = A->format == NG_BLOCK_NVFP4;
   DotParams p = {};
   EpiArgs& ea = p.out.ea;
-  ea.alpha = nv ? alpha * a.t * b.t : alpha;     // (powers of two)
+  ea.alpha = factor;
   ea.beta = beta; ea.relu = relu; ea.sr_bits = sr_bits;
   ea.seed_lo = static_cast<uint32_t>(seed); ea.seed_hi = static_cast<uint32_t>(seed >> 32); ea.rng_offset = rng_offset;
   p.out.C = C; p.out.ldc = ldc; p.out.out_f32 = out_f32;
