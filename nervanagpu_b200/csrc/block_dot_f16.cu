@@ -363,8 +363,8 @@ int launch_mix(DeviceCtx* c, MixParams& p, int splits, cudaStream_t stream) {
 
 }  // namespace
 
-// Long sums: the record as fp16 rows in scratch memory, then the product of two fp16 matrices. False when there is no
-// room for them.
+// Long sums: the record as fp16 rows in scratch memory, then the product of two fp16 matrices. False, with nothing queued, when
+// there is no room for the copy or for what the product needs (parts of its sum, A's odd rows in order).
 static bool from_scratch(DeviceCtx* c, const void* A, int lda, const ng_block_desc& d, const BlockView& x, void* C, int m, int ldc,
                          int out_f32, const EpiArgs& ea, cudaStream_t stream, int& rc) {
   AuxClaim room;
@@ -374,13 +374,14 @@ static bool from_scratch(DeviceCtx* c, const void* A, int lda, const ng_block_de
     cudaGetLastError();
     return false;
   }
-  rc = dequantize_f16(c, d, x, static_cast<__half*>(plain), ld, stream);
-  if (rc != NG_OK) return true;
   GemmCall g = {};
   g.A = A; g.B = plain; g.C = C; g.b_t = 1; g.m = m; g.n = x.outer; g.k = x.inner;
   g.lda = lda; g.ldb = ld; g.ldc = ldc; g.alpha = ea.alpha; g.beta = ea.beta; g.relu = ea.relu; g.sr_bits = ea.sr_bits;
   g.seed = static_cast<unsigned long long>(ea.seed_hi) << 32 | ea.seed_lo; g.rng_offset = ea.rng_offset;
   g.batch = 1; g.loops = 1; g.out_f32 = out_f32;
+  if (!reserve_gemm(c, g, stream)) return false;
+  rc = dequantize_f16(c, d, x, static_cast<__half*>(plain), ld, stream);
+  if (rc != NG_OK) return true;
   rc = run_gemm(g, stream);
   return true;
 }

@@ -181,51 +181,51 @@ bool tma_ok(const void* p, long long ld, long long zstride) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld & 7) == 0 && (zstride & 7) == 0;
 }
 
-}  // namespace
-
-int run_gemm(const GemmCall& call, cudaStream_t stream) {
-  GemmCall g = call;
+int check_gemm(const GemmCall& g) {
   if (!g.A || !g.B || !g.C) return fail(NG_ERR_INVALID_ARG, "null operand");
   if (g.m <= 0 || g.n <= 0 || g.k <= 0) return fail(NG_ERR_INVALID_ARG, "m, n, k must be positive");
   if (g.a_t && g.b_t) return fail(NG_ERR_UNSUPPORTED, "op 'tt' is not supported");
   if (g.sr_bits < 0 || g.sr_bits > 10) return fail(NG_ERR_INVALID_ARG, "stochastic rounding keeps 1..10 mantissa bits");
   const long long min_lda = g.a_t ? g.m : g.k, min_ldb = g.b_t ? g.k : g.n;
   if (g.lda < min_lda || g.ldb < min_ldb || g.ldc < g.n) return fail(NG_ERR_INVALID_ARG, "leading dimension too small");
-  DeviceCtx* c = current_ctx();
-  if (!c) return NG_ERR_CUDA;
+  return NG_OK;
+}
 
+// How a product runs: what run_gemm decides before it touches the device.
+struct GemmPlan {
   EpiArgs ea;
+  bool sum = false;                       // over the batch
+  int nza = 1, nzb = 1;                   // batch entries of the operands
+  PackArgs packA = {}, packB = {};        // operands to be packed (total > 0)
+  bool by_rule = false;                   // on the CUDA cores because that is shorter
+  bool on_tc = false;                     // on the tensor cores, with the fields below
+  TcParams p = {};
+  TcOperandLayout lay;
+  int bn_cta = 0;
+  size_t off = 0, bytesA = 0, room = 0;   // scratch memory: partial sums, packed A behind them, all of it
+};
+
+int plan_gemm(const DeviceCtx* c, const GemmCall& g, GemmPlan& plan) {
+  EpiArgs& ea = plan.ea;
   ea.alpha = g.alpha; ea.beta = g.beta; ea.relu = g.relu; ea.sr_bits = g.sr_bits;
   ea.seed_lo = static_cast<uint32_t>(g.seed); ea.seed_hi = static_cast<uint32_t>(g.seed >> 32);
   ea.rng_offset = g.rng_offset;
 
   // one batch dimension per operand: independent products, or products summed into one output
-  const bool sum = g.loops > 1;
+  const bool sum = plan.sum = g.loops > 1;
   const long long zsa = sum ? g.alz : g.az, zsb = sum ? g.blz : g.bz;
-  const int nza = zsa == 0 ? 1 : (sum ? g.loops : g.batch), nzb = zsb == 0 ? 1 : (sum ? g.loops : g.batch);
-  PackArgs packA = {}, packB = {};
+  const int nza = plan.nza = zsa == 0 ? 1 : (sum ? g.loops : g.batch), nzb = plan.nzb = zsb == 0 ? 1 : (sum ? g.loops : g.batch);
+  PackArgs &packA = plan.packA, &packB = plan.packB;
   bool use_tc = !g.force_simt && !(sum && g.batch > 1);
   if (use_tc && !tma_ok(g.A, g.lda, zsa))
     use_tc = plan_pack(packA, g.A, g.lda, zsa, nza, g.a_t ? g.k : g.m, g.a_t ? g.m : g.k);
   if (use_tc && !tma_ok(g.B, g.ldb, zsb))
     use_tc = plan_pack(packB, g.B, g.ldb, zsb, nzb, g.b_t ? g.n : g.k, g.b_t ? g.k : g.n);
-  const bool by_rule = use_tc && (packA.total || packB.total) && shorter_unpacked(c, g);
-  auto cuda_cores = [&](bool counted) -> int {
-    SimtGemmArgs s;
-    s.A = static_cast<const __half*>(g.A); s.B = static_cast<const __half*>(g.B); s.C = g.C;
-    s.a_t = g.a_t; s.b_t = g.b_t; s.m = g.m; s.n = g.n; s.k = g.k;
-    s.lda = g.lda; s.ldb = g.ldb; s.ldc = g.ldc;
-    s.az = g.az; s.bz = g.bz; s.cz = g.cz; s.loops = g.loops; s.alz = g.alz; s.blz = g.blz;
-    s.out_f32 = g.out_f32; s.ea = ea;
-    dim3 grid((g.n + 63) / 64, (g.m + 63) / 64, g.batch);
-    if (counted) count_fallback_launch();
-    gemm_simt_kernel<<<grid, 256, 0, stream>>>(s);
-    NG_CHECK_LAUNCH();
-    return NG_OK;
-  };
-  if (!use_tc || by_rule) return cuda_cores(!by_rule);
+  plan.by_rule = use_tc && (packA.total || packB.total) && shorter_unpacked(c, g);
+  plan.on_tc = use_tc && !plan.by_rule;
+  if (!plan.on_tc) return NG_OK;
 
-  TcParams p = {};
+  TcParams& p = plan.p;
   p.mode = TC_GEMM;
   p.block_n = g.n <= 64 ? 64 : (g.n <= 128 ? 128 : 256);
   p.M = g.m; p.N = g.n;
@@ -242,8 +242,8 @@ int run_gemm(const GemmCall& call, cudaStream_t stream) {
     p.m_halves = 1;
     p.tiles_m = (g.m + 2 * kTileM - 1) / (2 * kTileM);
   }
-  const int bn_cta = p.pair ? p.block_n / 2 : p.block_n;
-  TcOperandLayout lay;
+  const int bn_cta = plan.bn_cta = p.pair ? p.block_n / 2 : p.block_n;
+  TcOperandLayout& lay = plan.lay;
   lay.a_mn_major = g.a_t ? 1 : 0;   // stored k x m: m contiguous
   lay.b_mn_major = g.b_t ? 0 : 1;   // stored k x n: n contiguous
   lay.kb_rows = kChunk;
@@ -272,10 +272,52 @@ int run_gemm(const GemmCall& call, cudaStream_t stream) {
     p.n_store = g.n;
     p.N = (g.n + 7) & ~7;
   }
-  size_t off = p.splits > 1 ? static_cast<size_t>(p.splits) * p.nz * p.M * p.N * sizeof(float) : 0;
+  size_t& off = plan.off;
+  off = p.splits > 1 ? static_cast<size_t>(p.splits) * p.nz * p.M * p.N * sizeof(float) : 0;
   off = (off + 255) & ~size_t(255);
-  const size_t bytesA = (static_cast<size_t>(packA.total) * 16 + 255) & ~size_t(255);
-  const size_t room_bytes = off + bytesA + static_cast<size_t>(packB.total) * 16;
+  plan.bytesA = (static_cast<size_t>(packA.total) * 16 + 255) & ~size_t(255);
+  plan.room = off + plan.bytesA + static_cast<size_t>(packB.total) * 16;
+  return NG_OK;
+}
+
+}  // namespace
+
+bool reserve_gemm(DeviceCtx* c, const GemmCall& call, cudaStream_t stream) {
+  GemmPlan plan;
+  return check_gemm(call) == NG_OK && plan_gemm(c, call, plan) == NG_OK && plan.on_tc && (plan.room == 0 || scratch_or_none(c, stream, plan.room));
+}
+
+int run_gemm(const GemmCall& call, cudaStream_t stream) {
+  GemmCall g = call;
+  int rc = check_gemm(g);
+  if (rc != NG_OK) return rc;
+  DeviceCtx* c = current_ctx();
+  if (!c) return NG_ERR_CUDA;
+  GemmPlan plan;
+  rc = plan_gemm(c, g, plan);
+  if (rc != NG_OK) return rc;
+  const EpiArgs& ea = plan.ea;
+  const bool sum = plan.sum;
+  const int nza = plan.nza, nzb = plan.nzb, bn_cta = plan.bn_cta;
+  PackArgs &packA = plan.packA, &packB = plan.packB;
+  TcParams& p = plan.p;
+  const TcOperandLayout& lay = plan.lay;
+  const size_t off = plan.off, bytesA = plan.bytesA, room_bytes = plan.room;
+  auto cuda_cores = [&](bool counted) -> int {
+    SimtGemmArgs s;
+    s.A = static_cast<const __half*>(g.A); s.B = static_cast<const __half*>(g.B); s.C = g.C;
+    s.a_t = g.a_t; s.b_t = g.b_t; s.m = g.m; s.n = g.n; s.k = g.k;
+    s.lda = g.lda; s.ldb = g.ldb; s.ldc = g.ldc;
+    s.az = g.az; s.bz = g.bz; s.cz = g.cz; s.loops = g.loops; s.alz = g.alz; s.blz = g.blz;
+    s.out_f32 = g.out_f32; s.ea = ea;
+    dim3 grid((g.n + 63) / 64, (g.m + 63) / 64, g.batch);
+    if (counted) count_fallback_launch();
+    gemm_simt_kernel<<<grid, 256, 0, stream>>>(s);
+    NG_CHECK_LAUNCH();
+    return NG_OK;
+  };
+  if (!plan.on_tc) return cuda_cores(!plan.by_rule);
+
   // (without room, the kernel that needs none)
   if ((packA.total || packB.total || sum) && room_bytes > 0 && !scratch_or_none(c, stream, room_bytes)) return cuda_cores(true);
   if (packA.total || packB.total) {

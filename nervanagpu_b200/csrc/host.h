@@ -161,5 +161,7 @@ struct GemmCall {
   int long_kb;               // > 0: partitions of no more k-blocks than this, in up to two waves (shorter_partitions)
 };
 int run_gemm(const GemmCall& g, cudaStream_t stream);
+// Whether run_gemm will run this call on the tensor cores, for a caller that has another form: makes room for its scratch memory.
+bool reserve_gemm(DeviceCtx* c, const GemmCall& g, cudaStream_t stream);
 
 }  // namespace ngb
