@@ -22,6 +22,7 @@ struct DeviceCtx {
   struct Scratch {
     float* ptr = nullptr;
     size_t bytes = 0;
+    size_t refused = 0, refused_free = 0;   // a size that the device had no memory for, and what was free then
   };
   std::map<cudaStream_t, Scratch> scratch;
   // second buffer per stream, for operands that a call re-lays-out before it hands them to another

@@ -111,28 +111,48 @@ DeviceCtx* current_ctx() {
   return c;
 }
 
-// grows one scratch buffer to at least `bytes`
+// Grows one scratch buffer to at least `bytes`. A buffer that cannot grow stays as it is.
 static int grow_scratch(DeviceCtx* c, DeviceCtx::Scratch& s, size_t bytes) {
-  if (bytes > s.bytes) {
-    if (c->capturing) {
-      return fail(NG_ERR_UNSUPPORTED,
-                  "the workspace would have to grow during a capture: run the sequence once before recording it");
-    }
-    // growing: earlier launches may still read the old buffer, and so does every replay of a
-    // recorded sequence that was recorded with it
-    NG_CUDA(cudaDeviceSynchronize());
-    if (s.ptr) {
-      if (c->live_graphs > 0) c->retired.push_back(s.ptr);
-      else NG_CUDA(cudaFree(s.ptr));
-    }
-    s.ptr = nullptr;
-    s.bytes = 0;
-    size_t want = bytes + (bytes >> 2);
-    want = (want + (1u << 20) - 1) & ~((size_t(1) << 20) - 1);
-    NG_CUDA(cudaMalloc(&s.ptr, want));
-    s.bytes = want;
+  if (bytes <= s.bytes) return NG_OK;
+  if (c->capturing) {
+    return fail(NG_ERR_UNSUPPORTED,
+                "the workspace would have to grow during a capture: run the sequence once before recording it");
   }
-  return NG_OK;
+  // what the device has refused is not asked for again while no more memory is free: a try waits for all launches
+  size_t free_bytes = 0, total = 0;
+  if (s.refused > 0 && bytes >= s.refused && cudaMemGetInfo(&free_bytes, &total) == cudaSuccess && free_bytes <= s.refused_free)
+    return fail(NG_ERR_CUDA, "no device memory for a workspace of %zu bytes", bytes);
+  size_t want = bytes + (bytes >> 2);
+  want = (want + (1u << 20) - 1) & ~((size_t(1) << 20) - 1);
+  float* fresh = nullptr;
+  cudaError_t e = cudaMalloc(&fresh, want);
+  // earlier launches may still read the old buffer, and so does every replay of a recorded sequence that was
+  // recorded with it
+  if (s.ptr && (e == cudaSuccess || c->live_graphs == 0)) {
+    if (c->live_graphs > 0) {
+      c->retired.push_back(s.ptr);
+    } else {
+      NG_CUDA(cudaDeviceSynchronize());
+      NG_CUDA(cudaFree(s.ptr));
+      if (e != cudaSuccess) {       // not beside the old one: in its place
+        cudaGetLastError();
+        e = cudaMalloc(&fresh, want);
+        if (e != cudaSuccess && cudaMalloc(&fresh, s.bytes) == cudaSuccess) want = s.bytes;      // (and as it was)
+      }
+    }
+  }
+  if (fresh || c->live_graphs == 0) {
+    s.ptr = fresh;
+    s.bytes = fresh ? want : 0;
+  }
+  if (e == cudaSuccess) {
+    s.refused = 0;
+    return NG_OK;
+  }
+  cudaGetLastError();
+  s.refused = bytes;
+  if (cudaMemGetInfo(&s.refused_free, &total) != cudaSuccess) s.refused = 0;
+  return cuda_fail(e, "workspace allocation");
 }
 
 int ensure_workspace(DeviceCtx* c, cudaStream_t stream, size_t bytes) {
