@@ -52,6 +52,11 @@ class Layer(object):
             self.fprop_out = shared[0].share(self.dimO)
             shared.reverse()
         self.act_stats = self.lib.empty((self.dimO2[0], 1), dtype=np.float32)
+        self.init_blocks()
+
+    def init_blocks(self):
+        """What the layer keeps in blocks: part of init_activations, and called by itself for a layer whose output is part of
+        a container's (Inception)."""
         if self.checkpoint:
             self.record = self.lib.block_empty(self.dimI2, "mxfp8")
 
@@ -236,8 +241,8 @@ class FullLayer(Layer):
         self.dimF = self.dimF2 = (nOut, nIn)
         self.sizeI, self.sizeO, self.sizeF = nIn * N, nOut * N, nIn * nOut
 
-    def init_activations(self, shared=None):
-        super(FullLayer, self).init_activations(shared)
+    def init_blocks(self):
+        super(FullLayer, self).init_blocks()
         if self.products:
             ws, xs = self.scales if self.products == "nvfp4" else (1.0, 1.0)
             self.weight_blocks = self.lib.block_empty(self.dimF, self.products, axis=1, scale=ws)
@@ -358,8 +363,8 @@ class ConvLayer(Layer):
         self.mask_below()
         return self.bprop_out
 
-    def init_activations(self, shared=None):
-        super(ConvLayer, self).init_activations(shared)
+    def init_blocks(self):
+        super(ConvLayer, self).init_blocks()
         if self.checkpoint and self.restored is None:
             self.init_restored()
 
@@ -504,6 +509,7 @@ class Inception(Layer):
             last = part[-1]
             last.fprop_out = self.fprop_out[k0:k0 + last.K]
             last.act_stats = self.lib.empty((last.dimO2[0], 1), dtype=np.float32)
+            last.init_blocks()
             k0 += last.K
 
     def init_deltas(self, shared=None):
