@@ -569,6 +569,8 @@ def link_records(layers):
     Returns, for each layer, whether its output is not needed any more once the layer above has run (the backward pass
     of a pooling layer reads its input, not its output): these outputs can share buffers (init_activations(shared))."""
     released = [False] * len(layers)
+    for layer in layers:        # (as it is now: the chain may have been linked before, with other records)
+        layer.masks_below = layer.masked_above = False
     for i in range(len(layers) - 1):
         below, above = layers[i], layers[i + 1]
         if not above.checkpoint:
