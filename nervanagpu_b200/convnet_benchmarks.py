@@ -134,7 +134,10 @@ def build_network(ng, confs, dtype=np.float16, zeros=False, seed=0, checkpoint=F
             layer.init_restored(shared_inputs)
     rng = np.random.RandomState(seed)
     for i, layer in enumerate(layers):
-        layer.init_activations(shared_acts if released[i] else None)
+        if released[i]:
+            layer.init_activations(shared_acts)
+        else:
+            layer.init_activations()        # (a class of the user's own may take no argument)
         layer.init_weights(shared=shared_updates, zeros=zeros, rng=rng)
         if i > 1:
             layer.init_deltas(shared=shared_deltas)
