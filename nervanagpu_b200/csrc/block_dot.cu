@@ -50,6 +50,7 @@ struct DotTile {
   static constexpr uint32_t kSmem = kStages * kStageBytes + kParts + kDotCtrl + 1024u;
   // (this CTA's tile takes the ring's place when its products are done; the others' parts of its share have their own)
   static_assert(kParts <= kStages * kStageBytes, "the ring is smaller than the tile");
+  static_assert(kSmem > kDotSmemLimit / 2, "an SM takes two CTAs: dot_room() asks for one instance only");
 };
 
 struct DotParams {
@@ -256,17 +257,11 @@ int check_output(const void* C, int ldc, int n, int sr_bits, int out_f32) {
 
 }  // namespace
 
-// CTAs that run at the same time in clusters of 2^log: larger ones leave SMs of their GPCs over (132 in clusters of 4, 120
-// in clusters of 8; 2048 x 128 x 2048 as 128 CTAs in clusters of 8 took two rounds, 12.0 us).
-int cluster_room(const DeviceCtx* c, int log) {
-  static std::atomic<int> known[64][4];
-  int n = known[c->device][log].load(std::memory_order_relaxed);
-  if (n > 0) return n;
-  using T = DotTile<128, true>;
+int cluster_room(const DeviceCtx* c, const void* kernel, int threads, uint32_t smem, int log) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(c->sm_count >> log << log));
-  cfg.blockDim = dim3(kDotThreads);
-  cfg.dynamicSmemBytes = T::kSmem;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1u << log;
@@ -275,11 +270,20 @@ int cluster_room(const DeviceCtx* c, int log) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int clusters = 0;
-  if (cudaFuncSetAttribute(block_dot_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&clusters, block_dot_kernel<128, true>, &cfg) != cudaSuccess)
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess)
     cudaGetLastError();
-  n = std::max(1, clusters << log);
-  known[c->device][log].store(n, std::memory_order_relaxed);
+  return std::max(1, clusters << log);
+}
+
+// Of this kernel, asked once per device and cluster size. (All its instances take an SM each.)
+static int dot_room(const DeviceCtx* c, int log) {
+  static std::atomic<int> known[64][4];
+  int n = known[c->device][log].load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = cluster_room(c, reinterpret_cast<const void*>(block_dot_kernel<128, true>), kDotThreads, DotTile<128, true>::kSmem, log);
+    known[c->device][log].store(n, std::memory_order_relaxed);
+  }
   return n;
 }
 
@@ -336,7 +340,7 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   const long long tiles = static_cast<long long>(p.tiles_m) * ((p.out.N + cols - 1) / cols);
   int splits = 1;
   double here = 0.0;
-  for (int s = 1, log = 0; s <= 8 && (s == 1 || (p.num_kb >= s && tiles * s <= cluster_room(c, log))); s *= 2, ++log) {
+  for (int s = 1, log = 0; s <= 8 && (s == 1 || (p.num_kb >= s && tiles * s <= dot_room(c, log))); s *= 2, ++log) {
     const double kb = (20480.0 + 128.0 * cols) * 7.4e-6, out = 0.5 + cols / 128.0;
     const double us = 4.5 + (tiles * s + c->sm_count - 1) / c->sm_count * (kb * ((p.num_kb + s - 1) / s) + out / s) +
                       (s > 1 ? 1.0 + 512.0 * cols * (s - 1) / s * 3.3e-5 : 0.0);

@@ -45,6 +45,7 @@ struct MixTile {
   static constexpr int kStages = kRoom < 6 ? kRoom : 6;
   static constexpr uint32_t kSmem = kStages * kSlot + kMixRaw * kRaw + kOut + kMixCtrl + 1024u;
   static_assert(!kSplit || kOut <= kStages * kSlot, "the ring is smaller than the tile");
+  static_assert(kSmem > kMixSmemLimit / 2, "an SM takes two CTAs: mix_room() asks for one instance only");
   static constexpr uint32_t kCols = 2 * kN;               // of tensor memory: two accumulators
   static constexpr int kEpiCols = kN > 64 ? kN / 2 : 64;  // columns of an output-stage warp (64: one of the two has them all)
 };
@@ -363,6 +364,17 @@ int launch_mix(DeviceCtx* c, MixParams& p, int splits, cudaStream_t stream) {
 
 }  // namespace
 
+// CTAs of a split product that run at the same time, asked once per device and cluster size.
+static int mix_room(const DeviceCtx* c, int log) {
+  static std::atomic<int> known[64][4];
+  int n = known[c->device][log].load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = cluster_room(c, reinterpret_cast<const void*>(block_dot_f16_kernel<128, kMixSplit>), kMixThreads, MixTile<128, true>::kSmem, log);
+    known[c->device][log].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 // Long sums: the record as fp16 rows in scratch memory, then the product of two fp16 matrices. False, with nothing queued, when
 // there is no room for the copy or for what the product needs (parts of its sum, A's odd rows in order).
 static bool from_scratch(DeviceCtx* c, const void* A, int lda, const ng_block_desc& d, const BlockView& x, void* C, int m, int ldc,
@@ -425,7 +437,7 @@ int run_block_dot_f16(DeviceCtx* c, const void* A, int lda, const ng_block_desc&
   for (int n = 64; n <= 128; n *= 2)
     for (int log = 1; log <= 3; ++log) {
       const int s = 1 << log;
-      if (p.num_kb < s || row_tiles * ((p.N + n - 1ll) / n) * s > cluster_room(c, log)) break;
+      if (p.num_kb < s || row_tiles * ((p.N + n - 1ll) / n) * s > mix_room(c, log)) break;
       const double us = 3.6 + (p.num_kb + s - 1) / s * kblock(n) + 1.0 + 512.0 * n * (s - 1) / s * 3.3e-5 + 1.0 / s;
       if (us < here) {
         here = us;

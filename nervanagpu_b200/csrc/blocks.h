@@ -20,8 +20,9 @@ int plain_map(CUtensorMap* map, const void* base, long long rows, long long cols
 // Output stage of a product: its parameters, the boxes it stores, and whether its lean form will do.
 OutParams make_out(void* C, int m, int n, int ldc, int out_f32, const EpiArgs& ea);
 int out_map(CUtensorMap* map, const OutParams& out);
-// CTAs with an SM each that run at the same time in clusters of 2^log.
-int cluster_room(const DeviceCtx* c, int log);
+// CTAs of a kernel that run at the same time in clusters of 2^log: larger clusters leave SMs of their GPCs over (132 of 148 in
+// clusters of 4, 120 in clusters of 8; 2048 x 128 x 2048 as 128 CTAs in clusters of 8 took two rounds, 12.0 us).
+int cluster_room(const DeviceCtx* c, const void* kernel, int threads, uint32_t smem, int log);
 // The product of block_dot_pair.cu: two 4-bit matrices of more than 64 outer rows each.
 int run_block_dot_pair(DeviceCtx* c, const BlockView& a, const BlockView& b, bool nv, const OutParams& out, cudaStream_t stream);
 // The product of block_dot_f16.cu, from checked operands.
