@@ -123,13 +123,17 @@ def build_network(ng, confs, dtype=np.float16, zeros=False, seed=0, checkpoint=F
     shared_deltas = [ng.empty(deltas.dimI, dtype=deltas.dtype), ng.empty(deltas.dimI, dtype=deltas.dtype)]
     shared_updates = ng.empty(widest.dimF, dtype=np.float32)
     released = link_records(layers)
-    shared_acts = shared_inputs = None
-    if any(released):
-        largest = max((l for l, r in zip(layers, released) if r), key=lambda l: l.sizeO)
-        shared_acts = [ng.empty(largest.dimO, dtype=largest.dtype), ng.empty(largest.dimO, dtype=largest.dtype)]
+    # outputs that are needed no more once the layer above has run take turns in two buffers, each as large as its largest
+    turns = [l for l, r in zip(layers, released) if r]
+    largest = [max(turns[i::2], key=lambda l: l.sizeO) for i in range(min(2, len(turns)))]
+    shared_acts = [ng.empty(l.dimO, dtype=l.dtype) for l in largest]
     recorded = [l for l in layers if l.checkpoint and isinstance(l, ConvLayer)]
     if recorded:
-        shared_inputs = ng.empty(max(recorded, key=lambda l: l.sizeI).dimI, dtype=dtype)
+        # what is restored in the backward pass goes where one of these was: they have been read by then
+        widest_in = max(recorded, key=lambda l: l.sizeI)
+        shared_inputs = max(shared_acts, key=lambda t: t.size, default=None)
+        if shared_inputs is None or shared_inputs.size < widest_in.sizeI:
+            shared_inputs = ng.empty(widest_in.dimI, dtype=dtype)
         for layer in recorded:
             layer.init_restored(shared_inputs)
     rng = np.random.RandomState(seed)
