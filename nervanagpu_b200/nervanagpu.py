@@ -819,6 +819,9 @@ class NervanaGPU(object):
         the same 4-bit format, or A a plain fp16 matrix and B in "mxfp8". C is fp16 or fp32 with contiguous rows;
         sums are taken in fp32. relu and stochastic_round as in dot.
 
+        An "mxfp8" operand counts as fp16 numbers: exact where it was made from such; made from fp32, values beyond
+        65504 count as that and those below 2^-14 in fewer bits.
+
         With X a layer's input (features x images): block_dot(W, X4, Y, relu=True) is its forward product from 4-bit
         weights and inputs, block_dot(E, X8.T, dW) its weight gradient from the input's 8-bit record."""
         if repeat == 1 and not self.bench and _native.block_dot(self, A, B, C, alpha, beta, relu, stochastic_round):
