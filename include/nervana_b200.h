@@ -96,7 +96,8 @@ int ng_fallback_launch_count(unsigned long long* count);
  * offsets; ng_launch_count counts the kernels of every replay. A recording also keeps the
  * library's scratch pointers of its calls: if a later, larger call on the same stream makes the
  * scratch grow, the old buffer stays allocated until the last recording is destroyed
- * (ng_graph_destroy), so replays stay valid. */
+ * (ng_graph_destroy), so replays stay valid. Recordings made on one stream share its scratch memory:
+ * replay them in turn, not on two streams at the same time. */
 int ng_graph_capture_begin(void* stream);
 int ng_graph_capture_end(void* stream, void** graph);
 int ng_graph_launch(void* graph, void* stream);
@@ -258,7 +259,7 @@ typedef struct ng_block_desc {
 
 int ng_block_bytes(const ng_block_desc* desc, size_t* codes_bytes, size_t* scales_bytes);
 /* Every element of A (rows x cols, fp16 or fp32, element (r, c) at r * row_stride + c * col_stride elements) into
- * the n_outs (1 to 4) matrices in blocks, all of A's shape. */
+ * the n_outs (1 to 4) matrices in blocks, all of A's shape: one call, one launch for each, which reads A. */
 int ng_block_quantize(const void* A, int dtype_bytes, long long row_stride, long long col_stride,
                       const ng_block_desc* outs, int n_outs, void* stream);
 /* The values that the codes stand for; rounded to fp16 where dtype_bytes is 2, and limited to the type's
@@ -276,7 +277,12 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
                  float beta, int relu, int sr_bits, unsigned long long seed, unsigned int rng_offset, void* stream);
 /* The same with A an m x k fp16 matrix (leading dimension lda) and B in mxfp8: the weight gradient of a
  * fully-connected layer, from its deltas and the 8-bit record of its input. The record's values are taken as
- * fp16, limited to +-65504; all others are exact when the record was made from fp16 numbers. */
+ * fp16, limited to +-65504; all others are exact when the record was made from fp16 numbers, and those of a record of
+ * fp32 numbers are rounded to fp16 (once) where they lie below 2^-14.
+ * Long sums take an fp16 copy of the record in scratch memory of the stream (2.5 bytes per number, kept for the next such
+ * call); where there is no room for it, as in a recording that would have to grow it, another form runs. The forms
+ * add up in different orders: a call gives the same bits each time with the same room, and may differ in the last bits
+ * between a live call and a recorded one. */
 int ng_block_dot_f16(const void* A, int lda, const ng_block_desc* B, void* C, int m, int ldc, int out_f32, float alpha,
                      float beta, int relu, int sr_bits, unsigned long long seed, unsigned int rng_offset,
                      void* stream);

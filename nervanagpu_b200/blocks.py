@@ -24,8 +24,9 @@ class BlockTensor(object):
     """A (rows, cols) matrix in blocks along `axis` (1: along its rows, 0: down its columns).
 
     Products sum over the blocked axis, so the left operand of block_dot has axis 1 and the right one axis 0.
-    `scale` (nvfp4 only) is the matrix's power of two: block scales hold max|block| / (6 * scale) in 8 bits, from
-    2^-9 to 448, so it should bring most blocks' max / 6 near 1 (2^-32 to 2^32). `.T` is a view of the same memory with the other
+    `scale` (nvfp4 only) is the matrix's power of two, 2^-32 to 2^32: block scales hold max|block| / (6 * scale) in 8 bits,
+    from 2^-9 to 448, so it should bring most blocks' max / 6 near 1. Numbers beyond 2688 * scale are limited to that,
+    without a word; nothing here measures the matrix. `.T` is a view of the same memory with the other
     axis. codes and scales are uint8 tensors (the padding between rows stays zero) that a program may save and
     set again."""
 

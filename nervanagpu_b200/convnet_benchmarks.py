@@ -9,8 +9,9 @@ alternating layers, the initial weights are scaled so that activations stay near
 iterations of fprop over all layers and bprop (deltas, weight update and SGD step, in reverse) are
 timed with events. Output lines have the reference's form ("Avg(10) fprop: ... msecs ... gflops"),
 flops per layer from Layer.flops with the backward pass counted twice. --checkpoint keeps the inputs of
-convolutions and fully-connected layers as 8-bit records for the backward pass and lets their fp16 forms share two
-buffers; --products takes the fully-connected layers' forward products from 4-bit blocks.
+the chain's convolutions and fully-connected layers (not of those inside an Inception, nor of the first, whose input is
+data) as 8-bit records for the backward pass and lets their fp16 forms share two buffers; --products takes the
+fully-connected layers' forward products from 4-bit blocks.
 
 Networks: the convolution/pooling/fully-connected stacks of AlexNet (one-column variant), Overfeat
 (fast), VGG model A and VGG model E as the public convnet-benchmarks lists them, and GoogLeNet (v1,

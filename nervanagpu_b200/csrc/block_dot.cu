@@ -307,7 +307,8 @@ int ng_block_dot(const ng_block_desc* A, const ng_block_desc* B, void* C, int ld
   // The output stage multiplies once, with alpha times the operands' powers of two (themselves from 2^-64 to 2^64, 1 in mxfp4).
   const float factor = alpha * (A->scale * B->scale);
   if (std::isfinite(alpha) && static_cast<double>(factor) != static_cast<double>(alpha) * A->scale * B->scale)
-    return fail(NG_ERR_UNSUPPORTED, "alpha times the operands' scales is beyond the range of fp32: %g * %g * %g", alpha, A->scale, B->scale);
+    return fail(NG_ERR_UNSUPPORTED, "alpha times the operands' scales is beyond the range of fp32: %g * %g * %g", alpha, A->scale,
+                B->scale);
   DeviceCtx* c = current_ctx();
   if (!c) return NG_ERR_CUDA;
   BlockView a, b;

@@ -369,7 +369,8 @@ static int mix_room(const DeviceCtx* c, int log) {
   static std::atomic<int> known[64][4];
   int n = known[c->device][log].load(std::memory_order_relaxed);
   if (n == 0) {
-    n = cluster_room(c, reinterpret_cast<const void*>(block_dot_f16_kernel<128, kMixSplit>), kMixThreads, MixTile<128, true>::kSmem, log);
+    n = cluster_room(c, reinterpret_cast<const void*>(block_dot_f16_kernel<128, kMixSplit>), kMixThreads,
+                     MixTile<128, true>::kSmem, log);
     known[c->device][log].store(n, std::memory_order_relaxed);
   }
   return n;

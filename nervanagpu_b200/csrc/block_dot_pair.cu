@@ -4,10 +4,10 @@
 // cannot take them in that fast (366 ns measured, 150 bytes/ns). Two SMs on one tile of 256 x 256 share B: each
 // holds 128 rows of A, half of B's columns and the scales, 38 KB per k-block. The first CTA's thread issues the MMAs for
 // both; the copies of both CTAs are counted on its barriers (which TMA does for pairs, and plain bulk copies do not:
-// with those, the second CTA passed the news on, which took 0.6 us per k-block as a release). CTAs stay on the device and take tile after
-// tile. The accumulator and the scales leave no room for a second accumulator in tensor memory, so that a tile's
-// output stage first takes the accumulator to registers, rounded to fp16, and the next tile's products start while it
-// is stored.
+// with those, the second CTA passed the news on, which took 0.6 us per k-block as a release). CTAs stay on the device and
+// take tile after tile. The accumulator and the scales leave no room for a second accumulator in tensor memory, so that a
+// tile's output stage first takes the accumulator to registers, rounded to fp16, and the next tile's products start while
+// it is stored.
 //
 //   warp 0      producer, of this CTA's operands
 //   warp 1      scale copies and MMAs of both, in the first CTA

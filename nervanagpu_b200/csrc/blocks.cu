@@ -2,8 +2,10 @@
 // (the formats and the layout are described in blocks.cuh).
 //
 // All three move each number once and are bound by that: a quantisation reads 2 or 4 bytes per number and writes
-// half a byte or one, plus a scale per block. Two forms each, by how the blocks lie in the plain matrix:
-//   rows      neighbours of a block are neighbours in memory: a lane takes 16 of them, two share a block of 32
+// half a byte or one, plus a scale per block. (A call with several outputs is a launch for each, which reads A.) Two forms
+// each, by how the blocks lie in the plain matrix:
+//   rows      neighbours of a block are neighbours in memory: a lane takes 16 of them, two share a block of 32, or (a
+//             quantisation from fp16 to 4 bits) 32
 //   strided   a thread takes whole blocks, lanes run along the other axis, which is then the contiguous one (the
 //             usual case: a layer's inputs, features x images, in blocks of features); any strides
 #include <algorithm>
@@ -417,8 +419,9 @@ __global__ void __launch_bounds__(256) relu_mask_rows_kernel(BlockView q, PlainV
 // A CTA takes 64 outer rows x 4 blocks: half a tile of 4-bit scales, and 32 to 128 neighbouring bytes of codes per outer
 // row, so that a quantisation leaves in whole sectors through shared memory. A warp has one block, a lane two outer
 // rows: neighbours, in one access, where the outer axis is the contiguous one in aligned pairs (a quantisation
-// from fp16: at any address; words put together for the way back were slower than numbers, 16.8 to 13.9 us); else 32 apart, one by one. (Four rows per lane were faster for large matrices by 5 % and took 6.7 us instead of 2.9 for a
-// minibatch of 9216 x 128, with too few warps to hide their latency.)
+// from fp16: at any address; words put together for the way back were slower than numbers, 16.8 to 13.9 us); else 32 apart,
+// one by one. (Four rows per lane were faster for large matrices by 5 % and took 6.7 us instead of 2.9 for a minibatch of
+// 9216 x 128, with too few warps to hide their latency.)
 constexpr int kStridedThreads = 128;
 constexpr int kStridedRows = 64;
 
@@ -877,7 +880,7 @@ int ng_block_quantize(const void* A, int dtype_bytes, long long row_stride, long
                       const ng_block_desc* outs, int n_outs, void* stream) {
   if (!A || !outs) return fail(NG_ERR_INVALID_ARG, "null operand");
   if (dtype_bytes != 2 && dtype_bytes != 4) return fail(NG_ERR_UNSUPPORTED, "matrices in blocks are made from fp16 and fp32");
-  if (n_outs < 1 || n_outs > 4) return fail(NG_ERR_INVALID_ARG, "1 to 4 matrices in blocks from one pass");
+  if (n_outs < 1 || n_outs > 4) return fail(NG_ERR_INVALID_ARG, "1 to 4 matrices in blocks from one call");
   for (int i = 0; i < n_outs; ++i) {
     const int rc = check_shape(outs + i);
     if (rc != NG_OK) return rc;

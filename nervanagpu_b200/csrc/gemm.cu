@@ -284,7 +284,8 @@ int plan_gemm(const DeviceCtx* c, const GemmCall& g, GemmPlan& plan) {
 
 bool reserve_gemm(DeviceCtx* c, const GemmCall& call, cudaStream_t stream) {
   GemmPlan plan;
-  return check_gemm(call) == NG_OK && plan_gemm(c, call, plan) == NG_OK && plan.on_tc && (plan.room == 0 || scratch_or_none(c, stream, plan.room));
+  if (check_gemm(call) != NG_OK || plan_gemm(c, call, plan) != NG_OK || !plan.on_tc) return false;
+  return plan.room == 0 || scratch_or_none(c, stream, plan.room);
 }
 
 int run_gemm(const GemmCall& call, cudaStream_t stream) {

@@ -96,7 +96,8 @@ class Layer(object):
     def record_input(self, fprop_in, *operands):
         """Quantise the input into this layer's 8-bit record, for its backward pass, and into any operands of its
         product, in one call. With a record, a layer needs its input no more after its forward pass: the weight
-        gradient is taken from the record, and so is the mask of the ReLU below. (An extension: the reference keeps
+        gradient is taken from the record, and so is the mask of the ReLU below (link_records; a subclass with a bprop of
+        its own ends it with mask_below). (An extension: the reference keeps
         every activation in fp16, nervanagpu/layers.py:64-70.)"""
         outs = list(operands)
         if self.checkpoint:
@@ -223,8 +224,10 @@ class DataLayer(Layer):
 
 class FullLayer(Layer):
     """products: "mxfp4" or "nvfp4" for a forward product from weights and inputs in 4-bit blocks (block_dot); the
-    backward pass multiplies with the fp16 weights. scales: the powers of two of nvfp4 weights and inputs. The weights are
-    quantised in every forward pass, as they change in every step, or once by fix_weights, for inference.
+    backward pass multiplies with the fp16 weights. scales: the powers of two of nvfp4 weights and inputs; numbers beyond 2688
+    times them are limited to that (weights to 2.6 and inputs to 672 as it stands). The weights are quantised in every
+    forward pass, as they change in every step, or once by fix_weights, for inference. That is what it is for: 9216 ->
+    4096, 128 images, 9.7 us with fixed weights, 25.0 without, 22.4 in fp16.
     checkpoint: keep the input as an 8-bit record for the backward pass (see Layer.record_input)."""
 
     def __init__(self, lib, dtype, N, nIn, nOut, products=None, scales=(2.0 ** -10, 2.0 ** -2), checkpoint=False):
@@ -567,7 +570,8 @@ def link_records(layers):
     """For a chain of layers some of which keep 8-bit records of their inputs: such a layer masks the deltas that it
     passes to a convolution or fully-connected layer below by that layer's ReLU, which then does not do it itself.
     Returns, for each layer, whether its output is not needed any more once the layer above has run (the backward pass
-    of a pooling layer reads its input, not its output): these outputs can share buffers (init_activations(shared))."""
+    of a pooling layer reads its input, not its output): these outputs can share buffers (init_activations(shared)).
+    Layers inside an Inception are not part of the chain."""
     released = [False] * len(layers)
     for layer in layers:        # (as it is now: the chain may have been linked before, with other records)
         layer.masks_below = layer.masked_above = False

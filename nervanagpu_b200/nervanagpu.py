@@ -480,7 +480,8 @@ class NervanaGPU(object):
         """Record the device work `fn()` queues on `self.stream` (which must be a stream from
         new_stream, not the default one) and return a RecordedSequence whose launch() replays it
         with one host call. `fn` must have run once before with the same tensors, so that scratch
-        memory has its final size and generated kernels exist. No pycuda-era counterpart: the
+        memory has its final size and generated kernels exist. Recordings made on one stream share its scratch memory:
+        replay them in turn, not on two streams at the same time. No pycuda-era counterpart: the
         reference launches every kernel from Python (nervanagpu/nervanagpu.py:705-729)."""
         _lib.check(self.lib.ng_graph_capture_begin(self.stream))
         graph = ctypes.c_void_p()
@@ -780,8 +781,8 @@ class NervanaGPU(object):
 
     def quantize(self, A, *outs):
         """The numbers of A (fp16 or fp32, any strides), to nearest, into each of up to four matrices in blocks, of
-        any formats and axes: a layer's input as an operand of its product and as the record of its backward pass, say.
-        A block that holds an infinity or NaN reads back as NaN."""
+        any formats and axes: a layer's input as an operand of its product and as the record of its backward pass, say
+        (one launch for each, which reads A). A block that holds an infinity or NaN reads back as NaN."""
         if _native.quantize(self, A, outs):
             return outs[0] if len(outs) == 1 else outs
         assert 1 <= len(outs) <= 4, "one to four matrices in blocks"
@@ -820,7 +821,9 @@ class NervanaGPU(object):
         sums are taken in fp32. relu and stochastic_round as in dot.
 
         An "mxfp8" operand counts as fp16 numbers: exact where it was made from such; made from fp32, values beyond
-        65504 count as that and those below 2^-14 in fewer bits.
+        65504 count as that and those below 2^-14 in fewer bits. Long sums with one use scratch memory where there is
+        room, and another order of adding up where there is none (a recording that would have to grow it): a recorded call
+        may differ from a live one in the last bits, repeats of either do not.
 
         With X a layer's input (features x images): block_dot(W, X4, Y, relu=True) is its forward product from 4-bit
         weights and inputs, block_dot(E, X8.T, dW) its weight gradient from the input's 8-bit record."""
