@@ -573,14 +573,9 @@ def link_records(layers):
     of a pooling layer reads its input, not its output): these outputs can share buffers (init_activations(shared)).
     Layers inside an Inception are not part of the chain."""
     released = [False] * len(layers)
-    for layer in layers:        # (as it is now: the chain may have been linked before, with other records)
-        layer.masks_below = layer.masked_above = False
     for i in range(len(layers) - 1):
         below, above = layers[i], layers[i + 1]
-        if not above.checkpoint:
-            continue
-        relu = type(below) in (ConvLayer, FullLayer)
-        if relu:
-            above.masks_below = below.masked_above = True
-        released[i] = relu or type(below) is PoolLayer
+        # (set either way: the chain may have been linked before, with other records)
+        above.masks_below = below.masked_above = above.checkpoint and type(below) in (ConvLayer, FullLayer)
+        released[i] = above.masks_below or (above.checkpoint and type(below) is PoolLayer)
     return released
